@@ -46,6 +46,8 @@ typedef enum talos_status {
 } talos_status;
 
 enum { TALOS_F32 = 0, TALOS_Q4_0 = 2, TALOS_Q8_0 = 8, TALOS_Q6_K = 14 };
+/* Further element types of the device operators' arrays (ggml tags). */
+enum { TALOS_F16 = 1, TALOS_BF16 = 30 };
 
 /* Model hyper-parameters: the fields of `Config` (src/model/config.rs:14-25) as
  * fixed-width C types (usize -> uint32_t); a binding copies them by name. */
@@ -395,6 +397,88 @@ talos_status talos_matvec_dev_noalloc(const talos_weight* w, const float* x_dev,
  */
 talos_status talos_matvec_bench(const talos_weight* const* ws, int n, const float* x_dev,
                                 float* y_dev, int reps, float* us_per_launch);
+
+/* ------------------------------------------------------------ batch operators
+ *
+ * Device operators for many sequences that start from one prompt. Pointers named
+ * *_dev and those inside the argument structs' "device" fields are device
+ * pointers on CUDA device `device`; the work is enqueued on `stream`
+ * (cudaStream_t as void*, NULL = legacy default stream) and not waited for, the
+ * caller's current device is left as it was, nothing is allocated, and the calls
+ * can be captured into a CUDA graph.
+ */
+
+/*
+ * The choice of a token per row of logits, with one given random number each:
+ * sample (src/sample.rs:19-76) on the GPU, with min-p besides. In the order of
+ * descending logit (equal logits: the lower index first):
+ *   w_i = exp((logit_i - max) / temperature)
+ *   top_k > 0:  keep the first top_k                          (0: all)
+ *   top_p < 1:  of these the shortest prefix with weight >= top_p * their weight
+ *               (at least one; >= 1: all)
+ *   min_p > 0:  of these the ones with w_i >= min_p (min_p above 1 acts as 1)
+ *   the token is the first whose cumulative weight exceeds u * (kept weight).
+ * temperature <= 0 (or NaN) takes the first of the order, as top_k = 1 does:
+ * where several logits are exactly equal, talos_argmax takes the last index and
+ * this the first. NaN logits count as -inf; -inf is never chosen, and +inf
+ * shares the whole weight with the other +inf. A row with nothing above -inf
+ * gives token -1 and probability 0. u outside [0, 1) is clamped (NaN: 0).
+ * Sums are exact to 2^-43 of the largest weight and do not depend on any order,
+ * so a call gives the same tokens every time. probs (optional): the weight of
+ * the token over the kept weight.
+ */
+typedef struct talos_sample_args {
+    int device;
+    int type;            /* TALOS_F32, TALOS_F16 or TALOS_BF16 */
+    uint32_t n, vocab;   /* rows; logits per row, 1 .. 1,048,576 */
+    const void* logits;  /* device, [n] rows */
+    size_t row_stride;   /* elements between rows, >= vocab if n > 1 */
+    const float* u;      /* device, [n] */
+    /* device, [n] each, or NULL: the value below for every row */
+    const float* temperature_dev;
+    const int32_t* top_k_dev;
+    const float* top_p_dev;
+    const float* min_p_dev;
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+    int32_t* tokens; /* device, [n] */
+    float* probs;    /* device, [n], or NULL */
+} talos_sample_args;
+talos_status talos_sample_dev(const talos_sample_args* args, void* stream);
+
+/*
+ * The same for one row of n host logits on the current CUDA device, beside
+ * talos_argmax: *index_out is the token; prob_out may be NULL. A row with
+ * nothing above -inf fails with TALOS_ERR_INVALID_ARG.
+ */
+talos_status talos_sample(const float* logits, size_t n, float u, float temperature, int32_t top_k, float top_p,
+                          float min_p, uint32_t* index_out, float* prob_out);
+
+/*
+ * Move rows between cache slots: for every i, rows [start, start + len) of slot
+ * src become those rows of slot dst, in each of the n_base arrays (K and V,
+ * say) and each of the n_outer planes (layers). The moves are simultaneous:
+ * every one reads what the slots held before the call, whatever the order
+ * (compaction, permutations, one slot to many). Rows outside the ranges keep
+ * their values. A slot may be the destination of one move only (INVALID_ARG
+ * otherwise); src == dst or len == 0 does nothing. At most 512 moves. The
+ * geometry must not make rows overlap (INVALID_ARG). No reference counterpart
+ * (the reference keeps one sequence, src/kv_cache.rs:7-52).
+ */
+typedef struct talos_kv_slots {
+    int device;
+    int n_base;         /* arrays, 1 .. 8 */
+    void* const* base;  /* host array of device pointers */
+    uint32_t n_slots, n_outer, n_rows;
+    size_t slot_stride, outer_stride, row_stride; /* bytes */
+    size_t row_bytes;
+} talos_kv_slots;
+typedef struct talos_kv_copy {
+    uint32_t src, dst, start, len;
+} talos_kv_copy;
+talos_status talos_kv_move_dev(const talos_kv_slots* slots, const talos_kv_copy* moves, size_t n, void* stream);
 
 #ifdef __cplusplus
 }

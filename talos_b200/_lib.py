@@ -30,6 +30,24 @@ class Cfg(C.Structure):
         "rope_dim")] + [("rms_eps", C.c_float), ("rope_freq_base", C.c_float)]
 
 
+class SampleArgs(C.Structure):
+    """``talos_sample_args``."""
+
+    _fields_ = [("device", C.c_int), ("type", C.c_int), ("n", C.c_uint32), ("vocab", C.c_uint32),
+                ("logits", C.c_void_p), ("row_stride", C.c_size_t), ("u", C.c_void_p),
+                ("temperature_dev", C.c_void_p), ("top_k_dev", C.c_void_p), ("top_p_dev", C.c_void_p),
+                ("min_p_dev", C.c_void_p), ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
+
+
+class KvSlots(C.Structure):
+    """``talos_kv_slots``."""
+
+    _fields_ = [("device", C.c_int), ("n_base", C.c_int), ("base", C.c_void_p), ("n_slots", C.c_uint32),
+                ("n_outer", C.c_uint32), ("n_rows", C.c_uint32), ("slot_stride", C.c_size_t),
+                ("outer_stride", C.c_size_t), ("row_stride", C.c_size_t), ("row_bytes", C.c_size_t)]
+
+
 # Every symbol include/talos_cuda.h declares, with its ctypes signature.
 _vp, _sz, _u32, _i = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int
 SIGNATURES = {
@@ -63,6 +81,10 @@ SIGNATURES = {
     "talos_profile_phases": (_i, [_vp, _u32, _sz, _vp, _sz, C.POINTER(_i), C.POINTER(_i)]),
     "talos_dequant": (_i, [_i, _vp, _sz, _vp]),
     "talos_argmax": (_i, [_vp, _sz, C.POINTER(C.c_uint32)]),
+    "talos_sample": (_i, [_vp, _sz, C.c_float, C.c_float, C.c_int32, C.c_float, C.c_float, C.POINTER(C.c_uint32),
+                          C.POINTER(C.c_float)]),
+    "talos_sample_dev": (_i, [C.POINTER(SampleArgs), _vp]),
+    "talos_kv_move_dev": (_i, [C.POINTER(KvSlots), _vp, _sz, _vp]),
     "talos_matvec": (_i, [_i, _i, _vp, _sz, _sz, _sz, _vp, _vp]),
     "talos_matvec_resident": (_i, [_vp, C.c_char_p, _i, _vp, _sz, _sz, _sz, _vp, _vp]),
     "talos_weight_create": (_i, [_i, _i, _vp, _sz, _sz, _sz, C.POINTER(_vp)]),

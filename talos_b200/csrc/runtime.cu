@@ -30,6 +30,7 @@
 
 #include "../../include/talos_cuda.h"
 #include "kernels.cuh"
+#include "status.cuh"
 
 using namespace talos;
 
@@ -70,7 +71,7 @@ static const NcclApi& nccl() {
 
 static thread_local std::string g_last_error;
 
-static talos_status set_err(talos_status st, const char* fmt, ...) {
+talos_status talos::set_err(talos_status st, const char* fmt, ...) {
     char buf[768];
     va_list ap;
     va_start(ap, fmt);
@@ -79,21 +80,6 @@ static talos_status set_err(talos_status st, const char* fmt, ...) {
     g_last_error = buf;
     return st;
 }
-
-#define CK(call)                                                                                 \
-    do {                                                                                         \
-        cudaError_t e_ = (call);                                                                 \
-        if (e_ != cudaSuccess)                                                                   \
-            return set_err(e_ == cudaErrorMemoryAllocation ? TALOS_ERR_OOM : TALOS_ERR_CUDA,     \
-                           "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__,     \
-                           __LINE__);                                                            \
-    } while (0)
-
-#define TRY(call)                              \
-    do {                                       \
-        talos_status s_ = (call);              \
-        if (s_ != TALOS_OK) return s_;         \
-    } while (0)
 
 extern "C" const char* talos_last_error(void) { return g_last_error.c_str(); }
 
@@ -361,7 +347,7 @@ static talos_status device_setup(int device) {
     return TALOS_OK;
 }
 
-static int sm_count_dev(int device) {
+int talos::sm_count_dev(int device) {
     if (device >= 0 && device < 64 && g_sms[device]) return g_sms[device];
     int sms = 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return 148;

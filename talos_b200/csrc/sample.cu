@@ -1,0 +1,571 @@
+// sample.cu -- the choice of a token from logits on B200 (sm_100a): temperature,
+// top-k, top-p and min-p with one given random number per row (the truncations
+// of Tsuskov/talos src/sample.rs:19-76, on the device).
+//
+// For a row of logits l with temperature T, in the order of descending logit
+// (equal logits: the lower index first; NaN counts as -inf):
+//   w_i = exp((l_i - max) / T), 0 for l_i = -inf
+//   keep the first k; of these the shortest prefix with sum w >= p * (their sum);
+//   of these the w_i >= m (the largest w is 1); W = sum of the kept w
+//   the token is the first whose cumulative w exceeds u * W.
+// All three truncations keep a prefix of the order, so each is known by its
+// cumulative weight, and the choice is one search for a cumulative weight.
+//
+// Exactness. An answer is a border between cumulative sums, so weights are
+// computed in f64 and summed as 64-bit integers in units of 2^-42: sums do not
+// depend on their order, and a weight is off by at most 2^-43 (a million weights
+// add up to less than 2^63).
+//
+// Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
+// shared memory, so the row is read from HBM once. No sort of the row: a
+// histogram over 1024 bins of (max - l) / T (1/32 nat each; beyond 32 nats the
+// weight is 0) counts and sums the weights per bin in shared memory, the leading
+// CTA adds the cluster's histograms through distributed shared memory, scans
+// them, and finds the bins of the borders. When the elements up to the first
+// truncating border are few (top-k, most top-p and min-p settings), they are
+// gathered, ranked and finished in one step; otherwise each border's bin is
+// gathered and ranked by itself. A bin that holds more elements than the list
+// (equal or nearly equal logits) is split further by the bits of the
+// (logit, index) key. The leading CTA drives; the others follow its commands.
+#include <cooperative_groups.h>
+
+#include "ops.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace talos {
+
+typedef unsigned long long u64;
+
+constexpr int SP_THREADS = 512;
+constexpr int SP_WARPS = SP_THREADS / 32;
+constexpr int SP_NB = 1024;       // bins; two per thread
+constexpr float SP_PER_NAT = 32;  // bins per nat
+constexpr int SP_CAP = 1024;      // elements of a ranked list; two per thread
+constexpr double SP_ONE = 4398046511104.0;  // 2^42
+constexpr int SP_SLICE = 16384;  // logits of a row that one CTA keeps
+constexpr int SP_IDX_BITS = 20;
+static_assert((1 << SP_IDX_BITS) == SAMPLE_MAX_VOCAB, "index bits");
+
+enum SpOp : int { SP_COUNT = 0, SP_WEIGH = 1, SP_GATHER_BINS = 2, SP_GATHER_KEYS = 3, SP_RANGE = 4, SP_SPLIT = 5,
+                  SP_SUM_MIN = 6, SP_DONE = 7 };
+struct SpCmd {
+    int op, b0, b1, shift;
+    u64 k0, k1;
+};
+
+struct SpSmem {
+    uint32_t cnt[SP_NB], wlo[SP_NB], whi[SP_NB];
+    u64 list[SP_CAP];  // gathered keys (leader)
+    u64 key[SP_CAP];   // ranked
+    u64 cum[SP_CAP];   // cumulative weights of the ranked list
+    float cmax[8];     // each CTA's maximum
+    SpCmd cmd;
+    uint32_t nlist;    // leader: gathered so far
+    u64 ra, rb;        // this CTA's SP_RANGE (smallest, largest key) or SP_SUM_MIN (sum)
+    u64 wa[SP_WARPS], wb[SP_WARPS];  // block scans
+    float fa[SP_WARPS];
+    // result of a search
+    uint32_t f_cnt, f_bin;
+    u64 f_bc, f_bw;
+    uint32_t keep;     // elements of the list with w >= min_p
+};
+
+__device__ __forceinline__ float sp_load(float v) { return isnan(v) ? -INFINITY : v + 0.0f; }  // -0 -> +0
+__device__ __forceinline__ float sp_load(__half v) { return sp_load(__half2float(v)); }
+__device__ __forceinline__ float sp_load(__nv_bfloat16 v) { return sp_load(__bfloat162float(v)); }
+
+// Position in the order: a smaller key comes first.
+__device__ __forceinline__ u64 sp_key(float v, uint32_t i) { return ((u64)~total_order_key(v) << SP_IDX_BITS) | i; }
+__device__ __forceinline__ float sp_key_value(u64 k) {
+    const uint32_t o = ~(uint32_t)(k >> SP_IDX_BITS);
+    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
+
+// w of value v as f64 (1 at the maximum, +inf included).
+__device__ __forceinline__ double sp_weight(float v, float vmax, double inv_t) {
+    return v == vmax ? 1.0 : exp(((double)v - (double)vmax) * inv_t);
+}
+__device__ __forceinline__ u64 sp_fixed(double w) { return (u64)__double2ll_rn(w * SP_ONE); }
+// Bin of value v, SP_NB for weight 0. Non-decreasing as v falls: every rounding here is monotone.
+__device__ __forceinline__ int sp_bin(float v, float vmax, float inv_t) {
+    if (v == vmax) return 0;
+    const float z = __fmul_rn(__fmul_rn(__fsub_rn(vmax, v), inv_t), SP_PER_NAT);
+    return z < (float)SP_NB ? (int)z : SP_NB;  // NaN (-inf * 0) gives SP_NB
+}
+
+// Exclusive block scan of (a, b); returns the totals through ta, tb.
+__device__ __forceinline__ void sp_scan(SpSmem& s, u64& a, u64& b, u64& ta, u64& tb) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 x = a, y = b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) x += p, y += q;
+    }
+    __syncthreads();
+    if (lane == 31) s.wa[warp] = x, s.wb[warp] = y;
+    __syncthreads();
+    u64 px = 0, py = 0;
+    ta = tb = 0;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) {
+        if (w == warp) px = ta, py = tb;
+        ta += s.wa[w], tb += s.wb[w];
+    }
+    a = px + x - a;
+    b = py + y - b;
+}
+
+// RES: the CTA's slice of the row stays in shared memory (up to SP_SLICE
+// logits as f32); otherwise every pass reads it again (vocabularies above
+// 8 x SP_SLICE). (In registers, 32 logits a thread, the f64 weights spilled.)
+template <typename T, bool RES, bool VEC>
+__global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant__ SampleArgs a, int slice) {
+    __shared__ SpSmem s;
+    extern __shared__ __align__(16) float vals[];  // RES: [slice]
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int row = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int VW = 16 / (int)sizeof(T);
+    SpSmem* lead = cluster.map_shared_rank(&s, 0);
+    const int i0 = min(a.vocab, rank * slice), n_own = min(a.vocab, i0 + slice) - i0;
+    const T* lg = (const T*)a.logits + (size_t)row * a.stride + i0;
+
+    float mx = -INFINITY;
+    if (VEC) {  // slice is a multiple of VW, so lg is 16-byte aligned
+#pragma unroll 4
+        for (int i = tid * VW; i < n_own; i += SP_THREADS * VW) {
+            float v[VW];
+            if (i + VW <= n_own) {
+                const uint4 q = ldg_stream_u4(lg + i);
+                const T* t = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int k = 0; k < VW; ++k) v[k] = sp_load(t[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VW; ++k) v[k] = i + k < n_own ? sp_load(lg[i + k]) : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < VW; ++k) mx = fmaxf(mx, v[k]);
+#pragma unroll
+            for (int k = 0; k < VW; k += 4)
+                if (RES) *(float4*)(vals + i + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        }
+    } else {
+#pragma unroll 8
+        for (int i = tid; i < n_own; i += SP_THREADS) {
+            const float v = sp_load(lg[i]);
+            if (RES) vals[i] = v;
+            mx = fmaxf(mx, v);
+        }
+    }
+    auto each = [&](auto&& f) {  // (after the barriers of the maximum)
+#pragma unroll 4
+        for (int i = tid; i < n_own; i += SP_THREADS) f(RES ? vals[i] : sp_load(lg[i]), (uint32_t)(i0 + i));
+    };
+
+    // settings of the row; T <= 0 (or NaN) is the greedy choice: the first of the order
+    float temp = a.temperature_dev ? a.temperature_dev[row] : a.temperature;
+    int topk = a.top_k_dev ? a.top_k_dev[row] : a.top_k;
+    const float topp = a.top_p_dev ? a.top_p_dev[row] : a.top_p;
+    float minp = a.min_p_dev ? a.min_p_dev[row] : a.min_p;
+    minp = minp > 0.f ? fminf(minp, 1.0f) : 0.f;  // NaN: off
+    if (!(temp > 0.f)) temp = 1.f, topk = 1;
+    const double inv_t = fmin(1.0 / (double)temp, 1e30);
+    const float inv_tf = (float)inv_t;
+
+    // the row's maximum
+    mx = warp_max(mx);
+    if (lane == 0) s.fa[warp] = mx;
+    __syncthreads();
+    if (tid < C) {
+        float m = s.fa[0];
+        for (int w = 1; w < SP_WARPS; ++w) m = fmaxf(m, s.fa[w]);
+        cluster.map_shared_rank(&s, tid)->cmax[rank] = m;
+    }
+    cluster.sync();
+    float vmax = s.cmax[0];
+    for (int c = 1; c < C; ++c) vmax = fmaxf(vmax, s.cmax[c]);
+    if (vmax == -INFINITY) {  // nothing to choose from; the whole cluster agrees
+        if (rank == 0 && tid == 0) {
+            a.tokens[row] = -1;
+            if (a.probs) a.probs[row] = 0.f;
+        }
+        return;
+    }
+
+    auto zero_hist = [&]() {
+        for (int b = tid; b < SP_NB; b += SP_THREADS) s.cnt[b] = 0, s.wlo[b] = 0, s.whi[b] = 0;
+        __syncthreads();
+    };
+    auto add_hist = [&](int b, u64 w) {
+        // 64-bit add as two 32-bit ones: the carry comes from the value that the low word had
+        const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.wlo[b], lo);
+        const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+        if (hi) atomicAdd(&s.whi[b], hi);
+    };
+    auto gather = [&](u64 k) {
+        const uint32_t at = atomicAdd(&lead->nlist, 1u);
+        if (at < SP_CAP) lead->list[at] = k;
+    };
+    // one command, by every CTA of the cluster
+    auto execute = [&](const SpCmd& c) {
+        switch (c.op) {
+            case SP_COUNT:
+            case SP_WEIGH:
+                zero_hist();
+                each([&](float v, uint32_t) {
+                    const int b = sp_bin(v, vmax, inv_tf);
+                    if (b < SP_NB) {
+                        atomicAdd(&s.cnt[b], 1u);
+                        if (c.op == SP_WEIGH) add_hist(b, sp_fixed(sp_weight(v, vmax, inv_t)));
+                    }
+                });
+                break;
+            case SP_GATHER_BINS:
+                each([&](float v, uint32_t i) {
+                    const int b = sp_bin(v, vmax, inv_tf);
+                    if (b >= c.b0 && b <= c.b1) gather(sp_key(v, i));
+                });
+                break;
+            case SP_GATHER_KEYS:
+                each([&](float v, uint32_t i) {
+                    const u64 k = sp_key(v, i);
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, inv_tf) < SP_NB) gather(k);
+                });
+                break;
+            case SP_RANGE: {
+                u64 lo = ~0ull, hi = 0ull;
+                each([&](float v, uint32_t i) {
+                    if (sp_bin(v, vmax, inv_tf) == c.b0) {
+                        const u64 k = sp_key(v, i);
+                        lo = k < lo ? k : lo;
+                        hi = k > hi ? k : hi;
+                    }
+                });
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const u64 p = __shfl_xor_sync(0xffffffffu, lo, o), q = __shfl_xor_sync(0xffffffffu, hi, o);
+                    lo = p < lo ? p : lo;
+                    hi = q > hi ? q : hi;
+                }
+                // (64-bit atomics in another CTA's shared memory lost updates: each CTA
+                // leaves its own result for the leader to read)
+                if (lane == 0) s.wa[warp] = lo, s.wb[warp] = hi;
+                __syncthreads();
+                if (tid == 0) {
+                    for (int w = 1; w < SP_WARPS; ++w) {
+                        lo = s.wa[w] < lo ? s.wa[w] : lo;
+                        hi = s.wb[w] > hi ? s.wb[w] : hi;
+                    }
+                    s.ra = lo, s.rb = hi;
+                }
+                break;
+            }
+            case SP_SPLIT:
+                zero_hist();
+                each([&](float v, uint32_t i) {
+                    const u64 k = sp_key(v, i);
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, inv_tf) < SP_NB) {
+                        const int b = (int)((k - c.k0) >> c.shift);
+                        atomicAdd(&s.cnt[b], 1u);
+                        add_hist(b, sp_fixed(sp_weight(v, vmax, inv_t)));
+                    }
+                });
+                break;
+            case SP_SUM_MIN: {
+                u64 sum = 0;
+                each([&](float v, uint32_t) {
+                    if (sp_bin(v, vmax, inv_tf) < SP_NB) {
+                        const double w = sp_weight(v, vmax, inv_t);
+                        if (w >= (double)minp) sum += sp_fixed(w);
+                    }
+                });
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0) s.wa[warp] = sum;
+                __syncthreads();
+                if (tid == 0) {
+                    for (int w = 1; w < SP_WARPS; ++w) sum += s.wa[w];
+                    s.ra = sum;
+                }
+                break;
+            }
+        }
+    };
+
+    // with a top-k that fits the list, counts alone find the candidates; the
+    // weights of all elements are only needed without one
+    const bool count_only = topk > 0 && topk <= SP_CAP / 2;
+    const SpCmd first{count_only ? SP_COUNT : SP_WEIGH, 0, 0, 0, 0, 0};
+    if (tid == 0) s.nlist = 0;
+    execute(first);
+    cluster.sync();
+    if (rank != 0) {
+        for (;;) {
+            cluster.sync();  // the leader has written this CTA's cmd
+            const SpCmd c = s.cmd;
+            if (c.op == SP_DONE) return;
+            execute(c);
+            cluster.sync();
+        }
+    }
+
+    // ---------------------------------------------------------- the leading CTA
+    auto step = [&](const SpCmd& c) {
+        __syncthreads();
+        if (tid < C) cluster.map_shared_rank(&s, tid)->cmd = c;
+        if (tid == 0) s.nlist = 0;
+        cluster.sync();
+        execute(c);
+        cluster.sync();
+    };
+    // the cluster's histogram: this thread's two bins and what lies before them
+    uint32_t c0, c1;
+    u64 w0, w1, bc, bw, tc, tw;
+    auto load_hist = [&]() {
+        c0 = c1 = 0;
+        w0 = w1 = 0;
+        for (int q = 0; q < C; ++q) {
+            const SpSmem* o = cluster.map_shared_rank(&s, q);
+            const uint2 n = *(const uint2*)&o->cnt[2 * tid], lo = *(const uint2*)&o->wlo[2 * tid],
+                        hi = *(const uint2*)&o->whi[2 * tid];
+            c0 += n.x, c1 += n.y;
+            w0 += ((u64)hi.x << 32) + lo.x, w1 += ((u64)hi.y << 32) + lo.y;
+        }
+        bc = (u64)c0 + c1, bw = w0 + w1;
+        sp_scan(s, bc, bw, tc, tw);
+    };
+    // first bin whose cumulative count (or weight), on top of (xc, xw), reaches x >= 1
+    auto find = [&](bool by_count, u64 x, u64 xc, u64 xw) {
+        __syncthreads();
+        if (tid == 0) s.f_bin = 0, s.f_cnt = 0, s.f_bc = xc, s.f_bw = xw;
+        __syncthreads();
+        const u64 b = by_count ? xc + bc : xw + bw, p = by_count ? (u64)c0 : w0, q = by_count ? (u64)c1 : w1;
+        if (b < x && x <= b + p) s.f_bin = 2 * tid, s.f_cnt = c0, s.f_bc = xc + bc, s.f_bw = xw + bw;
+        if (b + p < x && x <= b + p + q)
+            s.f_bin = 2 * tid + 1, s.f_cnt = c1, s.f_bc = xc + bc + c0, s.f_bw = xw + bw + w0;
+        __syncthreads();
+    };
+    // rank the gathered list (keys are unique) and sum its weights
+    auto rank_list = [&](int n) {
+        __syncthreads();
+        for (int i = tid; i < n; i += SP_THREADS) {
+            const u64 k = s.list[i];
+            int pos = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) pos += s.list[j] < k ? 1 : 0;
+            s.key[pos] = k;
+        }
+        if (tid == 0) s.keep = 0;
+        __syncthreads();
+        u64 x[2] = {0, 0};
+        uint32_t keep = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * tid + j;
+            if (i < n) {
+                const double w = sp_weight(sp_key_value(s.key[i]), vmax, inv_t);
+                x[j] = sp_fixed(w);
+                keep += !(w < (double)minp) ? 1u : 0u;
+            }
+        }
+        u64 ex = x[0] + x[1], dummy = 0, t1, t2;
+        sp_scan(s, ex, dummy, t1, t2);
+        if (2 * tid < n) s.cum[2 * tid] = ex + x[0];
+        if (2 * tid + 1 < n) s.cum[2 * tid + 1] = ex + x[0] + x[1];
+        if (keep) atomicAdd(&s.keep, keep);
+        __syncthreads();
+    };
+    // first of the ranked list with base + cum >= x (all threads get it)
+    auto list_find = [&](int n, u64 base, u64 x) {
+        int lo = 0, hi = n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (base + s.cum[mid] >= x) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    };
+    auto p_target = [&](u64 z) {  // smallest integer >= p * z, within 1 .. z
+        const double t = ceil((double)topp * (double)z);
+        return t < 1.0 ? 1ull : (t >= (double)z ? z : (u64)t);
+    };
+    auto draw_target = [&](u64 w) {  // first cumulative weight > u * W
+        const double t = floor((double)a.u[row] * (double)w);
+        const u64 x = t > 0.0 ? (t >= (double)w ? w - 1 : (u64)t) : 0ull;  // NaN: 0
+        return (x >= w ? w - 1 : x) + 1;
+    };
+    u64 chosen = 0, W = 0;
+    load_hist();
+    // the last bin that any truncation can keep
+    int bcut = SP_NB;
+    u64 ncut = tc;
+    const bool k_active = topk > 0 && (u64)topk < tc;
+    if (k_active) {
+        find(true, (u64)topk, 0, 0);
+        bcut = (int)s.f_bin, ncut = s.f_bc + s.f_cnt;
+    }
+    // (top-p is a share of the top-k's weight: with both, the list holds the whole top-k)
+    const bool sum_known = !k_active && !count_only;
+    if (minp > 0.f && (sum_known || !(topp < 1.f))) {
+        // w < m beyond bin -32 ln m; one bin more covers the roundings of both
+        const float zb = -logf(minp) * SP_PER_NAT + 2.0f;
+        const int b = zb < (float)(SP_NB - 1) ? (int)zb : SP_NB - 1;
+        if (b < bcut) {
+            __syncthreads();
+            if (tid == b / 2) s.f_bc = bc + c0 + (b & 1 ? c1 : 0);
+            __syncthreads();
+            if (s.f_bc < ncut) ncut = s.f_bc;
+            bcut = b;
+        }
+    }
+    if (topp < 1.f && sum_known) {
+        find(false, p_target(tw), 0, 0);
+        if ((int)s.f_bin < bcut) bcut = (int)s.f_bin, ncut = s.f_bc + s.f_cnt;
+    }
+    if (ncut <= SP_CAP) {
+        // everything that can be kept fits the list
+        const int n = (int)ncut;
+        step(SpCmd{SP_GATHER_BINS, 0, bcut < SP_NB ? bcut : SP_NB - 1, 0, 0, 0});
+        rank_list(n);
+        int keep = n;
+        u64 z = tw;  // weight under top-k
+        if (!sum_known) {
+            if (topk < keep) keep = topk;
+            z = s.cum[keep - 1];
+        }
+        if (topp < 1.f) {
+            const int j = list_find(n, 0, p_target(z)) + 1;
+            if (j < keep) keep = j;
+        }
+        if (minp > 0.f && (int)s.keep < keep) keep = (int)s.keep;
+        if (keep < 1) keep = 1;
+        W = s.cum[keep - 1];
+        const int j = list_find(n, 0, draw_target(W));
+        chosen = s.key[j];
+    } else {
+        if (count_only) {  // more equal logits at the border than the list holds
+            step(SpCmd{SP_WEIGH, 0, 0, 0, 0, 0});
+            load_hist();
+        }
+        const uint32_t hc0 = c0, hc1 = c1;
+        const u64 hw0 = w0, hw1 = w1, hbc = bc, hbw = bw, htw = tw;
+        // the element at cumulative count / weight x: its bin, then its place in
+        // the bin. Returns the cumulative weight up to and with it.
+        auto resolve = [&](bool by_count, u64 x) {
+            c0 = hc0, c1 = hc1, w0 = hw0, w1 = hw1, bc = hbc, bw = hbw;
+            find(by_count, x, 0, 0);
+            uint32_t n = s.f_cnt;
+            u64 xc = s.f_bc, xw = s.f_bw;
+            const int b = (int)s.f_bin;
+            if (n <= SP_CAP) {
+                step(SpCmd{SP_GATHER_BINS, b, b, 0, 0, 0});
+            } else {
+                step(SpCmd{SP_RANGE, b, b, 0, 0, 0});
+                u64 k0 = ~0ull, k1 = 0;
+                for (int q = 0; q < C; ++q) {
+                    const SpSmem* o = cluster.map_shared_rank(&s, q);
+                    k0 = o->ra < k0 ? o->ra : k0;
+                    k1 = o->rb > k1 ? o->rb : k1;
+                }
+                while (n > SP_CAP) {
+                    int shift = 0;
+                    while (((k1 - k0) >> shift) >= SP_NB) ++shift;
+                    step(SpCmd{SP_SPLIT, 0, 0, shift, k0, k1});
+                    load_hist();
+                    find(by_count, x, xc, xw);
+                    n = s.f_cnt, xc = s.f_bc, xw = s.f_bw;
+                    k0 += (u64)s.f_bin << shift;
+                    const u64 last = k0 + ((1ull << shift) - 1);
+                    k1 = last < k1 ? last : k1;
+                }
+                step(SpCmd{SP_GATHER_KEYS, 0, 0, 0, k0, k1});
+            }
+            rank_list((int)n);
+            const int j = by_count ? (int)(x - xc) - 1 : list_find((int)n, xw, x);
+            chosen = s.key[j];
+            const u64 cum = xw + s.cum[j];
+            __syncthreads();
+            return cum;
+        };
+        W = htw;
+        if (k_active) W = resolve(true, (u64)topk);
+        if (topp < 1.f) W = resolve(false, p_target(W));
+        if (minp > 0.f) {
+            step(SpCmd{SP_SUM_MIN, 0, 0, 0, 0, 0});
+            u64 sum = 0;
+            for (int q = 0; q < C; ++q) sum += cluster.map_shared_rank(&s, q)->ra;
+            if (sum < W) W = sum;
+        }
+        resolve(false, draw_target(W));
+    }
+    if (tid == 0) {
+        a.tokens[row] = (int32_t)(chosen & (SAMPLE_MAX_VOCAB - 1));
+        if (a.probs)
+            a.probs[row] = (float)(sp_weight(sp_key_value(chosen), vmax, inv_t) / ((double)W / SP_ONE));
+    }
+    __syncthreads();
+    if (tid < C) cluster.map_shared_rank(&s, tid)->cmd.op = SP_DONE;
+    cluster.sync();
+}
+
+template <typename T, bool RES, bool VEC>
+static cudaError_t launch_one(const SampleArgs& a, int C, int slice, cudaStream_t s) {
+    auto* k = k_sample<T, RES, VEC>;
+    const size_t smem = RES ? (size_t)slice * 4 : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.n * C);
+    cfg.blockDim = dim3(SP_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, a, slice);
+}
+
+template <typename T>
+static cudaError_t launch_type(const SampleArgs& a, int sms, cudaStream_t s) {
+    // CTAs per row: enough that a slice fits, then more (down to 4096 logits
+    // each) while all of them still run at once, two per SM
+    int C = 1;
+    while (C < 8 && (long)C * SP_SLICE < a.vocab) C *= 2;
+    while (C < 8 && (long)C * 4096 < a.vocab && 2L * C * a.n <= 2L * sms) C *= 2;
+    const int slice = ((a.vocab + C - 1) / C + 15) / 16 * 16;
+    const bool res = slice <= SP_SLICE;
+    const bool vec = ((uintptr_t)a.logits % 16 == 0) && (a.stride * sizeof(T)) % 16 == 0;
+    return res ? vec ? launch_one<T, true, true>(a, C, slice, s) : launch_one<T, true, false>(a, C, slice, s)
+               : vec ? launch_one<T, false, true>(a, C, slice, s) : launch_one<T, false, false>(a, C, slice, s);
+}
+
+// Opt-in shared memory of the current device's kernels (once per device).
+cudaError_t sample_configure() {
+    auto set = [](const void* k) {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_SLICE * 4);
+    };
+    const void* ks[] = {(const void*)k_sample<float, true, true>,         (const void*)k_sample<float, true, false>,
+                        (const void*)k_sample<__half, true, true>,        (const void*)k_sample<__half, true, false>,
+                        (const void*)k_sample<__nv_bfloat16, true, true>, (const void*)k_sample<__nv_bfloat16, true, false>};
+    for (const void* k : ks) {
+        const cudaError_t e = set(k);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_sample(const SampleArgs& a, int type, int sms, cudaStream_t s) {
+    switch (type) {
+        case DT_F32: return launch_type<float>(a, sms, s);
+        case DT_F16: return launch_type<__half>(a, sms, s);
+        case DT_BF16: return launch_type<__nv_bfloat16>(a, sms, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace talos

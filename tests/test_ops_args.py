@@ -1,0 +1,75 @@
+"""Arguments of the batch operators that are refused before any GPU work, and
+the plan of a call's moves (no GPU needed)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import talos_b200
+from talos_b200 import _lib, build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build_cuda()
+    return _lib.load()
+
+
+def sample_args(**kw):
+    a = _lib.SampleArgs(0, 0, 2, 100, 256, 100, 256)
+    a.tokens = 256
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_sample_refusals(lib):
+    assert lib.talos_sample_dev(None, None) == _lib.INVALID_ARG
+    assert lib.talos_sample_dev(C.byref(sample_args(n=0)), None) == _lib.OK
+    assert lib.talos_sample_dev(C.byref(sample_args(type=2)), None) == _lib.UNSUPPORTED
+    for kw in (dict(logits=None), dict(u=None), dict(tokens=None), dict(vocab=0), dict(vocab=(1 << 20) + 1),
+               dict(row_stride=99), dict(top_k=-1), dict(logits=258), dict(probs=1), dict(top_k_dev=2),
+               dict(n=(1 << 24) + 1)):
+        assert lib.talos_sample_dev(C.byref(sample_args(**kw)), None) == _lib.INVALID_ARG, kw
+    out, v = C.c_uint32(), np.zeros(4, np.float32)
+    assert lib.talos_sample(None, 4, 0.5, 1.0, 0, 1.0, 0.0, C.byref(out), None) == _lib.INVALID_ARG
+    assert lib.talos_sample(v.ctypes.data, 0, 0.5, 1.0, 0, 1.0, 0.0, C.byref(out), None) == _lib.INVALID_ARG
+    assert lib.talos_sample(v.ctypes.data, 4, 0.5, 1.0, -1, 1.0, 0.0, C.byref(out), None) == _lib.INVALID_ARG
+    assert lib.talos_sample(v.ctypes.data, 4, 0.5, 1.0, 0, 1.0, 0.0, None, None) == _lib.INVALID_ARG
+
+
+def move(lib, moves, n_slots=4, n_rows=8, bases=(256, 4096), **kw):
+    base = (C.c_void_p * max(len(bases), 1))(*bases)
+    g = _lib.KvSlots(0, len(bases), C.addressof(base), n_slots, 1, n_rows, 64 * n_rows, 64 * n_rows * n_slots, 64, 64)
+    for k, v in kw.items():
+        setattr(g, k, v)
+    m = (C.c_uint32 * (4 * len(moves)))(*[x for y in moves for x in y])
+    return lib.talos_kv_move_dev(C.byref(g), m, len(moves), None)
+
+
+def test_move_refusals(lib):
+    assert lib.talos_kv_move_dev(None, None, 0, None) == _lib.INVALID_ARG
+    assert move(lib, []) == _lib.OK
+    assert move(lib, [(1, 1, 0, 8), (0, 2, 3, 0)]) == _lib.OK  # nothing to do
+    for moves in ([(4, 0, 0, 1)], [(0, 4, 0, 1)], [(0, 1, 0, 9)], [(0, 1, 8, 1)], [(0, 1, 0xffffffff, 2)],
+                  [(0, 2, 0, 1), (1, 2, 4, 1)], [(0, 1, 0, 1)] * 513):
+        assert move(lib, moves) == _lib.INVALID_ARG, moves[:2]
+    one = [(0, 1, 0, 1)]
+    for kw in (dict(bases=()), dict(bases=(256, 256)), dict(bases=(256, 0)), dict(bases=tuple(range(256, 256 * 10, 256))),
+               dict(row_stride=63), dict(slot_stride=63 * 8), dict(row_bytes=0), dict(n_outer=0),
+               dict(n_outer=2, outer_stride=64), dict(base=None)):
+        assert move(lib, one, **kw) == _lib.INVALID_ARG, kw
+    m = (C.c_uint32 * 4)(0, 1, 0, 1)
+    base = (C.c_void_p * 1)(256)
+    g = _lib.KvSlots(0, 1, C.addressof(base), 4, 1, 8, 512, 2048, 64, 64)
+    assert lib.talos_kv_move_dev(C.byref(g), None, 1, None) == _lib.INVALID_ARG
+    assert lib.talos_kv_move_dev(C.byref(g), m, 0, None) == _lib.OK
+
+
+def test_python_checks_without_a_gpu():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(2, 5)
+    with pytest.raises(ValueError, match="CUDA"):
+        talos_b200.sample_dev(x, torch.zeros(2))
+    with pytest.raises(ValueError, match="CUDA"):
+        talos_b200.kv_move_dev([torch.zeros(2, 1, 4, 4)], [0], [1], [1])
