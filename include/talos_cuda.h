@@ -457,6 +457,52 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
                           float min_p, uint32_t* index_out, float* prob_out);
 
 /*
+ * Attention of n sequences over one shared prefix and a suffix of each one's own
+ * (a prompt that many sequences continue): for sequence i and query head h, with
+ * kv head h / (n_head / n_head_kv), the keys are prefix rows 0 .. prefix_len-1
+ * and rows 0 .. lens[i]-1 of cache slot slots[i];
+ *   out[i][h] = softmax(scale * q . K) V        (src/model/llama.rs:135-155)
+ * and zeros where there is no key at all. The prefix is read once for all
+ * sequences of a row tile (128 / (n_head / n_head_kv) of them) instead of once
+ * per sequence. Rows behind lens[i], and slots that no sequence names, are not
+ * read. Types (q and out, cache): F32 with F32 (the reference's cache) or F16,
+ * F16 with F16, BF16 with BF16; f32 queries get f32 accuracy on the tensor
+ * cores. head_dim up to 128, a multiple of 8 (4 where all is F32); n_head at
+ * most 128 times n_head_kv; n up to 1024. The last dimension is contiguous;
+ * strides are in elements; pointers and strides are multiples of 16 bytes. K
+ * and V share their strides. lens are clamped to 0 .. slot_len; a sequence
+ * whose slot is out of range has no suffix. Keys that are attended to hold
+ * finite values; one sequence's infinities or NaN do not reach another's output.
+ *
+ * work: talos_attention_shared_work bytes of device memory, 16-byte aligned,
+ * used by this call alone until it has run (two calls in flight, or two graphs
+ * that may run at once, need one each); its contents need not be kept or set.
+ * Every wait inside is bounded (2 s): rows of a CTA whose wait ran out are NaN.
+ * No reference counterpart (the reference decodes one sequence at a time).
+ */
+typedef struct talos_attention_shared_args {
+    int device;
+    int q_type, kv_type;
+    uint32_t n, n_head, n_head_kv, head_dim;
+    uint32_t prefix_len;          /* may be 0 */
+    uint32_t n_slots, slot_len;   /* the caches' slots and rows per slot */
+    const void* q;                /* device, [n][n_head][head_dim] */
+    size_t q_stride_n, q_stride_h;
+    const void *k_prefix, *v_prefix; /* device, [prefix_len][n_head_kv][head_dim] */
+    size_t prefix_stride_t, prefix_stride_h;
+    const void *k, *v;            /* device, [n_slots][slot_len][n_head_kv][head_dim] */
+    size_t slot_stride, slot_stride_t, slot_stride_h;
+    const int32_t* slots;         /* device, [n], or NULL: sequence i in slot i */
+    const int32_t* lens;          /* device, [n] */
+    void* out;                    /* device, [n][n_head][head_dim] */
+    size_t out_stride_n, out_stride_h;
+    float scale;                  /* usually 1 / sqrt(head_dim); 1e-30 .. 1e30 */
+} talos_attention_shared_args;
+talos_status talos_attention_shared_work(int device, uint32_t n, uint32_t n_head, uint32_t n_head_kv, size_t* out);
+talos_status talos_attention_shared_dev(const talos_attention_shared_args* args, void* work, size_t work_bytes,
+                                        void* stream);
+
+/*
  * Move rows between cache slots: for every i, rows [start, start + len) of slot
  * src become those rows of slot dst, in each of the n_base arrays (K and V,
  * say) and each of the n_outer planes (layers). The moves are simultaneous:

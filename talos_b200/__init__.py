@@ -6,13 +6,13 @@ Public API (mirrors Tsuskov/talos ``src/model`` for the CUDA backend):
     Model.generate_greedy / prefill
     Model.set_batch / forward_batch / prefill_slot / generate_batch_greedy  (batches)
     argmax, dequant, matvec, Weight   (single-kernel entry points)
-    sample, sample_dev, kv_move_dev   (batch operators; the *_dev ones on torch tensors)
+    attention_shared_dev, sample, sample_dev, kv_move_dev   (batch operators; the *_dev ones on torch tensors)
 The compute runs in libtalos_cuda.so through the C ABI of include/talos_cuda.h.
 """
 from .gguf import F32, Q4_0, Q6_K, Q8_0, GgufError, GgufFile, GgufWriter, TensorInfo
 from .model import Config, Context, Model, Weight, argmax, dequant, matvec, nccl_unique_id, weight_shapes
-from .ops import kv_move_dev, sample, sample_dev
+from .ops import attention_shared_dev, kv_move_dev, sample, sample_dev
 
 __all__ = ["F32", "Q4_0", "Q6_K", "Q8_0", "GgufError", "GgufFile", "GgufWriter", "TensorInfo", "Config",
-           "Context", "Model", "Weight", "argmax", "dequant", "kv_move_dev", "matvec", "nccl_unique_id", "sample", "sample_dev",
-           "weight_shapes"]
+           "Context", "Model", "Weight", "argmax", "attention_shared_dev", "dequant", "kv_move_dev", "matvec", "nccl_unique_id",
+           "sample", "sample_dev", "weight_shapes"]

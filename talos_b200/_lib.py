@@ -40,6 +40,20 @@ class SampleArgs(C.Structure):
                 ("min_p", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
 
 
+class AttentionSharedArgs(C.Structure):
+    """``talos_attention_shared_args``."""
+
+    _fields_ = ([("device", C.c_int), ("q_type", C.c_int), ("kv_type", C.c_int)]
+                + [(n, C.c_uint32) for n in ("n", "n_head", "n_head_kv", "head_dim", "prefix_len", "n_slots",
+                                             "slot_len")]
+                + [("q", C.c_void_p), ("q_stride_n", C.c_size_t), ("q_stride_h", C.c_size_t),
+                   ("k_prefix", C.c_void_p), ("v_prefix", C.c_void_p), ("prefix_stride_t", C.c_size_t),
+                   ("prefix_stride_h", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p),
+                   ("slot_stride", C.c_size_t), ("slot_stride_t", C.c_size_t), ("slot_stride_h", C.c_size_t),
+                   ("slots", C.c_void_p), ("lens", C.c_void_p), ("out", C.c_void_p), ("out_stride_n", C.c_size_t),
+                   ("out_stride_h", C.c_size_t), ("scale", C.c_float)])
+
+
 class KvSlots(C.Structure):
     """``talos_kv_slots``."""
 
@@ -84,6 +98,8 @@ SIGNATURES = {
     "talos_sample": (_i, [_vp, _sz, C.c_float, C.c_float, C.c_int32, C.c_float, C.c_float, C.POINTER(C.c_uint32),
                           C.POINTER(C.c_float)]),
     "talos_sample_dev": (_i, [C.POINTER(SampleArgs), _vp]),
+    "talos_attention_shared_work": (_i, [_i, _u32, _u32, _u32, C.POINTER(_sz)]),
+    "talos_attention_shared_dev": (_i, [C.POINTER(AttentionSharedArgs), _vp, _sz, _vp]),
     "talos_kv_move_dev": (_i, [C.POINTER(KvSlots), _vp, _sz, _vp]),
     "talos_matvec": (_i, [_i, _i, _vp, _sz, _sz, _sz, _vp, _vp]),
     "talos_matvec_resident": (_i, [_vp, C.c_char_p, _i, _vp, _sz, _sz, _sz, _vp, _vp]),

@@ -43,6 +43,7 @@ talos_status configured(int device) {
     std::lock_guard<std::mutex> lk(mu);
     if (done[device]) return TALOS_OK;
     CK(sample_configure());
+    CK(attn_shared_configure());
     done[device] = true;
     return TALOS_OK;
 }
@@ -116,6 +117,72 @@ extern "C" talos_status talos_sample(const float* logits, size_t n, float u, flo
     if (token < 0) return set_err(TALOS_ERR_INVALID_ARG, "no logit above -inf");
     *index_out = (uint32_t)token;
     if (prob_out) *prob_out = prob;
+    return TALOS_OK;
+}
+
+// ------------------------------------------------------------------ attention over a shared prefix
+
+extern "C" talos_status talos_attention_shared_work(int device, uint32_t n, uint32_t n_head, uint32_t n_head_kv,
+                                                    size_t* out) {
+    if (!out) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
+    if (!n || n > 1024) return set_err(TALOS_ERR_INVALID_ARG, "%u sequences (1 .. 1024)", n);
+    if (!n_head_kv || n_head % n_head_kv || !n_head || n_head / n_head_kv > 128)
+        return set_err(TALOS_ERR_INVALID_ARG, "%u heads over %u kv heads (a multiple, at most 128 times)", n_head,
+                       n_head_kv);
+    *out = attn_shared_work_bytes((int)n, (int)(n_head / n_head_kv), sm_count_dev(device));
+    return TALOS_OK;
+}
+
+extern "C" talos_status talos_attention_shared_dev(const talos_attention_shared_args* a, void* work, size_t work_bytes,
+                                                   void* stream) {
+    if (!a) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
+    if (!attn_shared_types(a->q_type, a->kv_type))
+        return set_err(TALOS_ERR_UNSUPPORTED, "queries of type %d with a cache of type %d", a->q_type, a->kv_type);
+    if (a->n == 0) return TALOS_OK;
+    size_t need = 0;
+    TRY(talos_attention_shared_work(a->device, a->n, a->n_head, a->n_head_kv, &need));
+    const int qs = dtype_bytes(a->q_type), ks = dtype_bytes(a->kv_type);
+    if (!a->head_dim || a->head_dim > 128 || a->head_dim % (qs == 4 && ks == 4 ? 4 : 8))
+        return set_err(TALOS_ERR_UNSUPPORTED, "head_dim %u (a multiple of 8, or of 4 with an f32 cache, up to 128)",
+                       a->head_dim);
+    if (!(a->scale >= 1e-30f && a->scale <= 1e30f)) return set_err(TALOS_ERR_INVALID_ARG, "scale %g", (double)a->scale);
+    if (!a->q || !a->out || !a->lens || !work) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
+    if ((a->prefix_len && (!a->k_prefix || !a->v_prefix)) || (a->n_slots && a->slot_len && (!a->k || !a->v)))
+        return set_err(TALOS_ERR_INVALID_ARG, "NULL cache");
+    if (work_bytes < need) return set_err(TALOS_ERR_INVALID_ARG, "workspace of %zu bytes, needs %zu", work_bytes, need);
+    if (a->n_slots > 0x7fffffffu || !a->n_slots)
+        return set_err(TALOS_ERR_INVALID_ARG, "%u slots", a->n_slots);
+    const uint64_t spt = 128 / (a->n_head / a->n_head_kv);
+    const uint64_t tiles = a->prefix_len / 64 + 1 + std::min<uint64_t>(a->n, spt) * (a->slot_len / 64 + 1ull);
+    if (tiles * a->n_head_kv > 0x3fffffffull || a->prefix_len > 0x3fffffffu || a->slot_len > 0x3fffffffu)
+        return set_err(TALOS_ERR_UNSUPPORTED, "prefix of %u and slots of %u positions", a->prefix_len, a->slot_len);
+    AttnSharedArgs k{};
+    // a dimension of one element (or none) has no stride to speak of
+    auto st = [](size_t stride, uint32_t count) { return count > 1 ? stride : 0; };
+    k.q_sn = st(a->q_stride_n, a->n), k.q_sh = st(a->q_stride_h, a->n_head);
+    k.out_sn = st(a->out_stride_n, a->n), k.out_sh = st(a->out_stride_h, a->n_head);
+    k.pre_st = st(a->prefix_stride_t, a->prefix_len);
+    k.pre_sh = a->prefix_len ? st(a->prefix_stride_h, a->n_head_kv) : 0;
+    if (a->slot_len) {
+        k.slot_ss = st(a->slot_stride, a->n_slots), k.slot_st = st(a->slot_stride_t, a->slot_len);
+        k.slot_sh = st(a->slot_stride_h, a->n_head_kv);
+    }
+    for (size_t x : {k.q_sn * qs, k.q_sh * qs, k.out_sn * qs, k.out_sh * qs, k.pre_st * ks, k.pre_sh * ks,
+                     k.slot_ss * ks, k.slot_st * ks, k.slot_sh * ks})
+        if (x % 16) return set_err(TALOS_ERR_INVALID_ARG, "a stride of %zu bytes (multiples of 16)", x);
+    for (const void* p : {a->q, (const void*)a->out, a->k_prefix, a->v_prefix, a->k, a->v, (const void*)work})
+        if (!aligned(p, 16)) return set_err(TALOS_ERR_INVALID_ARG, "a pointer is not 16-byte aligned");
+    if (!aligned(a->lens, 4) || !aligned(a->slots, 4))
+        return set_err(TALOS_ERR_INVALID_ARG, "a pointer is not aligned to its element");
+    OnDevice d(a->device);
+    TRY(on_device(d, a->device));
+    TRY(configured(a->device));
+    k.q = a->q, k.kp = a->k_prefix, k.vp = a->v_prefix, k.k = a->k, k.v = a->v, k.out = a->out;
+    k.n = (int)a->n, k.n_kv = (int)a->n_head_kv, k.group = (int)(a->n_head / a->n_head_kv), k.hd = (int)a->head_dim;
+    k.prefix = (int)a->prefix_len, k.n_slots = (int)a->n_slots, k.slot_len = (int)a->slot_len;
+    k.lens = a->lens, k.slots = a->slots;
+    k.scale = a->scale;
+    CK(launch_attn_shared(k, a->q_type, a->kv_type, work, sm_count_dev(a->device), (cudaStream_t)stream));
     return TALOS_OK;
 }
 

@@ -54,4 +54,42 @@ constexpr uint32_t MOVE_TMP = 0xffffffffu;
 // are the instructions of component c (components touch disjoint slots).
 cudaError_t launch_kv_move(const MoveGeom& g, const MoveIns* ins, const uint32_t* comp, int n_comp, cudaStream_t s);
 
+// ---------------------------------------------------------------- attention over a shared prefix
+
+struct AttnSharedArgs {
+    // element strides: s*n sequences, *h heads, *t positions, *s slots
+    const void* q;
+    size_t q_sn, q_sh;
+    const void *kp, *vp;  // prefix
+    size_t pre_st, pre_sh;
+    const void *k, *v;    // the sequences' slots
+    size_t slot_ss, slot_st, slot_sh;
+    void* out;
+    size_t out_sn, out_sh;
+    int n, n_kv, group, hd;
+    int prefix, n_slots, slot_len;
+    const int32_t* lens;   // suffix rows of each sequence
+    const int32_t* slots;  // its slot (null: sequence i in slot i)
+    float scale;
+    // batched steps: the sequence count and the prefix length in device memory (n and
+    // prefix are then their largest values), positions instead of lengths (the
+    // suffix has pos + 1 - prefix rows), suffix rows stored from row `prefix` of
+    // the slot (slot_row0 = 1), error bits for a wait that ran out
+    const int* n_dev;
+    const uint32_t* prefix_dev;
+    const uint32_t* pos;
+    int slot_row0;
+    uint32_t* error;
+    // set by launch_attn_shared
+    int whole;
+    float4* part_ml;
+    float* part_o;
+    int* plan;
+};
+bool attn_shared_types(int q_type, int kv_type);
+cudaError_t attn_shared_configure();  // once per device, on the current one
+size_t attn_shared_work_bytes(int n, int group, int sms);
+// group <= 128, hd <= 128; work: attn_shared_work_bytes, 16-byte aligned
+cudaError_t launch_attn_shared(AttnSharedArgs a, int q_type, int kv_type, void* work, int sms, cudaStream_t s);
+
 }  // namespace talos

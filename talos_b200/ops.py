@@ -1,6 +1,7 @@
 """Device operators for many sequences that start from one prompt, on torch CUDA
-tensors: the choice of tokens (``sample_dev``) and moves of rows between cache
-slots (``kv_move_dev``).
+tensors: attention over a prefix that they share (``attention_shared_dev``), the
+choice of tokens (``sample_dev``) and moves of rows between cache slots
+(``kv_move_dev``).
 
 Each call checks its tensors, enqueues the work on the tensors' device (on the
 current stream there unless ``stream`` gives a cudaStream_t) and returns without
@@ -27,7 +28,7 @@ class _Torch:
 
         self.torch = torch
         self.tag = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-        self.f32, self.i32 = torch.float32, torch.int32
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
         self.lib = _lib.load()
 
 
@@ -54,6 +55,61 @@ def _vector(T: _Torch, t, name: str, n: int, dtype, dev: int) -> int:
         raise ValueError(f"{name} must be a contiguous [{n}] {dtype} tensor on cuda:{dev}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
+
+
+_work_bytes: dict[tuple[int, int, int, int], int] = {}  # of talos_attention_shared_work
+
+
+def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, scale=None, stream=None):
+    """talos_attention_shared_dev: attention of n sequences over a prefix they share
+    and a suffix of each one's own. ``q`` [n, n_head, head_dim]; ``k_prefix`` /
+    ``v_prefix`` [prefix, n_head_kv, head_dim] (prefix 0: an empty tensor); ``k`` /
+    ``v`` [n_slots, rows, n_head_kv, head_dim], of which sequence i attends to rows
+    0 .. lens[i] - 1 of slot slots[i] (``slots`` None: slot i); ``slots`` and
+    ``lens`` int32 on the device. f32 queries go with f32 or f16 caches, f16 and
+    bf16 with their own; the last dimension is contiguous. ``scale`` None is
+    1 / sqrt(head_dim). Returns ``out`` ([n, n_head, head_dim], q's type): zeros for
+    a sequence without keys. The workspace comes from torch's allocator on the
+    current stream; with another ``stream`` the caller orders the two."""
+    T = _torch()
+    dev = _device(q, "q")
+    if q.dim() != 3 or k.dim() != 4 or k_prefix.dim() != 3:
+        raise ValueError("q is [n, n_head, head_dim], a prefix [prefix, n_head_kv, head_dim], a cache [n_slots, rows, "
+                         f"n_head_kv, head_dim], got {tuple(q.shape)}, {tuple(k_prefix.shape)}, {tuple(k.shape)}")
+    n, n_head, hd = q.shape
+    prefix, (n_slots, rows, n_kv, _) = k_prefix.shape[0], k.shape
+    if k.shape[3] != hd or k_prefix.shape[1] != n_kv or k_prefix.shape[2] != hd:
+        raise ValueError(f"q {tuple(q.shape)}, prefix {tuple(k_prefix.shape)} and cache {tuple(k.shape)} do not match")
+    kt, qs, ps, cs = k.dtype, q.stride(), k_prefix.stride(), k.stride()
+    for name, t, like, st in (("v_prefix", v_prefix, k_prefix, ps), ("v", v, k, cs), ("k_prefix", k_prefix, k_prefix, ps)):
+        if t.shape != like.shape or t.dtype != kt or t.device.index != dev or (t.stride() != st and t.numel()):
+            raise ValueError(f"{name} must be {kt} on cuda:{dev} with the shape and strides of its keys, got "
+                             f"{tuple(t.shape)} {t.dtype} {t.stride()} on {t.device}")
+    if k.device.index != dev or (hd > 1 and (qs[2] != 1 or cs[3] != 1 or (prefix and ps[2] != 1))):
+        raise ValueError("q and the caches must be on one device with a contiguous last dimension")
+    if q.dtype not in T.tag or kt not in T.tag:
+        raise ValueError(f"queries of {q.dtype} with a cache of {kt}")
+    if out is None:
+        out = T.torch.empty((n, n_head, hd), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (hd > 1 and out.stride(2) != 1):
+        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device} with a contiguous last dimension")
+    if n == 0:
+        return out
+    key = (dev, n, n_head, n_kv)
+    size = _work_bytes.get(key)
+    if size is None:
+        need = C.c_size_t()
+        _lib.check(T.lib.talos_attention_shared_work(dev, n, n_head, n_kv, C.byref(need)))
+        size = _work_bytes[key] = need.value
+    work = T.torch.empty(size, dtype=T.u8, device=q.device)
+    os_ = out.stride()
+    a = _lib.AttentionSharedArgs(
+        dev, T.tag[q.dtype], T.tag[kt], n, n_head, n_kv, hd, prefix, n_slots, rows, q.data_ptr(), qs[0], qs[1],
+        k_prefix.data_ptr(), v_prefix.data_ptr(), ps[0], ps[1], k.data_ptr(), v.data_ptr(), cs[0], cs[1], cs[2],
+        None if slots is None else _vector(T, slots, "slots", n, T.i32, dev), _vector(T, lens, "lens", n, T.i32, dev),
+        out.data_ptr(), os_[0], os_[1], hd ** -0.5 if scale is None else scale)
+    _lib.check(T.lib.talos_attention_shared_dev(C.byref(a), work.data_ptr(), size, _stream(T, dev, stream)))
+    return out
 
 
 def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, probs=None, stream=None):
