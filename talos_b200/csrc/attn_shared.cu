@@ -32,32 +32,37 @@
 // multiplies its score (K) or moves its weight's exponent (V), so no input
 // overflows f16 and small ones keep their bits. lo x lo (2^-22) is left out.
 //
-// Roles of the 16 warps (one CTA per SM):
+// Roles (one CTA per SM):
 //  * warps 0-7: softmax. Warps w and w + 4 share the rows 32 w .. 32 w + 31 (their
 //    TMEM lanes), one half of the tile's keys and of the head's dims each; they
-//    exchange row maxima in shared memory.
-//  * warps 8-14: producers. 16-byte cp.async copies of K / V rows, zero-filled
-//    behind the last key, straight into the swizzled operand tiles (16-bit caches)
-//    or into a per-warp ring whose rows the same lanes then scale and split (f32).
-//  * warp 15: TMEM allocation; one lane issues the MMAs: QK of tile j ahead of PV
-//    of tile j - 1, so that the softmax of one tile runs beside the products of its
-//    neighbours.
-// Bound: HBM (the keys once) up to one row tile; above, softmax issue slots.
+//    exchange row maxima in shared memory. f32 queries are scaled and split by them.
+//  * 16-bit caches, 12 warps: warp 8 issues the TMA copies of the K tiles and the
+//    queries, warp 9 those of the V tiles (both straight into the swizzled operand
+//    tiles; separate, so that K runs ahead of V), warp 10 clears the V rows behind a
+//    suffix's last key, which the copy brought along and which may hold anything.
+//  * f32 cache, 16 warps: warp 14 issues TMA copies of half tiles (32 rows) into a
+//    ring, warps 8-13 scale and split them into the operand tiles.
+//  * the last warp: TMEM allocation, and the MMAs: QK of tile j ahead of PV of tile
+//    j - 1, so that the softmax of one tile runs beside the products of its neighbours.
+// Bound: HBM (the keys once) up to one row tile; above, the exponentials and the
+// tensor cores.
 //
 // Every wait is bounded (2 s); on expiry a CTA flag makes all roles run on without
 // waiting or multiplying, and the rows come out as NaN.
+#include <cuda.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "ops.cuh"
 #include "ptx.cuh"
 
 namespace talos {
 
-constexpr int AS_THREADS = 512;
-constexpr int AS_NP = 7;       // producer warps
-constexpr int AS_PW0 = 8, AS_MMA = 15;
 constexpr int AS_ROWS = 128;   // rows per tile = TMEM lanes
-constexpr int AS_SOFT_REGS = 184, AS_REST_REGS = 72;  // 256 x (184 + 72) = 512 x 128
+constexpr int AS_SOFT = 8;     // softmax warps
+constexpr int AS_CONV = 6;     // f32: converter warps
+constexpr int AS_HALF = 32;    // f32: rows of a half tile
 constexpr int AS_MISC = 12 * 1024;
 constexpr int AS_SMEM = 227 * 1024;
 constexpr float AS_LOG2E = 1.4426950408889634f;
@@ -66,43 +71,49 @@ constexpr float AS_LOG2E = 1.4426950408889634f;
 template <int MODE, int DP>
 struct AsCfg {
     static constexpr bool QF32 = MODE <= 1, KF32 = MODE == 0, BF = MODE == 3;
-    static constexpr int NQ = QF32 ? 2 : 1;  // planes (hi, lo) of Q and P
+    static constexpr int NQ = QF32 ? 2 : 1;  // planes (hi, lo) of Q
+    static constexpr int NP = QF32 ? 2 : 1;  // of P
     static constexpr int NK = KF32 ? 2 : 1;  // of K and V
-    static constexpr int KT = KF32 ? 64 : 128;  // keys per tile
-    static constexpr int ES = KF32 ? 4 : 2;     // bytes of a cache element
+    static constexpr int KT = KF32 ? 64 : 128;   // keys per tile
+    static constexpr int WARPS = KF32 ? 16 : 12;
+    static constexpr int THREADS = WARPS * 32;   // x 128 or 168 registers: the register file
+    // registers after the split: 256 x 168 + 256 x 88 = 512 x 128, 256 x 208 + 128 x 88 = 384 x 168
+    static constexpr int SOFT_REGS = KF32 ? 168 : 208, REST_REGS = 88;
     static constexpr int QPLANE = AS_ROWS * DP * 2, KPLANE = KT * DP * 2;
-    static constexpr int CPR = DP * ES / 16;   // 16-byte chunks of a cache row
-    static constexpr int RPW = 32 / CPR;       // rows per warp copy
-    static constexpr int ITERS = (KT / RPW + AS_NP - 1) / AS_NP;  // copies per warp and tile
-    static constexpr int RAWD = 24;            // f32: rows in flight per warp
-    static constexpr int RAW = KF32 ? AS_NP * RAWD * 512 : 0;
-    static constexpr int FIT = (AS_SMEM - AS_MISC - NQ * QPLANE - RAW) / (2 * NK * KPLANE);
-    static constexpr int NS = KF32 ? 1 : (FIT > 4 ? 4 : FIT);  // K / V stages
-    static constexpr int SMEM = NQ * QPLANE + NS * 2 * NK * KPLANE + RAW + AS_MISC;
+    static constexpr int RAW_HALF = AS_HALF * DP * 4;  // f32: one ring slot
+    static constexpr int NR = KF32 ? (DP == 128 ? 3 : 5) : 0;
+    // 16-bit outputs: the prefix's O is added up in tensor memory
+    static constexpr bool ACC = !QF32;
+    static constexpr int FIT = (AS_SMEM - AS_MISC - NQ * QPLANE) / KPLANE;  // 16-bit: operand tiles that fit
+    static constexpr int NSV = KF32 ? 2 : (FIT / 2 > 4 ? 4 : FIT / 2);
+    static constexpr int NSK = KF32 ? 1 : (FIT - NSV > 4 ? 4 : FIT - NSV);
+    static constexpr int SMEM = NQ * QPLANE + (NSK + NSV) * NK * KPLANE + NR * RAW_HALF + AS_MISC;
     static constexpr int S_COLS = KT;          // TMEM columns of one S buffer; P lies over it
     static constexpr int O_COL = 2 * KT;       // first column of the two O buffers
-    static_assert(NS >= 1 && SMEM <= AS_SMEM, "shared memory");
+    static_assert(NSV >= 1 && SMEM <= AS_SMEM, "shared memory");
     static_assert(2 * KT + 2 * DP <= 512, "tensor memory");
-    static_assert(RPW * ITERS <= 32, "one lane per row of a warp");
 };
 
 struct AsMisc {
-    uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4];
+    uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], v_raw[4], r_full[5], r_empty[5];
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], done;
     uint32_t tmem;
     int fail;
     int rt, b0, nb, tpg;     // row tile of this CTA, its first CTA and CTA count, tiles per kv head
-    int ntile_p, total;      // prefix tiles; tiles of the row tile
     int cum[AS_ROWS + 1];    // suffix tiles before each of the row tile's sequences
     int len[AS_ROWS], slot[AS_ROWS];
-    float qsc[2][AS_ROWS];   // row scale: scale * log2(e) * 2^(exponent of q)
+    float qsc[AS_ROWS];      // f32 queries: scale * log2(e) * 2^(exponent of the row)
     float mx[2][2][AS_ROWS], mx2[2][2][AS_ROWS];  // [tile parity][half] row maxima
     float lx[2][AS_ROWS];
     alignas(16) float ksc[4][64];   // f32 cache: 2^(key's exponent)
     alignas(16) float2 vsc[4][64];  // f32 cache: value row's exponent e and 2^e
-    int scan[16];
 };
 static_assert(sizeof(AsMisc) <= AS_MISC, "misc area");
+
+// The tensor maps of a call (CUtensorMap): queries (16-bit), the prefix's and the slots' rows.
+struct AsMaps {
+    CUtensorMap q, kp, vp, k, v;
+};
 
 // ---------------------------------------------------------------- PTX
 
@@ -152,6 +163,11 @@ __device__ __forceinline__ void as_ld32(uint32_t t, float* v) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(t));
 }
+__device__ __forceinline__ void as_ld8(uint32_t t, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(t));
+}
 __device__ __forceinline__ void as_st8(uint32_t t, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -160,13 +176,52 @@ __device__ __forceinline__ void as_st8(uint32_t t, const uint32_t* r) {
 __device__ __forceinline__ void as_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void as_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void as_pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void as_cp16(uint32_t dst, const void* src, uint32_t bytes) {  // the rest of 16: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ bool as_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
-__device__ __forceinline__ void as_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void as_cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void as_tma3(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void as_tma4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                        uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
+// two f32 in a 64-bit register pair
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 as_f2(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void as_un2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 as_fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 as_add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 as_mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float as_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ float as_ex2(float x) {
     float y;
@@ -189,6 +244,17 @@ __device__ __forceinline__ void as_split(float a, float b, uint32_t& hi, uint32_
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = as_pack<false>(a - f.x, b - f.y);
 }
+__device__ __forceinline__ void as_split_bf(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = as_pack<true>(a, b);
+    lo = as_pack<true>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+// The same split of a pair whose hi keeps 10 mantissa bits by truncation (exact in
+// f16 for |x| in its normal range; below it both parts round): fewer conversions.
+__device__ __forceinline__ void as_split_cut(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u), hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+    hi = as_pack<false>(ha, hb);
+    lo = as_pack<false>(a - ha, b - hb);
+}
 // The exponent e of the largest |x| (its bits), as used for scaling: x 2^(14 - e)
 // lies in [2^14, 2^15); kept where 2^(14 - e) and 2^(e - 14) are normal.
 __device__ __forceinline__ int as_exponent(uint32_t abs_bits) {
@@ -197,23 +263,47 @@ __device__ __forceinline__ int as_exponent(uint32_t abs_bits) {
 }
 __device__ __forceinline__ float as_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// Bounded wait; once the CTA has failed, no wait waits.
-__device__ __forceinline__ void as_wait(AsMisc* m, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return;
+// Bounded wait (2 s; the timer is read only after many polls, one read of it takes
+// about a microsecond). On expiry it marks the CTA as failed and `ok` as false:
+// the role then runs its loops to their end without waiting, copying, multiplying
+// or signalling (the pair barriers still match), and the others follow when their
+// own waits find the mark.
+__device__ __forceinline__ void as_wait(AsMisc* m, uint64_t* bar, uint32_t parity, bool& ok) {
+    if (!ok) return;
+#pragma unroll 1
+    for (int i = 0; i < 4096; ++i)
+        if (mbar_try_wait(bar, parity)) return;
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
-        for (int i = 0; i < 32; ++i)
+        if (*(volatile int*)&m->fail) break;
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
             if (mbar_try_wait(bar, parity)) return;
-        if (*(volatile int*)&m->fail) return;
-        if (globaltimer_ns() - t0 > 2000000000ull) {
-            *(volatile int*)&m->fail = 1;
-            return;
-        }
+        if (globaltimer_ns() - t0 > 2000000000ull) break;
     }
+    *(volatile int*)&m->fail = 1;
+    ok = false;
+}
+__device__ __forceinline__ void as_arrive(uint64_t* bar, bool ok) {
+    if (ok) mbar_arrive(bar);
+}
+// After a failure: time for the copies that a role has in flight to land.
+__device__ __forceinline__ void as_settle(bool ok) {
+    if (ok) return;
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
 }
 
-// First row of part i of n rows cut into nb even parts.
-__device__ __forceinline__ int as_part(int i, int n, int nb) { return (int)((long long)i * n / nb); }
+// First tile of part i of n tiles cut into nb even parts (the first n % nb parts
+// are one longer), and the part that holds tile x.
+__device__ __forceinline__ int as_part(int i, int n, int nb) {
+    const int q = n / nb, r = n - q * nb;
+    return i * q + min(i, r);
+}
+__device__ __forceinline__ int as_part_of(int x, int n, int nb) {
+    const int q = n / nb, r = n - q * nb, cut = r * (q + 1);
+    return x < cut ? x / (q + 1) : r + (x - cut) / max(q, 1);
+}
 
 __device__ __forceinline__ int as_len(const AttnSharedArgs& a, int seq, int prefix) {
     int len;
@@ -250,15 +340,16 @@ __device__ __forceinline__ int as_suffix_tiles(const AttnSharedArgs& a, int seq0
 // ---------------------------------------------------------------- the kernel
 
 template <int MODE, int DP>
-__global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_constant__ AttnSharedArgs a) {
+__global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
+    k_attn_shared(const __grid_constant__ AttnSharedArgs a, const __grid_constant__ AsMaps maps) {
     using C = AsCfg<MODE, DP>;
-    constexpr int KT = C::KT;
+    constexpr int KT = C::KT, NB = DP / 64;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + C::NQ * C::QPLANE;            // [NS][planes]
-    uint8_t* sV = sK + C::NS * C::NK * C::KPLANE;    // [NS][planes]
-    uint8_t* sR = sV + C::NS * C::NK * C::KPLANE;    // f32: raw rows [producer warp][RAWD][512]
-    AsMisc* m = (AsMisc*)(sR + C::RAW);
+    uint8_t* sK = sQ + C::NQ * C::QPLANE;            // [NSK][planes]
+    uint8_t* sV = sK + C::NSK * C::NK * C::KPLANE;   // [NSV][planes]
+    uint8_t* sR = sV + C::NSV * C::NK * C::KPLANE;   // f32: [NR] half tiles
+    AsMisc* m = (AsMisc*)(sR + C::NR * C::RAW_HALF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const int n = a.n_dev ? *a.n_dev : a.n;
@@ -267,47 +358,94 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
     const int R = (n + spt - 1) / spt;
     const int ntp = (prefix + KT - 1) / KT;
 
-    // ---- this CTA's row tile and run of tiles
-    if (tid == 0) m->fail = 0;
-    if (R > 1 && !a.whole) {
+    // ---- set-up: barriers, TMEM, this CTA's row tile and its run of tiles
+    // (the parameters' lines are read here together: one miss instead of one after another)
+    asm volatile("" ::"l"(a.q), "l"(a.kp), "l"(a.k), "l"(a.slot_sh), "l"(a.out), "r"(a.hd), "l"(a.lens), "l"(a.n_dev),
+                 "l"(a.part_o));
+    if (warp == C::WARPS - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&m->tmem)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid >= 96 && tid < 101) {  // the call's tensor maps (those that it has)
+        const int i = tid - 96;
+        if (i == 0 ? !C::QF32 : i < 3 ? a.prefix > 0 : a.slot_len > 0)
+            asm volatile("prefetch.tensormap [%0];" ::"l"((const CUtensorMap*)&maps + i) : "memory");
+    }
+    if (tid == 64) {
+        m->fail = 0;
+        mbar_init(&m->q_full, C::QF32 ? AS_SOFT : 1);
+        mbar_init(&m->q_empty, 1);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&m->k_full[i], C::KF32 ? AS_CONV : 1);
+            mbar_init(&m->k_empty[i], 1);
+            mbar_init(&m->v_full[i], C::KF32 ? AS_CONV : 1);
+            mbar_init(&m->v_empty[i], 1);
+            mbar_init(&m->v_raw[i], 1);
+        }
+#pragma unroll 1
+        for (int i = 0; i < 5; ++i) {
+            mbar_init(&m->r_full[i], 1);
+            mbar_init(&m->r_empty[i], AS_CONV);
+        }
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&m->s_full[i], 1);
+            mbar_init(&m->p_full[i], AS_SOFT);
+            mbar_init(&m->o_full[i], 1);
+            mbar_init(&m->o_empty[i], AS_SOFT);
+        }
+        mbar_init(&m->done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    int rt = 0, b0 = 0, nb = (int)gridDim.x;
+    if (a.whole) {  // one CTA per (row tile, kv head)
+        rt = (int)blockIdx.x / a.n_kv, b0 = rt * a.n_kv, nb = a.n_kv;
+    } else if (R == 1) {
+        if (blockIdx.x == 0 && tid == 0) a.plan[0] = 0, a.plan[1] = nb;
+    } else {
         // CTAs in proportion to the row tiles' work: row tile r has CTAs b(r) ..
         // b(r + 1) - 1, b(r) = r + (N - R) * (tiles before r) / (all tiles)
-        const int N = gridDim.x;
-        long long total = 0, before = 0;
-        int found = -1, b_lo = 0, b_hi = 0;
-        for (int pass = 0; pass < 2; ++pass) {
-            before = 0;
-            for (int r0 = 0; r0 < R; r0 += 16) {
-                const int r = r0 + warp;  // a warp sums one row tile's suffix tiles
-                const int own = as_suffix_tiles(a, r * spt, min(spt, n - r * spt), prefix, KT);
-                __syncthreads();
-                if (lane == 0) m->scan[warp] = r < R ? (ntp + own) * a.n_kv : 0;
-                __syncthreads();
-                for (int k = 0; k < 16 && r0 + k < R; ++k) {
-                    const int t = m->scan[k];
-                    if (pass == 1) {
-                        const int lo = r0 + k + (int)(total ? (long long)(N - R) * before / total : 0);
-                        const int hi = r0 + k + 1 + (int)(total ? (long long)(N - R) * (before + t) / total : 0);
-                        if (blockIdx.x == 0 && tid == 0) a.plan[2 * (r0 + k)] = lo, a.plan[2 * (r0 + k) + 1] = hi - lo;
-                        if ((int)blockIdx.x >= lo && (int)blockIdx.x < hi) found = r0 + k, b_lo = lo, b_hi = hi;
-                    }
-                    before += t;
-                }
-            }
-            total = before;
+        int* cnt = (int*)smem;  // [R] suffix tiles, before the operand tiles are used
+        for (int r = tid; r < R; r += C::THREADS) cnt[r] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += C::THREADS) {
+            const int len = as_len(a, i, prefix);
+            if (as_slot(a, i) >= 0 && len > 0) atomicAdd(&cnt[i / spt], (len + KT - 1) / KT);
         }
-        if (tid == 0) m->rt = found, m->b0 = b_lo, m->nb = b_hi - b_lo;
-    } else if (tid == 0) {
-        // one row tile: all CTAs; or (whole) one CTA per (row tile, kv head)
-        m->rt = a.whole ? (int)blockIdx.x / a.n_kv : 0;
-        m->b0 = a.whole ? m->rt * a.n_kv : 0;
-        m->nb = a.whole ? a.n_kv : (int)gridDim.x;
-        if (!a.whole && blockIdx.x == 0) a.plan[0] = 0, a.plan[1] = (int)gridDim.x;
+        __syncthreads();
+        if (warp == 0) {
+            const int N = gridDim.x;
+            int total = 0, before = 0;  // tiles of one kv head
+            for (int r = lane; r < R; r += 32) total += ntp + cnt[r];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            const double per = total ? (double)(N - R) / (double)total : 0.0;
+            if (lane == 0) m->rt = -1;
+            __syncwarp();
+            for (int r0 = 0; r0 < R; r0 += 32) {
+                const int r = r0 + lane;
+                const int t = r < R ? ntp + cnt[r] : 0;
+                int x = t;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                const int lo = r + (int)(per * (double)(before + x - t)), hi = r + 1 + (int)(per * (double)(before + x));
+                if (r < R) {
+                    if (blockIdx.x == 0) a.plan[2 * r] = lo, a.plan[2 * r + 1] = hi - lo;
+                    if ((int)blockIdx.x >= lo && (int)blockIdx.x < hi) m->rt = r, m->b0 = lo, m->nb = hi - lo;
+                }
+                before += __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+        __syncthreads();
+        rt = m->rt, b0 = m->b0, nb = m->nb;
     }
-    __syncthreads();
-    const int rt = m->rt, b0 = m->b0, nb = m->nb;
-    if (rt < 0 || rt >= R) return;
-    const int seq0 = rt * spt, nseq = min(spt, n - seq0);
+    const bool mine = rt >= 0 && rt < R;
+    const int seq0 = mine ? rt * spt : 0, nseq = mine ? min(spt, n - seq0) : 0;
     if (warp == 0) {  // the row tile's suffix list
         int run = 0;
         for (int i0 = 0; i0 < nseq; i0 += 32) {
@@ -315,7 +453,8 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
             int slot = -1, len = 0;
             if (i < nseq) {
                 slot = as_slot(a, seq0 + i);
-                len = slot >= 0 ? as_len(a, seq0 + i, prefix) : 0;
+                len = as_len(a, seq0 + i, prefix);
+                if (slot < 0) len = 0;
             }
             const int nt = (len + KT - 1) / KT;
             int x = nt;
@@ -332,394 +471,499 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
             m->tpg = ntp + run;
         }
     }
-    if (tid == 32) {
-        mbar_init(&m->q_full, AS_NP);
-        mbar_init(&m->q_empty, 1);
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&m->k_full[i], AS_NP);
-            mbar_init(&m->k_empty[i], 1);
-            mbar_init(&m->v_full[i], AS_NP);
-            mbar_init(&m->v_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&m->s_full[i], 1);
-            mbar_init(&m->p_full[i], 8);
-            mbar_init(&m->o_full[i], 1);
-            mbar_init(&m->o_empty[i], 8);
-        }
-        mbar_init(&m->done, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    const int tpg = m->tpg, total = tpg * a.n_kv;  // tiles per kv head, tiles of the row tile
-    const int rank = (int)blockIdx.x - b0;
-    const int t0 = as_part(rank, total, nb), t1 = as_part(rank + 1, total, nb);
-    if (tpg == 0) {
-        // no key in the whole row tile: zeros
-        if (rank == 0)
-            for (int i = tid; i < nseq * G * a.n_kv * a.hd; i += AS_THREADS) {
-                const int d = i % a.hd, h = i / a.hd % (G * a.n_kv), s = seq0 + i / a.hd / (G * a.n_kv);
-                const size_t at = (size_t)s * a.out_sn + (size_t)h * a.out_sh + d;
-                if (C::QF32) ((float*)a.out)[at] = 0.f;
-                else ((uint16_t*)a.out)[at] = 0;
-            }
-        return;
-    }
-    if (t0 >= t1) return;
-    if (warp == AS_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&m->tmem)),
-                     "r"(512u));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
     as_tc_before();
     __syncthreads();
     as_tc_after();
     const uint32_t tmem = m->tmem;
+    const int tpg = m->tpg, total = tpg * a.n_kv;  // tiles per kv head, tiles of the row tile
+    const int rank = (int)blockIdx.x - b0;
+    const int t0 = mine ? as_part(rank, total, nb) : 0, t1 = mine ? as_part(rank + 1, total, nb) : 0;
     const int rows = nseq * G;  // live rows
+    if (mine && tpg == 0 && rank == 0) {
+        // no key in the whole row tile: zeros
+        for (int i = tid; i < rows * a.n_kv * a.hd; i += C::THREADS) {
+            const int d = i % a.hd, h = i / a.hd % (G * a.n_kv), sq = seq0 + i / a.hd / (G * a.n_kv);
+            const size_t at = (size_t)sq * a.out_sn + (size_t)h * a.out_sh + d;
+            if (C::QF32) ((float*)a.out)[at] = 0.f;
+            else ((uint16_t*)a.out)[at] = 0;
+        }
+    }
+    // the sequence and the first key of suffix tile off (from a kv head's first tile), its valid keys
+    auto suffix = [&](int off, int& i, int& key) {
+        i = as_owner(m, nseq, off - ntp);
+        key = (off - ntp - m->cum[i]) * KT;
+        return min(KT, m->len[i] - key);
+    };
 
-    if (warp >= AS_PW0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AS_REST_REGS));
-        if (warp == AS_MMA) {
-            // ------------------------------------------------ MMA issuer
-            if (lane == 0) {
-                const int ksteps = (a.hd + 15) / 16;
-                const uint32_t id_qk = as_idesc(KT, C::BF, false), id_pv = as_idesc(ksteps * 16, C::BF, true);
-                const uint32_t q_hi = smem_u32(sQ), q_lo = q_hi + C::QPLANE;
-                int j = 0, seg = -1, cur = -1;
-                auto issue_pv = [&](int i) {  // tile i (counted from the CTA's first)
-                    const int sv = i % C::NS, bf = i & 1;
-                    as_wait(m, &m->p_full[bf], (i >> 1) & 1);
-                    as_wait(m, &m->v_full[sv], (i / C::NS) & 1);
-                    as_wait(m, &m->o_empty[bf], ((i >> 1) & 1) ^ 1);
-                    as_tc_after();
-                    if (!*(volatile int*)&m->fail) {
-                        const uint32_t d = tmem + C::O_COL + bf * DP, p = tmem + bf * C::S_COLS;
-                        const uint32_t v = smem_u32(sV + sv * C::NK * C::KPLANE);
-                        uint32_t acc = 0;
-                        // the small terms first
+    bool ok = true;
+    if (t0 >= t1) {
+        // nothing to do (TMEM is freed below)
+    } else if (warp >= AS_SOFT) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
+    if (warp == C::WARPS - 1) {
+        // ---------------------------------------------------- MMA issuer: the warp walks the
+        // tiles together (uniform control flow and descriptors), one lane issues
+        const bool lead = as_elect();
+        const int ksteps = (a.hd + 15) / 16;
+        const uint32_t id_qk = as_idesc(KT, C::BF, false), id_pv = as_idesc(ksteps * 16, C::BF, true);
+        const uint64_t dq = as_desc(smem_u32(sQ), 16), dk0 = as_desc(smem_u32(sK), 16),
+                       dv0 = as_desc(smem_u32(sV), KT * 128);
+        int j = 0, seg = -1, cur = -1;
+        uint32_t sk = 0, pk = 0, sv = 0, pv = 0;  // stage and its parity
+        uint32_t acc_buf = 0;       // ACC: O buffer of the segment's prefix tiles
+        bool pre = false, pre0 = false;  // the tile whose PV comes next: of the prefix, the segment's first
+        auto issue_pv = [&](int i) {  // tile i (counted from the CTA's first)
+            const uint32_t bf = i & 1, par = (i >> 1) & 1;
+            as_wait(m, &m->p_full[bf], par, ok);
+            as_wait(m, &m->v_full[sv], pv, ok);
+            as_wait(m, &m->o_empty[bf], par ^ 1, ok);
+            as_tc_after();
+            if (lead && ok) {
+                const uint32_t d = tmem + C::O_COL + (C::ACC && pre ? acc_buf : bf) * DP, p = tmem + bf * C::S_COLS;
+                const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
+                const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
+                // the small terms first
 #pragma unroll
-                        for (int pr = C::NQ + C::NK - 2; pr >= 0; --pr) {
-                            const bool p_lo = C::NQ == 2 && pr == 1, v_lo = pr == 2;
-                            const uint32_t pa = p + (p_lo ? KT / 2 : 0);
-                            const uint64_t vd = as_desc(v + (v_lo ? C::KPLANE : 0), KT * 128);
+                for (int pr = C::NP + C::NK - 2; pr >= 0; --pr) {
+                    const bool p_lo = C::NP == 2 && pr == 1, v_lo = pr == 2;
+                    const uint32_t pa = p + (p_lo ? KT / 2 : 0);
+                    const uint64_t vd = v + (v_lo ? C::KPLANE >> 4 : 0);
 #pragma unroll
-                            for (int ks = 0; ks < KT / 16; ++ks) {
-                                as_mma_ts(d, pa + 8 * ks, vd + (uint64_t)(ks * 2048 >> 4), id_pv, acc);
-                                acc = 1;
-                            }
-                        }
-                    }
-                    as_commit(&m->v_empty[sv]);
-                    as_commit(&m->o_full[bf]);
-                };
-                for (int t = t0; t < t1; ++t, ++j) {
-                    const int kvh = t / tpg;
-                    if (kvh != cur) {
-                        cur = kvh, ++seg;
-                        as_wait(m, &m->q_full, seg & 1);
-                    }
-                    const int sk = j % C::NS, bf = j & 1;
-                    as_wait(m, &m->k_full[sk], (j / C::NS) & 1);
-                    if (j >= 2) as_wait(m, &m->o_full[bf], ((j - 2) >> 1) & 1);  // P over this S buffer was read
-                    as_tc_after();
-                    if (!*(volatile int*)&m->fail) {
-                        const uint32_t d = tmem + bf * C::S_COLS;
-                        const uint32_t k = smem_u32(sK + sk * C::NK * C::KPLANE);
-                        uint32_t acc = 0;
-#pragma unroll
-                        for (int pr = C::NQ + C::NK - 2; pr >= 0; --pr) {
-                            const bool ql = C::NQ == 2 && pr == 1, kl = pr == 2;
-                            const uint32_t qa = ql ? q_lo : q_hi, ka = k + (kl ? C::KPLANE : 0);
-                            for (int ks = 0; ks < ksteps; ++ks) {
-                                const uint64_t qd = as_desc(qa + (ks >> 2) * (AS_ROWS * 128) + (ks & 3) * 32, 16);
-                                const uint64_t kd = as_desc(ka + (ks >> 2) * (KT * 128) + (ks & 3) * 32, 16);
-                                as_mma_ss(d, qd, kd, id_qk, acc);
-                                acc = 1;
-                            }
-                        }
-                    }
-                    as_commit(&m->k_empty[sk]);
-                    as_commit(&m->s_full[bf]);
-                    if (t + 1 == t1 || (t + 1) / tpg != kvh) as_commit(&m->q_empty);  // the queries may be replaced
-                    if (j > 0) issue_pv(j - 1);
+                    for (int ks = 0; ks < KT / 16; ++ks)
+                        as_mma_ts(d, pa + 8 * ks, vd + (uint64_t)(ks * 2048 >> 4), id_pv,
+                                  pr == C::NP + C::NK - 2 && ks == 0 ? keep : 1u);
                 }
-                issue_pv(j - 1);
-                as_commit(&m->done);
-                as_wait(m, &m->done, 0);  // nothing in flight when TMEM is freed
             }
             __syncwarp();
-        } else {
-            // ------------------------------------------------ producers
-            const int w = warp - AS_PW0;
-            const int chunk = lane % C::CPR, sub = lane / C::CPR;
-            const uint32_t row_bytes = (uint32_t)a.hd * C::ES;
-            const uint32_t live_bytes = (uint32_t)chunk * 16 < row_bytes ? 16u : 0u;
-            // the lane's row of a tile: its address, or none
-            struct Rows {
-                const uint8_t *k, *v;
-                bool ok;
-            };
-            auto row_of = [&](int t) {
-                Rows r{(const uint8_t*)a.q, (const uint8_t*)a.q, false};
-                const int kvh = t / tpg, off = t % tpg;
-                const int row = (w + AS_NP * (lane / C::RPW)) * C::RPW + lane % C::RPW;
-                if (lane >= C::RPW * C::ITERS || row >= KT) return r;
-                if (off < ntp) {
-                    const int key = off * KT + row;
-                    if (key < prefix) {
-                        const size_t at = ((size_t)key * a.pre_st + (size_t)kvh * a.pre_sh) * C::ES;
-                        r = Rows{(const uint8_t*)a.kp + at, (const uint8_t*)a.vp + at, true};
-                    }
-                } else {
-                    const int i = as_owner(m, nseq, off - ntp), key = (off - ntp - m->cum[i]) * KT + row;
-                    if (key < m->len[i]) {
-                        const size_t at = ((size_t)m->slot[i] * a.slot_ss +
-                                           (size_t)(key + a.slot_row0 * prefix) * a.slot_st +
-                                           (size_t)kvh * a.slot_sh) * C::ES;
-                        r = Rows{(const uint8_t*)a.k + at, (const uint8_t*)a.v + at, true};
-                    }
+            if (lead && ok) {
+                as_commit(&m->v_empty[sv]);
+                as_commit(&m->o_full[bf]);
+            }
+            if (++sv == C::NSV) sv = 0, pv ^= 1;
+        };
+        for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t, ++j) {
+            const bool fresh = kvh != cur;
+            if (fresh) {
+                // the softmax warps finish a segment before they load the next one's queries
+                if (j > 0) issue_pv(j - 1);
+                cur = kvh, ++seg;
+                as_wait(m, &m->q_full, seg & 1, ok);
+            }
+            const uint32_t bf = j & 1;
+            const bool is_pre = off < ntp;
+            const int first_off = off;
+            as_wait(m, &m->k_full[sk], pk, ok);
+            if (j >= 2) as_wait(m, &m->o_full[bf], ((j - 2) >> 1) & 1, ok);  // P over this S buffer was read
+            as_tc_after();
+            if (lead && ok) {
+                const uint32_t d = tmem + bf * C::S_COLS;
+                const uint64_t k = dk0 + (uint64_t)(sk * (C::NK * C::KPLANE >> 4));
+#pragma unroll
+                for (int pr = C::NQ + C::NK - 2; pr >= 0; --pr) {
+                    const bool ql = C::NQ == 2 && pr == 1, kl = pr == 2;
+                    const uint64_t qd = dq + (ql ? C::QPLANE >> 4 : 0), kd = k + (kl ? C::KPLANE >> 4 : 0);
+#pragma unroll
+                    for (int ks = 0; ks < DP / 16; ++ks)
+                        if (ks < ksteps)
+                            as_mma_ss(d, qd + (uint64_t)(((ks >> 2) * (AS_ROWS * 128) + (ks & 3) * 32) >> 4),
+                                      kd + (uint64_t)(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), id_qk,
+                                      pr == C::NQ + C::NK - 2 && ks == 0 ? 0u : 1u);
                 }
-                return r;
-            };
-            // the queries of kv head kvh into sQ
-            auto load_q = [&](int kvh, int seg) {
-                if (seg > 0) as_wait(m, &m->q_empty, (seg - 1) & 1);
-                if constexpr (C::QF32) {
-                    constexpr int QC = DP / 4, QR = 32 / QC;  // float4 chunks of a row, rows per warp
-                    constexpr int QI = (AS_ROWS / QR + AS_NP - 1) / AS_NP, QB = 5;
-                    const int ch = lane % QC;
-                    for (int i0 = 0; i0 < QI; i0 += QB) {
-                        float4 v[QB];
+            }
+            __syncwarp();
+            if (++off == tpg) off = 0, ++kvh;
+            if (lead && ok) {
+                as_commit(&m->k_empty[sk]);
+                as_commit(&m->s_full[bf]);
+                if (t + 1 == t1 || off == 0) as_commit(&m->q_empty);  // the queries may be replaced
+            }
+            if (++sk == C::NSK) sk = 0, pk ^= 1;
+            if (!fresh) issue_pv(j - 1);
+            // the prefix's buffer is not that of the first suffix tile
+            if (fresh) acc_buf = (j + (is_pre ? min(ntp - first_off, t1 - t) : 0) + 1) & 1;
+            pre = is_pre, pre0 = fresh;
+        }
+        issue_pv(j - 1);
+        // nothing in flight when TMEM is freed (also after a failure: a wait of its own)
+        if (lead) as_commit(&m->done);
+        bool end_ok = true;
+        as_wait(m, &m->done, 0, end_ok);
+    } else if (!C::KF32 && (warp == 8 || warp == 9)) {
+        // ---------------------------------------------------- TMA: K (and 16-bit queries), V
+        if (as_elect()) {
+            const bool is_v = warp == 9;
+            const CUtensorMap *mp = is_v ? &maps.vp : &maps.kp, *ms = is_v ? &maps.v : &maps.k;
+            uint64_t *full = is_v ? m->v_full : m->k_full, *empty = is_v ? m->v_empty : m->k_empty;
+            const uint32_t ns = is_v ? C::NSV : C::NSK;
+            const uint32_t base = smem_u32(is_v ? sV : sK);
+            const int q_box = min(spt, a.n) * G;  // rows of the query box
+            uint32_t st = 0, par = 1;
+            int seg = -1, cur = -1;
+            for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t) {
+                as_wait(m, &empty[st], par, ok);
+                int i = 0, key = 0, valid = KT;
+                if (off >= ntp) valid = suffix(off, i, key);
+                // rows behind the suffix's last one that the copy brings along: warp 10 clears them first
+                const bool fix = is_v && valid < KT && key + valid < a.slot_len;
+                uint64_t* bar = fix ? &m->v_raw[st] : &full[st];
+                if (ok) {
+                mbar_expect_tx(bar, C::KPLANE);
 #pragma unroll
-                        for (int i = 0; i < QB; ++i) {
-                            const int r = (w + AS_NP * (i0 + i)) * QR + lane / QC;
-                            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (r < rows && 4 * ch < a.hd)
-                                v[i] = *(const float4*)((const float*)a.q + (size_t)(seq0 + r / G) * a.q_sn +
-                                                        (size_t)(kvh * G + r % G) * a.q_sh + 4 * ch);
-                        }
-#pragma unroll
-                        for (int i = 0; i < QB; ++i) {
-                            const int r = (w + AS_NP * (i0 + i)) * QR + lane / QC;
-                            uint32_t b = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)),
-                                                               fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
-#pragma unroll
-                            for (int o = QC / 2; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-                            if (r >= rows) continue;
-                            const int e = as_exponent(b);
-                            const float f = as_pow2(14 - e);
-                            uint2 hi, lo;
-                            as_split(v[i].x * f, v[i].y * f, hi.x, lo.x);
-                            as_split(v[i].z * f, v[i].w * f, hi.y, lo.y);
-                            uint8_t* dst = sQ + (ch / 16) * (AS_ROWS * 128) + r * 128 +
-                                           (((ch % 16 / 2) ^ (r & 7)) << 4) + (ch & 1) * 8;
-                            *(uint2*)dst = hi;
-                            *(uint2*)(dst + C::QPLANE) = lo;
-                            if (ch == 0) m->qsc[seg & 1][r] = as_pow2(e - 14) * (a.scale * AS_LOG2E);
-                        }
-                    }
-                } else {
-                    constexpr int QC = DP / 8, QR = 32 / QC;
-                    constexpr int QI = (AS_ROWS / QR + AS_NP - 1) / AS_NP, QB = 5;
-                    const int ch = lane % QC;
-                    for (int i0 = 0; i0 < QI; i0 += QB) {
-                        uint4 v[QB];
-#pragma unroll
-                        for (int i = 0; i < QB; ++i) {
-                            const int r = (w + AS_NP * (i0 + i)) * QR + lane / QC;
-                            v[i] = make_uint4(0, 0, 0, 0);
-                            if (r < rows && 8 * ch < a.hd)
-                                v[i] = *(const uint4*)((const uint16_t*)a.q + (size_t)(seq0 + r / G) * a.q_sn +
-                                                       (size_t)(kvh * G + r % G) * a.q_sh + 8 * ch);
-                        }
-#pragma unroll
-                        for (int i = 0; i < QB; ++i) {
-                            const int r = (w + AS_NP * (i0 + i)) * QR + lane / QC;
-                            if (r < rows)
-                                *(uint4*)(sQ + (ch / 8) * (AS_ROWS * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4)) = v[i];
-                        }
-                    }
+                for (int b = 0; b < NB; ++b) {
+                    const uint32_t dst = base + st * C::KPLANE + b * (KT * 128);
+                    if (off < ntp) as_tma3(dst, mp, 64 * b, kvh, off * KT, bar);
+                    else as_tma4(dst, ms, 64 * b, kvh, key, m->slot[i], bar);
                 }
+                }
+                if (!C::QF32 && !is_v && kvh != cur) {
+                    cur = kvh, ++seg;
+                    if (seg > 0) as_wait(m, &m->q_empty, (seg - 1) & 1, ok);
+                    if (ok) mbar_expect_tx(&m->q_full, (uint32_t)q_box * 128 * NB);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        if (ok) as_tma3(smem_u32(sQ) + b * (AS_ROWS * 128), &maps.q, 64 * b, kvh * G, seq0, &m->q_full);
+                }
+                if (++st == ns) st = 0, par ^= 1;
+                if (++off == tpg) off = 0, ++kvh;
+            }
+            as_settle(ok);
+        }
+        __syncwarp();
+    } else if (!C::KF32 && warp == 10) {
+        // ---------------------------------------------------- V rows behind a suffix's last key: zeros
+        uint32_t st = 0, raw_par = 0;  // bit s: parity of v_raw[s]
+        for (int t = t0, off = t0 % tpg; t < t1; ++t) {
+            int i = 0, key = 0, valid = KT;
+            if (off >= ntp) valid = suffix(off, i, key);
+            if (valid < KT && key + valid < a.slot_len) {
+                as_wait(m, &m->v_raw[st], (raw_par >> st) & 1, ok);
+                raw_par ^= 1u << st;
+                uint8_t* v = sV + st * C::KPLANE;
+                for (int c = valid * 8 + lane; c < KT * 8; c += 32)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) *(uint4*)(v + b * (KT * 128) + c * 16) = make_uint4(0, 0, 0, 0);
                 as_fence_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&m->q_full);
-            };
-
-            if constexpr (!C::KF32) {
-                // jobs: K then V of each tile; up to LAG jobs stay in flight. PV of a tile is
-                // issued behind QK of the next one, so a V stage is free again only after the
-                // K job 2 NS - 1 before has landed: LAG is at most 2 NS - 2
-                constexpr int LAG = 2 * C::NS - 2;
-                static_assert(LAG >= 1, "two stages at least");
-                int issued = 0, landed = 0;  // jobs
-                auto land = [&]() {  // the oldest job in flight has arrived
-                    as_fence_async();
-                    __syncwarp();
-                    const int i = landed >> 1;
-                    if (lane == 0) mbar_arrive(landed & 1 ? &m->v_full[i % C::NS] : &m->k_full[i % C::NS]);
-                    ++landed;
-                };
-                auto issue = [&](const Rows& r, bool is_v) {
-                    const int i = issued >> 1, s = i % C::NS;
-                    as_wait(m, is_v ? &m->v_empty[s] : &m->k_empty[s], ((i / C::NS) & 1) ^ 1);
-                    const uint32_t dst = smem_u32((is_v ? sV : sK) + s * C::KPLANE) + (chunk / 8) * (KT * 128);
-                    const unsigned long long p = (unsigned long long)(is_v ? r.v : r.k);
-#pragma unroll
-                    for (int it = 0; it < C::ITERS; ++it) {
-                        const int from = it * C::RPW + sub;
-                        const uint8_t* src = (const uint8_t*)__shfl_sync(0xffffffffu, p, from);
-                        const bool ok = __shfl_sync(0xffffffffu, (int)r.ok, from);
-                        const int row = (w + AS_NP * it) * C::RPW + sub;
-                        if (row < KT) {
-                            const uint32_t nb_ = ok ? live_bytes : 0u;
-                            as_cp16(dst + row * 128 + (((chunk % 8) ^ (row & 7)) << 4), nb_ ? src + chunk * 16 : a.q, nb_);
-                        }
-                    }
-                    as_cp_commit();
-                    ++issued;
-                };
-                int cur = -1, seg = -1;
-                for (int t = t0; t < t1; ++t) {
-                    const bool fresh = t / tpg != cur;
-                    if (fresh && seg >= 0) {  // the queries wait for every product of the segment before
-                        as_cp_wait<0>();
-                        while (landed < issued) land();
-                    }
-                    const Rows r = row_of(t);
-                    issue(r, false);
-                    if (issued - landed > LAG) {
-                        as_cp_wait<LAG>();
-                        land();
-                    }
-                    issue(r, true);
-                    if (fresh) cur = t / tpg, load_q(cur, ++seg);
-                    if (issued - landed > LAG) {
-                        as_cp_wait<LAG>();
-                        land();
-                    }
+                if (lane == 0) as_arrive(&m->v_full[st], ok);
+            }
+            if (++st == C::NSV) st = 0;
+            if (++off == tpg) off = 0;
+        }
+    } else if (C::KF32 && warp == 14) {
+        // ---------------------------------------------------- f32 rows: TMA of half tiles into the ring
+        if (as_elect()) {
+            uint32_t st = 0, par = 1;
+            for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t) {
+                int i = 0, key = off * KT, valid = min(KT, prefix - off * KT);
+                if (off >= ntp) valid = suffix(off, i, key);
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {  // K, K, V, V
+                    if ((h & 1) * AS_HALF >= valid) continue;
+                    as_wait(m, &m->r_empty[st], par, ok);
+                    if (!ok) continue;
+                    mbar_expect_tx(&m->r_full[st], C::RAW_HALF);
+                    const uint32_t dst = smem_u32(sR) + st * C::RAW_HALF;
+                    const int row = key + (h & 1) * AS_HALF;
+                    if (off < ntp) as_tma3(dst, h < 2 ? &maps.kp : &maps.vp, 0, kvh, row, &m->r_full[st]);
+                    else
+                        as_tma4(dst, h < 2 ? &maps.k : &maps.v, 0, kvh, row + a.slot_row0 * prefix, m->slot[i],
+                                &m->r_full[st]);
+                    if (++st == C::NR) st = 0, par ^= 1;
                 }
-                as_cp_wait<0>();
-                while (landed < issued) land();
-            } else {
-                // f32 rows: a lane's 16 bytes go through its own ring slots, RAWD - 1
-                // copies ahead of the conversion; K rows of a tile, then its V rows
-                const uint32_t ring = smem_u32(sR) + w * C::RAWD * 512 + lane * 16;
-                const int total_it = (t1 - t0) * 2 * C::ITERS;
-                int it_i = 0, t_i = t0, half_i = 0;  // issue cursor
-                uint32_t slot_i = 0, slot_c = 0;
-                Rows r_i = row_of(t0);
-                auto issue = [&]() {
-                    if (t_i < t1) {
-                        const unsigned long long p = (unsigned long long)(half_i ? r_i.v : r_i.k);
-                        const int from = it_i * C::RPW + sub;
-                        const uint8_t* src = (const uint8_t*)__shfl_sync(0xffffffffu, p, from);
-                        const bool ok = __shfl_sync(0xffffffffu, (int)r_i.ok, from);
-                        const uint32_t nb_ = ok ? live_bytes : 0u;
-                        as_cp16(ring + slot_i * 512, nb_ ? src + chunk * 16 : a.q, nb_);
-                        slot_i = slot_i + 1 == C::RAWD ? 0 : slot_i + 1;
-                        if (++it_i == C::ITERS) {
-                            it_i = 0;
-                            if (half_i) {
-                                if (++t_i < t1) r_i = row_of(t_i);
-                            }
-                            half_i ^= 1;
-                        }
-                    }
-                    as_cp_commit();  // (empty at the end: the count of groups stays in step)
-                };
-                for (int i = 0; i < C::RAWD - 1; ++i) issue();
-                int cur = -1, seg = -1, it_c = 0, half_c = 0, t_c = t0, j = 0;
-                for (int c = 0; c < total_it; ++c) {
-                    issue();
-                    if (it_c == 0) {
-                        if (half_c == 0 && t_c / tpg != cur) cur = t_c / tpg, load_q(cur, ++seg);
-                        if (j > 0) as_wait(m, half_c ? &m->v_empty[0] : &m->k_empty[0], (j - 1) & 1);
-                    }
-                    as_cp_wait<C::RAWD - 1>();
-                    float4 v;
-                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                                 : "r"(ring + slot_c * 512)
-                                 : "memory");
-                    slot_c = slot_c + 1 == C::RAWD ? 0 : slot_c + 1;
-                    const int row = (w + AS_NP * it_c) * C::RPW + sub;
-                    uint32_t b = __float_as_uint(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                    if constexpr (C::RPW == 1) {
-                        b = __reduce_max_sync(0xffffffffu, b);
+                if (++off == tpg) off = 0, ++kvh;
+            }
+            as_settle(ok);
+        }
+        __syncwarp();
+    } else if (C::KF32 && warp >= 8) {
+        // ---------------------------------------------------- converters: ring -> scaled f16 hi + lo
+        constexpr int QC = DP / 4, QR = 32 / QC;               // float4 chunks of a row, rows per warp step
+        constexpr int NI = (AS_HALF / QR + AS_CONV - 1) / AS_CONV;
+        const int w = warp - 8, ch = lane % QC, sub = lane / QC;
+        uint32_t st = 0, par = 0;
+        int j = 0;
+        for (int t = t0, off = t0 % tpg; t < t1; ++t, ++j) {
+            int i = 0, key = 0, valid = min(KT, prefix - off * KT);
+            if (off >= ntp) valid = suffix(off, i, key);
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
+                const bool is_v = h >= 2;
+                const int r0 = (h & 1) * AS_HALF;
+                const bool have = r0 < valid;
+                if ((h & 1) == 0) {
+                    if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
+                    if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+                }
+                float4 v[NI];
+                if (have) as_wait(m, &m->r_full[st], par, ok);
+#pragma unroll
+                for (int q = 0; q < NI; ++q) {
+                    const int r = (w + AS_CONV * q) * QR + sub;
+                    v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    // rows behind the last key (the next ones of the slot, or stale) become zeros
+                    if (r < AS_HALF && r0 + r < valid)
+                        v[q] = *(const float4*)(sR + st * C::RAW_HALF + (r * QC + ch) * 16);
+                }
+                uint32_t mxb[NI];
+#pragma unroll
+                for (int q = 0; q < NI; ++q) {
+                    mxb[q] = __float_as_uint(fmaxf(fmaxf(fabsf(v[q].x), fabsf(v[q].y)), fmaxf(fabsf(v[q].z), fabsf(v[q].w))));
+                    if constexpr (QR == 1) {
+                        mxb[q] = __reduce_max_sync(0xffffffffu, mxb[q]);
                     } else {
 #pragma unroll
-                        for (int o = C::CPR / 2; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-                    }
-                    if (row < KT) {
-                        const int e = as_exponent(b);
-                        const float f = as_pow2(14 - e);
-                        uint2 hi, lo;
-                        as_split(v.x * f, v.y * f, hi.x, lo.x);
-                        as_split(v.z * f, v.w * f, hi.y, lo.y);
-                        uint8_t* dst = (half_c ? sV : sK) + (chunk / 16) * (KT * 128) + row * 128 +
-                                       (((chunk % 16 / 2) ^ (row & 7)) << 4) + (chunk & 1) * 8;
-                        *(uint2*)dst = hi;
-                        *(uint2*)(dst + C::KPLANE) = lo;
-                        if (chunk == 0) {
-                            if (half_c) m->vsc[j & 3][row] = make_float2((float)(e - 14), as_pow2(e - 14));
-                            else m->ksc[j & 3][row] = as_pow2(e - 14);
-                        }
-                    }
-                    if (++it_c == C::ITERS) {
-                        as_fence_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(half_c ? &m->v_full[0] : &m->k_full[0]);
-                        it_c = 0;
-                        if (half_c) ++t_c, ++j;
-                        half_c ^= 1;
+                        for (int o = QC / 2; o > 0; o >>= 1) mxb[q] = max(mxb[q], __shfl_xor_sync(0xffffffffu, mxb[q], o));
                     }
                 }
-                as_cp_wait<0>();
+                if (have) {
+                    // the slot is free once its values have arrived, which the reductions above
+                    // waited for (an arrival may overtake loads that are still under way)
+                    __syncwarp();
+                    if (lane == 0) as_arrive(&m->r_empty[st], ok);
+                    if (++st == C::NR) st = 0, par ^= 1;
+                }
+#pragma unroll
+                for (int q = 0; q < NI; ++q) {
+                    const int r = (w + AS_CONV * q) * QR + sub;
+                    if (r >= AS_HALF) continue;
+                    const int e = as_exponent(mxb[q]), row = r0 + r;
+                    const float f = as_pow2(14 - e);
+                    uint2 hi, lo;
+                    as_split_cut(v[q].x * f, v[q].y * f, hi.x, lo.x);
+                    as_split_cut(v[q].z * f, v[q].w * f, hi.y, lo.y);
+                    uint8_t* dst = (is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK) + (ch / 16) * (KT * 128) + row * 128 +
+                                   (((ch % 16 / 2) ^ (row & 7)) << 4) + (ch & 1) * 8;
+                    *(uint2*)dst = hi;
+                    *(uint2*)(dst + C::KPLANE) = lo;
+                    if (ch == 0) {
+                        if (is_v) m->vsc[j & 3][row] = make_float2((float)(e - 14), as_pow2(e - 14));
+                        else m->ksc[j & 3][row] = as_pow2(e - 14);
+                    }
+                }
+                if (h & 1) {
+                    as_fence_async();
+                    __syncwarp();
+                    if (lane == 0) as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
+                }
             }
+            if (++off == tpg) off = 0;
         }
+    }
     } else {
-        // ------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AS_SOFT_REGS));
+        // ---------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFT_REGS));
         const int half = warp >> 2, q4 = warp & 3;
         const int row = q4 * 32 + lane, sq = row / G;
         const bool live = row < rows;
         const uint32_t lane_base = tmem + ((uint32_t)(q4 * 32) << 16);
         constexpr int HC = KT / 2, HD = DP / 2;  // this thread's keys of a tile, dims of the output
         constexpr float OFF = C::BF ? 0.f : 14.f;  // f16 weights: 2^14 at the maximum keeps small ones normal
-        float o[HD];
-        float mrun = -INFINITY, Mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = 0.f;
+        f2 o[HD / 2];
+        float mrun = -INFINITY, Mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = a.scale * AS_LOG2E;
         bool prev_act = false, prev_any = false;
         const int own0 = live ? m->cum[sq] : 0, own = live ? m->len[sq] : 0;  // its first suffix tile, its keys
 
-        auto add_o = [&](int i) {  // o = o * cprev + O of tile i
-            as_wait(m, &m->o_full[i & 1], (i >> 1) & 1);
+        // the queries of kv head kvh, scaled per row and split: 16 rows per warp
+        auto load_q = [&](int kvh) {
+            constexpr int QC = DP / 4, QR = 32 / QC, QI = 16 / QR, QB = 8;
+            const int ch = lane % QC;
+            const int r0 = q4 * 32 + half * 16 + lane / QC;
+            uint8_t* dst0 = sQ + (ch / 16) * (AS_ROWS * 128) + (ch & 1) * 8;
+#pragma unroll 1
+            for (int i0 = 0; i0 < QI; i0 += QB) {
+                float4 v[QB];
+#pragma unroll
+                for (int i = 0; i < QB; ++i) {
+                    const int r = r0 + (i0 + i) * QR, rs = (r * a.div_g) >> 16;  // r / G
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < rows && 4 * ch < a.hd)
+                        v[i] = *(const float4*)((const float*)a.q + (size_t)(seq0 + rs) * a.q_sn +
+                                                (size_t)(kvh * G + r - rs * G) * a.q_sh + 4 * ch);
+                }
+#pragma unroll
+                for (int i = 0; i < QB; ++i) {
+                    const int r = r0 + (i0 + i) * QR;
+                    uint32_t b = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+                    if constexpr (QR == 1) {
+                        b = __reduce_max_sync(0xffffffffu, b);
+                    } else {
+#pragma unroll
+                        for (int d = QC / 2; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
+                    }
+                    const int e = as_exponent(b);
+                    const float f = as_pow2(14 - e);
+                    uint2 hi, lo;
+                    as_split(v[i].x * f, v[i].y * f, hi.x, lo.x);
+                    as_split(v[i].z * f, v[i].w * f, hi.y, lo.y);
+                    uint8_t* dst = dst0 + r * 128 + (((ch % 16 / 2) ^ (r & 7)) << 4);
+                    *(uint2*)dst = hi;
+                    *(uint2*)(dst + C::QPLANE) = lo;
+                    if (ch == 0) m->qsc[r] = as_pow2(e - 14) * (a.scale * AS_LOG2E);
+                }
+            }
+            as_fence_async();
+            __syncwarp();
+            if (lane == 0) as_arrive(&m->q_full, ok);
+            as_pair_sync(1 + q4);
+            qs = m->qsc[row];
+        };
+        // ACC, a prefix tile after the segment's first: O so far times cnew, in tensor memory
+        auto rescale = [&](int j, uint32_t buf, float c) {
+            as_wait(m, &m->o_full[(j - 1) & 1], ((j - 1) >> 1) & 1, ok);
             as_tc_after();
-            if (prev_any) {
-                const uint32_t src = lane_base + C::O_COL + (i & 1) * DP + half * HD;
+            const uint32_t at = lane_base + C::O_COL + buf * DP + half * HD;
+#pragma unroll 1
+            for (int k = 0; k < HD; k += 8) {
+                uint32_t x[8];
+                as_ld8(at + k, x);
+                as_wait_ld();
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    float x[32];
-                    as_ld32(src + c, x);
-                    as_wait_ld();
+                for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * c);
+                as_st8(at + k, x);
+            }
+        };
+        // scores of tile j -> weights; FULL: every row of the warp has all of its half's keys
+        auto weigh = [&](auto full_c, int j, bool act, int h0, int acc_buf) {  // acc_buf: rescale there, or < 0
+            constexpr bool FULL = decltype(full_c)::value;
+            const uint32_t bf = j & 1, sb = lane_base + bf * C::S_COLS;
+            float s[HC];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[c + k] = prev_act ? fmaf(o[c + k], cprev, x[k]) : o[c + k];
+            for (int c = 0; c < HC; c += 32) as_ld32(sb + half * HC + c, s + c);
+            as_wait_ld();
+            if (C::KF32) {
+#pragma unroll
+                for (int k = 0; k < HC; k += 4) {
+                    const float4 ks = *(const float4*)&m->ksc[j & 3][half * HC + k];
+                    as_un2(as_mul2(as_f2(s[k], s[k + 1]), as_f2(ks.x, ks.y)), s[k], s[k + 1]);
+                    as_un2(as_mul2(as_f2(s[k + 2], s[k + 3]), as_f2(ks.z, ks.w)), s[k + 2], s[k + 3]);
+                }
+            }
+            if (!FULL) {
+#pragma unroll
+                for (int k = 0; k < HC; ++k) s[k] = k < h0 ? s[k] : -INFINITY;
+            }
+            // (s stays unscaled; the scaled maximum is the maximum of the scaled, qs > 0)
+            float mt, Mt = -INFINITY;
+            {
+                float m2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < HC; k += 8)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) m2[q] = as_max3(m2[q], s[k + 2 * q], s[k + 2 * q + 1]);
+                mt = fmaxf(as_max3(m2[0], m2[1], m2[2]), m2[3]) * qs;
+            }
+            const f2 q2 = as_f2(qs, qs);
+            if (C::KF32) {
+#pragma unroll
+                for (int k = 0; k < HC; k += 2) {
+                    const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k];
+                    float x, y;
+                    as_un2(as_fma2(as_f2(s[k], s[k + 1]), q2, as_f2(vs.x, vs.z)), x, y);
+                    Mt = as_max3(Mt, x, y);
+                }
+            }
+            m->mx[bf][half][row] = mt;
+            if (C::KF32) m->mx2[bf][half][row] = Mt;
+            as_pair_sync(1 + q4);  // (also: both halves of S are read, P may overwrite them)
+            float cnew = 1.f, fv = 0.f, fw = 0.f;
+            if (act) {
+                // integer exponents: exact powers of two (0 on the first tile)
+                const float mnew = fmaxf(mrun, ceilf(fmaxf(mt, m->mx[bf][half ^ 1][row])));
+                const float cl = as_ex2(mrun - mnew);
+                cnew = cl;
+                lsum *= cl;
+                mrun = mnew;
+                if (C::KF32) {
+                    const float Mnew = fmaxf(Mrun, ceilf(fmaxf(Mt, m->mx2[bf][half ^ 1][row])));
+                    cnew = as_ex2(Mrun - Mnew);
+                    Mrun = Mnew;
+                    // 2^(m - M + OFF) as two factors: it may pass 2^127 where the values are tiny
+                    const float d = mnew - Mnew + OFF, d2 = floorf(0.5f * d);
+                    fv = as_ex2(d2), fw = as_ex2(d - d2);
+                }
+            }
+            if (C::ACC && acc_buf >= 0 && __any_sync(0xffffffffu, cnew != 1.f)) rescale(j, acc_buf, cnew);
+            const float sub = C::KF32 ? mrun : mrun - OFF;
+            const f2 sub2 = as_f2(-sub, -sub);
+            f2 l2[2] = {0ull, 0ull};
+            // P over S: hi planes in the first half of the columns, lo in the second
+#pragma unroll
+            for (int k = 0; k < HC; k += 16) {
+                uint32_t ph[8], pl[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float x, y;
+                    as_un2(as_fma2(as_f2(s[k + 2 * i], s[k + 2 * i + 1]), q2, sub2), x, y);
+                    x = as_ex2(x), y = as_ex2(y);
+                    if (!FULL) x = k + 2 * i < h0 ? x : 0.f, y = k + 2 * i + 1 < h0 ? y : 0.f;
+                    l2[i & 1] = as_add2(l2[i & 1], as_f2(x, y));
+                    if (C::KF32) {
+                        // weight x 2^(its value row's exponent), relative to the running maximum M
+                        // (capped at 2^126: there the weight itself is below 2^-112, its share is lost either way)
+                        const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k + 2 * i];
+                        x *= fminf(vs.y * fv * fw, 0x1p126f);
+                        y *= fminf(vs.w * fv * fw, 0x1p126f);
+                    }
+                    if (C::NP == 2) {
+                        if (C::BF) as_split_bf(x, y, ph[i], pl[i]);
+                        else as_split(x, y, ph[i], pl[i]);
+                    } else {
+                        ph[i] = as_pack<C::BF>(x, y);
+                    }
+                }
+                as_st8(sb + (half * HC + k) / 2, ph);
+                if (C::NP == 2) as_st8(sb + KT / 2 + (half * HC + k) / 2, pl);
+            }
+            float x, y;
+            as_un2(as_add2(l2[0], l2[1]), x, y);
+            lsum += x + y;
+            return cnew;
+        };
+
+        // what becomes of a tile's O: added to o[] while the next tile is worked on;
+        // ACC: left in tensor memory (prefix), or brought from there (the last prefix tile)
+        enum { ADD = 0, LEAVE = 1, BRING = 2 };
+        int kind = ADD, acc_buf = 0;
+        float x[HD];
+        auto fetch_o = [&](int i) {  // tile i's O on its way to x
+            as_wait(m, &m->o_full[i & 1], (i >> 1) & 1, ok);
+            as_tc_after();
+            if (prev_any && kind != LEAVE) {
+                const uint32_t src = lane_base + C::O_COL + (C::ACC && kind == BRING ? acc_buf : i & 1) * DP + half * HD;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) as_ld32(src + c, x + c);
+            }
+        };
+        auto take_o = [&](int i) {  // o = o * cprev + x
+            if (prev_any && kind != LEAVE) {
+                as_wait_ld();
+                if (prev_act) {
+                    const f2 c2 = as_f2(cprev, cprev);
+                    if (C::ACC && kind == BRING) {
+#pragma unroll
+                        for (int k = 0; k < HD / 2; ++k) o[k] = as_f2(x[2 * k], x[2 * k + 1]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < HD / 2; ++k) o[k] = as_fma2(o[k], c2, as_f2(x[2 * k], x[2 * k + 1]));
+                    }
                 }
             }
             as_tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&m->o_empty[i & 1]);
+            if (lane == 0) as_arrive(&m->o_empty[i & 1], ok);
         };
 
-        int j = 0, cur = -1, seg = -1, seg_t0 = t0;
-        for (int t = t0; t < t1; ++t, ++j) {
-            const int kvh = t / tpg, off = t % tpg, bf = j & 1;
+        int j = 0, cur = -1, seg_t0 = t0;
+        for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t, ++j) {
             const bool first = kvh != cur;
             if (first) {
-                cur = kvh, ++seg, seg_t0 = t;
+                cur = kvh, seg_t0 = t;
+                if constexpr (C::QF32) load_q(kvh);  // (the segment before is done with the last ones)
 #pragma unroll
-                for (int k = 0; k < HD; ++k) o[k] = 0.f;
+                for (int k = 0; k < HD / 2; ++k) o[k] = 0ull;
                 mrun = Mrun = -INFINITY;
                 lsum = 0.f;
+                if (C::ACC) acc_buf = (j + (off < ntp ? min(ntp - off, t1 - t) : 0) + 1) & 1;
             }
             // the row's keys of this tile: the first hi
             int hi = 0;
@@ -730,99 +974,33 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
             }
             const bool act = hi > 0;
             const bool any = __any_sync(0xffffffffu, act);
-            as_wait(m, &m->s_full[bf], (j >> 1) & 1);
-            if (C::KF32) as_wait(m, &m->v_full[0], j & 1);  // the values' exponents
+            const uint32_t bf = j & 1;
+            as_wait(m, &m->s_full[bf], (j >> 1) & 1, ok);
+            if (C::KF32) as_wait(m, &m->v_full[bf], (j >> 1) & 1, ok);  // the values' exponents
             as_tc_after();
-            if (first) qs = C::QF32 ? (live ? m->qsc[seg & 1][row] : 0.f) : a.scale * AS_LOG2E;
             float cnew = 1.f;
             if (any) {
-                float s[HC];
-                const uint32_t sb = lane_base + bf * C::S_COLS;
-#pragma unroll
-                for (int c = 0; c < HC; c += 32) as_ld32(sb + half * HC + c, s + c);
-                as_wait_ld();
-                const int h0 = hi - half * HC;
-                const bool full = __all_sync(0xffffffffu, h0 >= HC);
-                float mt = -INFINITY, Mt = -INFINITY;
-                if (C::KF32) {
-#pragma unroll
-                    for (int k = 0; k < HC; k += 4) {
-                        const float4 ks = *(const float4*)&m->ksc[j & 3][half * HC + k];
-                        s[k] *= ks.x, s[k + 1] *= ks.y, s[k + 2] *= ks.z, s[k + 3] *= ks.w;
-                    }
-                }
-                // (s stays unscaled; the scaled maximum is the maximum of the scaled, qs > 0)
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < HC; ++k) m4[k & 3] = fmaxf(m4[k & 3], full || k < h0 ? s[k] : -INFINITY);
-                mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qs;
-                if (C::KF32) {
-#pragma unroll
-                    for (int k = 0; k < HC; k += 2) {
-                        const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k];
-                        Mt = fmaxf(Mt, fmaxf(full || k < h0 ? fmaf(s[k], qs, vs.x) : -INFINITY,
-                                             full || k + 1 < h0 ? fmaf(s[k + 1], qs, vs.z) : -INFINITY));
-                    }
-                }
-                m->mx[bf][half][row] = mt;
-                if (C::KF32) m->mx2[bf][half][row] = Mt;
-                as_pair_sync(1 + q4);  // (also: both halves of S are read, P may overwrite them)
-                mt = fmaxf(mt, m->mx[bf][half ^ 1][row]);
-                const float mnew = fmaxf(mrun, ceilf(mt));
-                float fv = 0.f, Mnew = Mrun;
-                if (C::KF32) {
-                    Mt = fmaxf(Mt, m->mx2[bf][half ^ 1][row]);
-                    Mnew = fmaxf(Mrun, ceilf(Mt));
-                }
-                if (act) {
-                    // integer exponents: exact powers of two (0 on the first tile)
-                    const float cl = as_ex2(mrun - mnew);
-                    cnew = C::KF32 ? as_ex2(Mrun - Mnew) : cl;
-                    lsum *= cl;
-                    mrun = mnew, Mrun = Mnew;
-                    if (C::KF32) fv = mnew - Mnew + OFF;
-                }
-                const float sub = C::KF32 ? mrun : mrun - OFF;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < HC; ++k) {
-                    s[k] = full || k < h0 ? as_ex2(fmaf(s[k], qs, -sub)) : 0.f;
-                    l4[k & 3] += s[k];
-                }
-                lsum += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                if (C::KF32) {
-                    // weight x 2^(its value row's exponent), relative to the running maximum M
-#pragma unroll
-                    for (int k = 0; k < HC; k += 2) {
-                        const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k];
-                        // (beyond 2^126 the weight itself is below 2^-112: its share is lost either way)
-                        s[k] *= as_ex2(fminf(vs.x + fv, 126.f));
-                        s[k + 1] *= as_ex2(fminf(vs.z + fv, 126.f));
-                    }
-                }
-                // P over S: hi planes in the first half of the columns, lo in the second
-#pragma unroll
-                for (int k = 0; k < HC; k += 16) {
-                    uint32_t ph[8], pl[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (C::NQ == 2) as_split(s[k + 2 * i], s[k + 2 * i + 1], ph[i], pl[i]);
-                        else ph[i] = as_pack<C::BF>(s[k + 2 * i], s[k + 2 * i + 1]);
-                    }
-                    as_st8(sb + (half * HC + k) / 2, ph);
-                    if (C::NQ == 2) as_st8(sb + KT / 2 + (half * HC + k) / 2, pl);
-                }
-                as_wait_st();
+                const int h0 = hi - half * HC, rb = off < ntp && !first ? acc_buf : -1;
+                if (__all_sync(0xffffffffu, h0 >= HC)) cnew = weigh(std::true_type{}, j, act, h0, rb);
+                else cnew = weigh(std::false_type{}, j, act, h0, rb);
             }
+            if (!first) fetch_o(j - 1);
+            as_wait_st();
             as_tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&m->p_full[bf]);
-            if (!first) add_o(j - 1);
+            if (lane == 0) as_arrive(&m->p_full[bf], ok);
+            if (!first) take_o(j - 1);
             cprev = cnew, prev_act = act, prev_any = any;
-            if (t + 1 < t1 && (t + 1) / tpg == kvh) continue;
+            const bool end = t + 1 == t1 || off + 1 == tpg;
+            if (C::ACC) {
+                kind = off >= ntp ? ADD : (end || off + 1 == ntp ? BRING : LEAVE);
+            }
+            if (++off == tpg) off = 0, ++kvh;
+            if (!end) continue;
 
             // ---- the segment's last tile: add it, then the output or a partial
-            add_o(j);
+            fetch_o(j);
+            take_o(j);
             m->lx[half][row] = lsum;
             as_pair_sync(1 + q4);
             float l = lsum + m->lx[half ^ 1][row];
@@ -830,42 +1008,47 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
             if (*(volatile int*)&m->fail) l = NAN;
             if (!live) continue;
             const int d0 = half * HD;
-            if (seg_t0 == kvh * tpg && t + 1 == (kvh + 1) * tpg) {
+            if (seg_t0 == cur * tpg && t + 1 == (cur + 1) * tpg) {
                 float inv = l == 0.f ? 0.f : 1.f / l;
                 if (C::KF32 && l != 0.f) inv *= exp2f(Mrun - mrun - OFF);
-                const size_t at = (size_t)(seq0 + sq) * a.out_sn + (size_t)(kvh * G + row % G) * a.out_sh + d0;
-                if constexpr (C::QF32) {
-                    float* dst = (float*)a.out + at;
+                const f2 inv2 = as_f2(inv, inv);
+                const size_t at = (size_t)(seq0 + sq) * a.out_sn + (size_t)(cur * G + row % G) * a.out_sh + d0;
 #pragma unroll
-                    for (int k = 0; k < HD; k += 4)
-                        if (d0 + k < a.hd)
-                            *(float4*)(dst + k) = make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
-                } else {
-                    uint16_t* dst = (uint16_t*)a.out + at;
+                for (int k = 0; k < HD; k += 8) {
+                    float x[8];
 #pragma unroll
-                    for (int k = 0; k < HD; k += 8)
-                        if (d0 + k < a.hd)
-                            *(uint4*)(dst + k) = make_uint4(as_pack<C::BF>(o[k] * inv, o[k + 1] * inv),
-                                                            as_pack<C::BF>(o[k + 2] * inv, o[k + 3] * inv),
-                                                            as_pack<C::BF>(o[k + 4] * inv, o[k + 5] * inv),
-                                                            as_pack<C::BF>(o[k + 6] * inv, o[k + 7] * inv));
+                    for (int i = 0; i < 4; ++i) as_un2(as_mul2(o[k / 2 + i], inv2), x[2 * i], x[2 * i + 1]);
+                    if constexpr (C::QF32) {
+                        float* dst = (float*)a.out + at + k;
+                        if (d0 + k < a.hd) *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
+                        if (d0 + k + 4 < a.hd) *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                    } else if (d0 + k < a.hd) {
+                        *(uint4*)((uint16_t*)a.out + at + k) =
+                            make_uint4(as_pack<C::BF>(x[0], x[1]), as_pack<C::BF>(x[2], x[3]),
+                                       as_pack<C::BF>(x[4], x[5]), as_pack<C::BF>(x[6], x[7]));
+                    }
                 }
             } else {
                 // slot 1: a run that began in an earlier kv head; slot 0: the others
-                const size_t ps = (size_t)blockIdx.x * 2 + (t0 < kvh * tpg ? 1 : 0);
+                const size_t ps = (size_t)blockIdx.x * 2 + (t0 < cur * tpg ? 1 : 0);
                 if (half == 0) a.part_ml[ps * AS_ROWS + row] = make_float4(mrun, l, C::KF32 ? Mrun - OFF : mrun, 0.f);
                 if (mrun != -INFINITY || isnan(l)) {
-                    float* dst = a.part_o + (ps * AS_ROWS + row) * 128 + d0;
+                    // [4 dims][128 rows]: neighbouring lanes write neighbouring addresses
+                    float4* dst = (float4*)a.part_o + (ps * 32 + d0 / 4) * AS_ROWS + row;
 #pragma unroll
                     for (int k = 0; k < HD; k += 4)
-                        if (d0 + k < a.hd) *(float4*)(dst + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        if (d0 + k < a.hd) {
+                            float x, y, z, w;
+                            as_un2(o[k / 2], x, y), as_un2(o[k / 2 + 1], z, w);
+                            dst[k / 4 * AS_ROWS] = make_float4(x, y, z, w);
+                        }
                 }
             }
         }
     }
     as_tc_before();
     __syncthreads();
-    if (warp == AS_MMA) {
+    if (warp == C::WARPS - 1) {
         as_tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
@@ -873,62 +1056,51 @@ __global__ void __launch_bounds__(AS_THREADS, 1) k_attn_shared(const __grid_cons
 }
 
 // Adds the partials of a (row tile, kv head) that several CTAs share, in CTA
-// order: out = sum O_i 2^(M_i - M) / sum l_i 2^(m_i - m) * 2^(M - m). One warp per row.
+// order: out = sum O_i 2^(M_i - M) / sum l_i 2^(m_i - m) * 2^(M - m) (integer
+// exponents). A warp takes 4 dims of 32 rows, a lane one row.
 template <typename OT, bool KF32>
 __global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ AttnSharedArgs a, int KT) {
     pdl_wait();
     const int lane = threadIdx.x & 31;
+    const int nd4 = (a.hd + 3) / 4;
     const int gw = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row = gw % AS_ROWS, kvh = gw / AS_ROWS % a.n_kv, rt = gw / AS_ROWS / a.n_kv;
+    const int d4 = gw % nd4, rb = gw / nd4 % (AS_ROWS / 32), g = gw / nd4 / (AS_ROWS / 32);
+    const int kvh = g % a.n_kv, rt = g / a.n_kv, row = rb * 32 + lane;
     const int n = a.n_dev ? *a.n_dev : a.n;
     const int prefix = a.prefix_dev ? (int)*a.prefix_dev : a.prefix;
     const int G = a.group, spt = AS_ROWS / G, seq = rt * spt + row / G;
-    if (row >= spt * G || seq >= n) return;
+    if (rt * spt >= n || rb * 32 >= min(spt, n - rt * spt) * G) return;
     const int tpg = (prefix + KT - 1) / KT + as_suffix_tiles(a, rt * spt, min(spt, n - rt * spt), prefix, KT);
     if (tpg == 0) return;
     const int b0 = a.plan[2 * rt], nb = a.plan[2 * rt + 1], total = tpg * a.n_kv;
     const int g0 = kvh * tpg, g1 = g0 + tpg;
-    const int i0 = (int)(((long long)(g0 + 1) * nb - 1) / total), i1 = (int)(((long long)g1 * nb - 1) / total);
+    const int i0 = as_part_of(g0, total, nb), i1 = as_part_of(g1 - 1, total, nb);
     if (as_part(i0, total, nb) <= g0 && as_part(i0 + 1, total, nb) >= g1) return;  // written by its one CTA
-    const int nseg = i1 - i0 + 1;
-    // lanes take segments: the maxima first
-    float m = -INFINITY, M = -INFINITY;
-    bool bad = false;
-    for (int i = lane; i < nseg; i += 32) {
-        const int s0 = as_part(i0 + i, total, nb), s1 = as_part(i0 + i + 1, total, nb);
-        if (s0 >= s1) continue;
-        const float4 x = a.part_ml[((size_t)(b0 + i0 + i) * 2 + (s0 < g0 ? 1 : 0)) * AS_ROWS + row];
-        m = fmaxf(m, x.x), M = fmaxf(M, x.z);
-        bad |= isnan(x.y);
-    }
-    m = warp_max(m), M = warp_max(M);
-    bad = __any_sync(0xffffffffu, bad);
-    float l = 0.f;
+    if (row >= spt * G || seq >= n) return;
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool on = 4 * lane < a.hd;
 #pragma unroll 4
-    for (int i = 0; i < nseg; ++i) {
-        const int s0 = as_part(i0 + i, total, nb), s1 = as_part(i0 + i + 1, total, nb);
+    for (int i = i0; i <= i1; ++i) {
+        const int s0 = as_part(i, total, nb), s1 = as_part(i + 1, total, nb);
         if (s0 >= s1) continue;
-        const size_t at = ((size_t)(b0 + i0 + i) * 2 + (s0 < g0 ? 1 : 0)) * AS_ROWS + row;
-        const float4 x = a.part_ml[at];
-        if (x.x == -INFINITY) continue;
-        l = fmaf(x.y, exp2f(x.x - m), l);
-        if (on) {
-            const float4 v = *(const float4*)(a.part_o + at * 128 + 4 * lane);
-            const float c = exp2f(x.z - M);
-            o.x = fmaf(v.x, c, o.x), o.y = fmaf(v.y, c, o.y), o.z = fmaf(v.z, c, o.z), o.w = fmaf(v.w, c, o.w);
-        }
+        const size_t ps = (size_t)(b0 + i) * 2 + (s0 < g0 ? 1 : 0);
+        const float4 x = a.part_ml[ps * AS_ROWS + row];
+        if (x.x == -INFINITY && !isnan(x.y)) continue;
+        const float4 v = ((const float4*)a.part_o)[(ps * 32 + d4) * AS_ROWS + row];
+        const float mn = fmaxf(m, x.x), Mn = fmaxf(M, x.z);
+        l = l * exp2f(m - mn) + x.y * exp2f(x.x - mn);
+        const float c = exp2f(M - Mn), cv = exp2f(x.z - Mn);
+        o.x = fmaf(v.x, cv, o.x * c), o.y = fmaf(v.y, cv, o.y * c);
+        o.z = fmaf(v.z, cv, o.z * c), o.w = fmaf(v.w, cv, o.w * c);
+        m = mn, M = Mn;
     }
     float inv = l == 0.f ? 0.f : 1.f / l;
     if (KF32 && l != 0.f) inv *= exp2f(M - m);
-    if (bad) inv = NAN;
-    if (!on) return;
-    const size_t at = (size_t)seq * a.out_sn + (size_t)(kvh * G + row % G) * a.out_sh + 4 * lane;
+    const size_t at = (size_t)seq * a.out_sn + (size_t)(kvh * G + row % G) * a.out_sh + 4 * d4;
     if constexpr (sizeof(OT) == 4) {
         *(float4*)((float*)a.out + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     } else {
-        constexpr bool BF = sizeof(OT) == 2 && !__is_same(OT, __half);
+        constexpr bool BF = std::is_same<OT, __nv_bfloat16>::value;
         *(uint2*)((uint16_t*)a.out + at) =
             make_uint2(as_pack<BF>(o.x * inv, o.y * inv), as_pack<BF>(o.z * inv, o.w * inv));
     }
@@ -957,21 +1129,69 @@ size_t attn_shared_work_bytes(int n, int group, int sms) {
     return cta * 2 * AS_ROWS * (16 + 128 * 4) + (size_t)as_row_tiles(n, group) * 8 + 256;
 }
 
+typedef CUresult (*AsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static AsEncodeFn g_as_encode = nullptr;  // set by attn_shared_configure
+
+// A map over [d3][d2][d1][d0] elements (strides in elements; a dimension of one
+// element gets a stride that any map accepts) with boxes of [1][b2][b1][b0].
+static cudaError_t as_map(CUtensorMap* out, CUtensorMapDataType type, int es, bool swizzle, const void* base, int rank,
+                          const uint64_t* dim, const uint64_t* stride, const uint32_t* box) {
+    cuuint64_t d[4], st[3];
+    cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) d[i] = dim[i], b[i] = box[i];
+    for (int i = 1; i < rank; ++i) st[i - 1] = dim[i] > 1 ? stride[i] * es : (dim[0] * es + 15) / 16 * 16;
+    const CUresult r = g_as_encode(out, type, rank, const_cast<void*>(base), d, st, b, one,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int MODE, int DP>
 static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
     using C = AsCfg<MODE, DP>;
     const int R = as_row_tiles(a.n, a.group), spt = AS_ROWS / a.group;
+    const CUtensorMapDataType type = C::KF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : C::BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    AsMaps maps{};
+    const int es = C::KF32 ? 4 : 2;
+    const uint32_t rows = C::KF32 ? AS_HALF : C::KT, cols = C::KF32 ? DP : 64;
+    cudaError_t e = cudaSuccess;
+    if (!C::QF32) {
+        const uint64_t d[3] = {(uint64_t)a.hd, (uint64_t)a.n_kv * a.group, (uint64_t)a.n}, st[3] = {1, a.q_sh, a.q_sn};
+        const uint32_t box[3] = {64, (uint32_t)a.group, (uint32_t)(spt < a.n ? spt : a.n)};
+        e = as_map(&maps.q, type, es, true, a.q, 3, d, st, box);
+    }
+    if (e == cudaSuccess && a.prefix) {
+        const uint64_t d[3] = {(uint64_t)a.hd, (uint64_t)a.n_kv, (uint64_t)a.prefix}, st[3] = {1, a.pre_sh, a.pre_st};
+        const uint32_t box[3] = {cols, 1, rows};
+        e = as_map(&maps.kp, type, es, !C::KF32, a.kp, 3, d, st, box);
+        if (e == cudaSuccess) e = as_map(&maps.vp, type, es, !C::KF32, a.vp, 3, d, st, box);
+    }
+    if (e == cudaSuccess && a.slot_len) {
+        const uint64_t d[4] = {(uint64_t)a.hd, (uint64_t)a.n_kv, (uint64_t)a.slot_len, (uint64_t)a.n_slots};
+        const uint64_t st[4] = {1, a.slot_sh, a.slot_st, a.slot_ss};
+        const uint32_t box[4] = {cols, 1, rows, 1};
+        e = as_map(&maps.k, type, es, !C::KF32, a.k, 4, d, st, box);
+        if (e == cudaSuccess) e = as_map(&maps.v, type, es, !C::KF32, a.v, 4, d, st, box);
+    }
+    if (e != cudaSuccess) return e;
     // Few tiles per (row tile, kv head): one CTA each, and no partials to add. A
-    // tile takes a CTA about 2 us with its latencies, the second kernel about 3.
+    // tile takes a CTA about 1 us with its latencies, the second kernel about 3.
     const long long most = (a.prefix + C::KT - 1) / C::KT +
                            (long long)(a.n < spt ? a.n : spt) * ((a.slot_len + C::KT - 1) / C::KT);
-    a.whole = !a.prefix_dev && most <= 3 && (long long)R * a.n_kv <= 0x7fffffff;
+    a.div_g = 65536 / a.group + 1;  // r * div_g >> 16 == r / group for r <= 128
+    a.whole = !a.prefix_dev && most <= 4 && (long long)R * a.n_kv <= 0x7fffffff;
     const int grid = a.whole ? R * a.n_kv : as_grid(a.n, a.group, sms);
-    k_attn_shared<MODE, DP><<<grid, AS_THREADS, C::SMEM, s>>>(a);
-    cudaError_t e = cudaGetLastError();
+    k_attn_shared<MODE, DP><<<grid, C::THREADS, C::SMEM, s>>>(a, maps);
+    e = cudaGetLastError();
     if (e != cudaSuccess || a.whole) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(R * a.n_kv * (AS_ROWS / 8)));
+    const long long warps = (long long)R * a.n_kv * (AS_ROWS / 32) * ((a.hd + 3) / 4);
+    cfg.gridDim = dim3((unsigned)((warps + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -1005,6 +1225,14 @@ static cudaError_t as_configure() {
                                 AsCfg<MODE, DP>::SMEM);
 }
 cudaError_t attn_shared_configure() {
+    if (!g_as_encode) {  // through the runtime's driver entry point (no link to libcuda)
+        cudaDriverEntryPointQueryResult q;
+        void* fn = nullptr;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q);
+        if (e != cudaSuccess) return e;
+        if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
+        g_as_encode = (AsEncodeFn)fn;
+    }
     cudaError_t e = as_configure<0, 64>();
     if (e == cudaSuccess) e = as_configure<0, 128>();
     if (e == cudaSuccess) e = as_configure<1, 64>();

@@ -81,7 +81,7 @@ struct AttnSharedArgs {
     int slot_row0;
     uint32_t* error;
     // set by launch_attn_shared
-    int whole;
+    int whole, div_g;
     float4* part_ml;
     float* part_o;
     int* plan;
