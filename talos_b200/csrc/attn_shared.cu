@@ -20,17 +20,18 @@
 // Per tile: S = Q K^T and O = P V on the 5th-generation tensor cores
 // (tcgen05.mma kind::f16, M 128), S and O in tensor memory, P written back over S
 // in 16 bits as the A operand. The softmax keeps a running maximum m, rounded up
-// to an integer (base 2), so every rescaling is by an exact power of two; O is
-// added up in registers in f32 (the tensor core only sums one tile: its
-// accumulation truncates).
+// to an integer (base 2), so every rescaling is by an exact power of two. For f32
+// outputs O is added up in registers (the tensor core only sums one tile: its
+// accumulation truncates); for 16-bit outputs it stays in tensor memory.
 //
 // Precision. f16 / bf16 queries: one product each, P rounded to 16 bits (half a
 // step of 2^-11 / 2^-8 relative per weight, averaged by the sum; the row sum uses
 // the unrounded weights), f32 everywhere else. f32 queries: q is scaled by a power
-// of two into [2^14, 2^15) at its largest element and split into f16 hi + lo (22
-// bits), and so is P; an f32 cache's rows too, with a power of two per key that
-// multiplies its score (K) or moves its weight's exponent (V), so no input
-// overflows f16 and small ones keep their bits. lo x lo (2^-22) is left out.
+// of two into [2^14, 2^15) at its row's largest element and split into f16 hi + lo
+// (22 bits), and so is P. An f32 cache's tiles are scaled (one power of two for 64
+// keys of K, and of V) and split too, so no input overflows f16; an element keeps
+// 22 bits, or 2^-39 of its tile's largest where that is more. lo x lo (2^-22) is
+// left out.
 //
 // Roles (one CTA per SM):
 //  * warps 0-7: softmax. Warps w and w + 4 share the rows 32 w .. 32 w + 31 (their
@@ -81,11 +82,13 @@ struct AsCfg {
     static constexpr int SOFT_REGS = KF32 ? 168 : 208, REST_REGS = 88;
     static constexpr int QPLANE = AS_ROWS * DP * 2, KPLANE = KT * DP * 2;
     static constexpr int RAW_HALF = AS_HALF * DP * 4;  // f32: one ring slot
-    static constexpr int NR = KF32 ? (DP == 128 ? 3 : 5) : 0;
-    // 16-bit outputs: the prefix's O is added up in tensor memory
+    static constexpr int NR = KF32 ? 5 : 0;
+    // 16-bit outputs: O is added up in tensor memory, in O buffer 0 (prefix tiles by
+    // the tensor core; suffix tiles go to buffer 1 and are added by their rows' warps,
+    // so that no other row meets their values)
     static constexpr bool ACC = !QF32;
     static constexpr int FIT = (AS_SMEM - AS_MISC - NQ * QPLANE) / KPLANE;  // 16-bit: operand tiles that fit
-    static constexpr int NSV = KF32 ? 2 : (FIT / 2 > 4 ? 4 : FIT / 2);
+    static constexpr int NSV = KF32 ? 1 : (FIT / 2 > 4 ? 4 : FIT / 2);
     static constexpr int NSK = KF32 ? 1 : (FIT - NSV > 4 ? 4 : FIT - NSV);
     static constexpr int SMEM = NQ * QPLANE + (NSK + NSV) * NK * KPLANE + NR * RAW_HALF + AS_MISC;
     static constexpr int S_COLS = KT;          // TMEM columns of one S buffer; P lies over it
@@ -103,10 +106,10 @@ struct AsMisc {
     int cum[AS_ROWS + 1];    // suffix tiles before each of the row tile's sequences
     int len[AS_ROWS], slot[AS_ROWS];
     float qsc[AS_ROWS];      // f32 queries: scale * log2(e) * 2^(exponent of the row)
-    float mx[2][2][AS_ROWS], mx2[2][2][AS_ROWS];  // [tile parity][half] row maxima
+    float mx[2][2][AS_ROWS];  // [tile parity][half] row maxima
     float lx[2][AS_ROWS];
-    alignas(16) float ksc[4][64];   // f32 cache: 2^(key's exponent)
-    alignas(16) float2 vsc[4][64];  // f32 cache: value row's exponent e and 2^e
+    float ksc[4], vsc[4];     // f32 cache: 2^exponent of a tile's keys, values
+    uint32_t cmax[2][8];      // f32 cache: largest |element| per converter warp (K, V)
 };
 static_assert(sizeof(AsMisc) <= AS_MISC, "misc area");
 
@@ -510,16 +513,16 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                        dv0 = as_desc(smem_u32(sV), KT * 128);
         int j = 0, seg = -1, cur = -1;
         uint32_t sk = 0, pk = 0, sv = 0, pv = 0;  // stage and its parity
-        uint32_t acc_buf = 0;       // ACC: O buffer of the segment's prefix tiles
         bool pre = false, pre0 = false;  // the tile whose PV comes next: of the prefix, the segment's first
         auto issue_pv = [&](int i) {  // tile i (counted from the CTA's first)
             const uint32_t bf = i & 1, par = (i >> 1) & 1;
             as_wait(m, &m->p_full[bf], par, ok);
             as_wait(m, &m->v_full[sv], pv, ok);
             as_wait(m, &m->o_empty[bf], par ^ 1, ok);
+            if (C::ACC && !pre && i > 0) as_wait(m, &m->o_empty[bf ^ 1], ((i - 1) >> 1) & 1, ok);  // one buffer
             as_tc_after();
             if (lead && ok) {
-                const uint32_t d = tmem + C::O_COL + (C::ACC && pre ? acc_buf : bf) * DP, p = tmem + bf * C::S_COLS;
+                const uint32_t d = tmem + C::O_COL + (C::ACC ? !pre : bf) * DP, p = tmem + bf * C::S_COLS;
                 const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
                 const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
                 // the small terms first
@@ -551,7 +554,6 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             }
             const uint32_t bf = j & 1;
             const bool is_pre = off < ntp;
-            const int first_off = off;
             as_wait(m, &m->k_full[sk], pk, ok);
             if (j >= 2) as_wait(m, &m->o_full[bf], ((j - 2) >> 1) & 1, ok);  // P over this S buffer was read
             as_tc_after();
@@ -579,8 +581,6 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             }
             if (++sk == C::NSK) sk = 0, pk ^= 1;
             if (!fresh) issue_pv(j - 1);
-            // the prefix's buffer is not that of the first suffix tile
-            if (fresh) acc_buf = (j + (is_pre ? min(ntp - first_off, t1 - t) : 0) + 1) & 1;
             pre = is_pre, pre0 = fresh;
         }
         issue_pv(j - 1);
@@ -676,75 +676,73 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         }
         __syncwarp();
     } else if (C::KF32 && warp >= 8) {
-        // ---------------------------------------------------- converters: ring -> scaled f16 hi + lo
+        // ---------------------------------------------------- converters: ring -> registers,
+        // the tile's largest element, -> scaled f16 hi + lo
         constexpr int QC = DP / 4, QR = 32 / QC;               // float4 chunks of a row, rows per warp step
-        constexpr int NI = (AS_HALF / QR + AS_CONV - 1) / AS_CONV;
+        constexpr int NI = (KT / QR + AS_CONV - 1) / AS_CONV;
         const int w = warp - 8, ch = lane % QC, sub = lane / QC;
+        uint8_t* dst0 = (ch / 16) * (KT * 128) + (ch & 1) * 8 + sK;
         uint32_t st = 0, par = 0;
         int j = 0;
         for (int t = t0, off = t0 % tpg; t < t1; ++t, ++j) {
             int i = 0, key = 0, valid = min(KT, prefix - off * KT);
             if (off >= ntp) valid = suffix(off, i, key);
 #pragma unroll 1
-            for (int h = 0; h < 4; ++h) {
-                const bool is_v = h >= 2;
-                const int r0 = (h & 1) * AS_HALF;
-                const bool have = r0 < valid;
-                if ((h & 1) == 0) {
-                    if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
-                    if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+            for (int is_v = 0; is_v < 2; ++is_v) {
+                const uint32_t s0 = st;
+                as_wait(m, &m->r_full[st], par, ok);
+                if (++st == C::NR) st = 0, par ^= 1;
+                const uint32_t s1 = st;
+                if (AS_HALF < valid) {
+                    as_wait(m, &m->r_full[st], par, ok);
+                    if (++st == C::NR) st = 0, par ^= 1;
                 }
+                const uint8_t *raw0 = sR + s0 * C::RAW_HALF + ch * 16, *raw1 = sR + s1 * C::RAW_HALF + ch * 16;
                 float4 v[NI];
-                if (have) as_wait(m, &m->r_full[st], par, ok);
+                float mx = 0.f;
 #pragma unroll
                 for (int q = 0; q < NI; ++q) {
                     const int r = (w + AS_CONV * q) * QR + sub;
                     v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
                     // rows behind the last key (the next ones of the slot, or stale) become zeros
-                    if (r < AS_HALF && r0 + r < valid)
-                        v[q] = *(const float4*)(sR + st * C::RAW_HALF + (r * QC + ch) * 16);
+                    if (r < valid) v[q] = *(const float4*)((r < AS_HALF ? raw0 : raw1) + r % AS_HALF * (QC * 16));
+                    mx = as_max3(mx, fabsf(v[q].x), fabsf(v[q].y));
+                    mx = as_max3(mx, fabsf(v[q].z), fabsf(v[q].w));
                 }
-                uint32_t mxb[NI];
+                const uint32_t own = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+                if (lane == 0) m->cmax[is_v][w] = own;
+                asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
+                // the ring's slots are free once their values have arrived, which the reduction
+                // waited for (an arrival may overtake loads that are still under way)
+                if (lane == 0) {
+                    as_arrive(&m->r_empty[s0], ok);
+                    if (AS_HALF < valid) as_arrive(&m->r_empty[s1], ok);
+                }
+                uint32_t all = m->cmax[is_v][0];
 #pragma unroll
-                for (int q = 0; q < NI; ++q) {
-                    mxb[q] = __float_as_uint(fmaxf(fmaxf(fabsf(v[q].x), fabsf(v[q].y)), fmaxf(fabsf(v[q].z), fabsf(v[q].w))));
-                    if constexpr (QR == 1) {
-                        mxb[q] = __reduce_max_sync(0xffffffffu, mxb[q]);
-                    } else {
-#pragma unroll
-                        for (int o = QC / 2; o > 0; o >>= 1) mxb[q] = max(mxb[q], __shfl_xor_sync(0xffffffffu, mxb[q], o));
-                    }
-                }
-                if (have) {
-                    // the slot is free once its values have arrived, which the reductions above
-                    // waited for (an arrival may overtake loads that are still under way)
-                    __syncwarp();
-                    if (lane == 0) as_arrive(&m->r_empty[st], ok);
-                    if (++st == C::NR) st = 0, par ^= 1;
-                }
+                for (int q = 1; q < AS_CONV; ++q) all = max(all, m->cmax[is_v][q]);
+                const int e = as_exponent(all);
+                const float f = as_pow2(14 - e);
+                const f2 ff = as_f2(f, f);
+                if (tid == 8 * 32) (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
+                if (j > 0) as_wait(m, is_v ? &m->v_empty[0] : &m->k_empty[0], (j - 1) & 1, ok);
+                uint8_t* base = dst0 + (is_v ? C::NSK * C::NK * C::KPLANE : 0);
 #pragma unroll
                 for (int q = 0; q < NI; ++q) {
                     const int r = (w + AS_CONV * q) * QR + sub;
-                    if (r >= AS_HALF) continue;
-                    const int e = as_exponent(mxb[q]), row = r0 + r;
-                    const float f = as_pow2(14 - e);
+                    if (r >= KT) continue;
+                    float x, y, z, u;
+                    as_un2(as_mul2(as_f2(v[q].x, v[q].y), ff), x, y), as_un2(as_mul2(as_f2(v[q].z, v[q].w), ff), z, u);
                     uint2 hi, lo;
-                    as_split_cut(v[q].x * f, v[q].y * f, hi.x, lo.x);
-                    as_split_cut(v[q].z * f, v[q].w * f, hi.y, lo.y);
-                    uint8_t* dst = (is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK) + (ch / 16) * (KT * 128) + row * 128 +
-                                   (((ch % 16 / 2) ^ (row & 7)) << 4) + (ch & 1) * 8;
+                    as_split_cut(x, y, hi.x, lo.x);
+                    as_split_cut(z, u, hi.y, lo.y);
+                    uint8_t* dst = base + r * 128 + (((ch % 16 / 2) ^ (r & 7)) << 4);
                     *(uint2*)dst = hi;
                     *(uint2*)(dst + C::KPLANE) = lo;
-                    if (ch == 0) {
-                        if (is_v) m->vsc[j & 3][row] = make_float2((float)(e - 14), as_pow2(e - 14));
-                        else m->ksc[j & 3][row] = as_pow2(e - 14);
-                    }
                 }
-                if (h & 1) {
-                    as_fence_async();
-                    __syncwarp();
-                    if (lane == 0) as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
-                }
+                as_fence_async();
+                __syncwarp();
+                if (lane == 0) as_arrive(is_v ? &m->v_full[0] : &m->k_full[0], ok);
             }
             if (++off == tpg) off = 0;
         }
@@ -758,10 +756,11 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const uint32_t lane_base = tmem + ((uint32_t)(q4 * 32) << 16);
         constexpr int HC = KT / 2, HD = DP / 2;  // this thread's keys of a tile, dims of the output
         constexpr float OFF = C::BF ? 0.f : 14.f;  // f16 weights: 2^14 at the maximum keeps small ones normal
-        f2 o[HD / 2];
-        float mrun = -INFINITY, Mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = a.scale * AS_LOG2E;
+        f2 o[C::ACC ? 1 : HD / 2];
+        float mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = a.scale * AS_LOG2E;
         bool prev_act = false, prev_any = false;
         const int own0 = live ? m->cum[sq] : 0, own = live ? m->len[sq] : 0;  // its first suffix tile, its keys
+        const uint32_t o_base = lane_base + C::O_COL + half * HD;
 
         // the queries of kv head kvh, scaled per row and split: 16 rows per warp
         auto load_q = [&](int kvh) {
@@ -807,84 +806,66 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_pair_sync(1 + q4);
             qs = m->qsc[row];
         };
-        // ACC, a prefix tile after the segment's first: O so far times cnew, in tensor memory
-        auto rescale = [&](int j, uint32_t buf, float c) {
-            as_wait(m, &m->o_full[(j - 1) & 1], ((j - 1) >> 1) & 1, ok);
-            as_tc_after();
-            const uint32_t at = lane_base + C::O_COL + buf * DP + half * HD;
+        // ACC: O (buffer 0) = O * c, or O * c + buffer 1 where `act`
+        auto rescale = [&](float c, bool add, bool act) {
+            const f2 c2 = as_f2(c, c);
 #pragma unroll 1
             for (int k = 0; k < HD; k += 8) {
-                uint32_t x[8];
-                as_ld8(at + k, x);
+                uint32_t x[8], y[8];
+                as_ld8(o_base + k, x);
+                if (add) as_ld8(o_base + DP + k, y);
                 as_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * c);
-                as_st8(at + k, x);
+                for (int i = 0; i < 8; i += 2) {
+                    const f2 v = as_f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    f2 r = as_mul2(v, c2);
+                    if (add && act) r = as_fma2(v, c2, as_f2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
+                    float p, q;
+                    as_un2(r, p, q);
+                    x[i] = __float_as_uint(p), x[i + 1] = __float_as_uint(q);
+                }
+                as_st8(o_base + k, x);
             }
+            as_wait_st();
         };
-        // scores of tile j -> weights; FULL: every row of the warp has all of its half's keys
-        auto weigh = [&](auto full_c, int j, bool act, int h0, int acc_buf) {  // acc_buf: rescale there, or < 0
+        // scores of tile j -> weights; FULL: every row of the warp has all of its half's keys.
+        // kq: the row's score factor (qs, times 2^exponent of an f32 tile); fix: an ACC prefix
+        // tile behind the segment's first, whose O so far is rescaled when a maximum grows
+        auto weigh = [&](auto full_c, int j, bool act, int h0, float kq, bool fix) {
             constexpr bool FULL = decltype(full_c)::value;
             const uint32_t bf = j & 1, sb = lane_base + bf * C::S_COLS;
             float s[HC];
 #pragma unroll
             for (int c = 0; c < HC; c += 32) as_ld32(sb + half * HC + c, s + c);
             as_wait_ld();
-            if (C::KF32) {
-#pragma unroll
-                for (int k = 0; k < HC; k += 4) {
-                    const float4 ks = *(const float4*)&m->ksc[j & 3][half * HC + k];
-                    as_un2(as_mul2(as_f2(s[k], s[k + 1]), as_f2(ks.x, ks.y)), s[k], s[k + 1]);
-                    as_un2(as_mul2(as_f2(s[k + 2], s[k + 3]), as_f2(ks.z, ks.w)), s[k + 2], s[k + 3]);
-                }
-            }
             if (!FULL) {
 #pragma unroll
                 for (int k = 0; k < HC; ++k) s[k] = k < h0 ? s[k] : -INFINITY;
             }
-            // (s stays unscaled; the scaled maximum is the maximum of the scaled, qs > 0)
-            float mt, Mt = -INFINITY;
-            {
-                float m2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // (s stays unscaled; the scaled maximum is the maximum of the scaled, kq > 0)
+            float m2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < HC; k += 8)
+            for (int k = 0; k < HC; k += 8)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) m2[q] = as_max3(m2[q], s[k + 2 * q], s[k + 2 * q + 1]);
-                mt = fmaxf(as_max3(m2[0], m2[1], m2[2]), m2[3]) * qs;
-            }
-            const f2 q2 = as_f2(qs, qs);
-            if (C::KF32) {
-#pragma unroll
-                for (int k = 0; k < HC; k += 2) {
-                    const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k];
-                    float x, y;
-                    as_un2(as_fma2(as_f2(s[k], s[k + 1]), q2, as_f2(vs.x, vs.z)), x, y);
-                    Mt = as_max3(Mt, x, y);
-                }
-            }
+                for (int q = 0; q < 4; ++q) m2[q] = as_max3(m2[q], s[k + 2 * q], s[k + 2 * q + 1]);
+            const float mt = fmaxf(as_max3(m2[0], m2[1], m2[2]), m2[3]) * kq;
             m->mx[bf][half][row] = mt;
-            if (C::KF32) m->mx2[bf][half][row] = Mt;
             as_pair_sync(1 + q4);  // (also: both halves of S are read, P may overwrite them)
-            float cnew = 1.f, fv = 0.f, fw = 0.f;
+            float cnew = 1.f;
             if (act) {
                 // integer exponents: exact powers of two (0 on the first tile)
                 const float mnew = fmaxf(mrun, ceilf(fmaxf(mt, m->mx[bf][half ^ 1][row])));
-                const float cl = as_ex2(mrun - mnew);
-                cnew = cl;
-                lsum *= cl;
+                cnew = as_ex2(mrun - mnew);
+                lsum *= cnew;
                 mrun = mnew;
-                if (C::KF32) {
-                    const float Mnew = fmaxf(Mrun, ceilf(fmaxf(Mt, m->mx2[bf][half ^ 1][row])));
-                    cnew = as_ex2(Mrun - Mnew);
-                    Mrun = Mnew;
-                    // 2^(m - M + OFF) as two factors: it may pass 2^127 where the values are tiny
-                    const float d = mnew - Mnew + OFF, d2 = floorf(0.5f * d);
-                    fv = as_ex2(d2), fw = as_ex2(d - d2);
-                }
             }
-            if (C::ACC && acc_buf >= 0 && __any_sync(0xffffffffu, cnew != 1.f)) rescale(j, acc_buf, cnew);
-            const float sub = C::KF32 ? mrun : mrun - OFF;
-            const f2 sub2 = as_f2(-sub, -sub);
+            if (C::ACC && fix && __any_sync(0xffffffffu, cnew != 1.f)) {
+                as_wait(m, &m->o_full[bf ^ 1], ((j - 1) >> 1) & 1, ok);
+                as_tc_after();
+                rescale(cnew, false, false);
+            }
+            const float sub = OFF - mrun;
+            const f2 q2 = as_f2(kq, kq), sub2 = as_f2(sub, sub);
             f2 l2[2] = {0ull, 0ull};
             // P over S: hi planes in the first half of the columns, lo in the second
 #pragma unroll
@@ -897,19 +878,8 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                     x = as_ex2(x), y = as_ex2(y);
                     if (!FULL) x = k + 2 * i < h0 ? x : 0.f, y = k + 2 * i + 1 < h0 ? y : 0.f;
                     l2[i & 1] = as_add2(l2[i & 1], as_f2(x, y));
-                    if (C::KF32) {
-                        // weight x 2^(its value row's exponent), relative to the running maximum M
-                        // (capped at 2^126: there the weight itself is below 2^-112, its share is lost either way)
-                        const float4 vs = *(const float4*)&m->vsc[j & 3][half * HC + k + 2 * i];
-                        x *= fminf(vs.y * fv * fw, 0x1p126f);
-                        y *= fminf(vs.w * fv * fw, 0x1p126f);
-                    }
-                    if (C::NP == 2) {
-                        if (C::BF) as_split_bf(x, y, ph[i], pl[i]);
-                        else as_split(x, y, ph[i], pl[i]);
-                    } else {
-                        ph[i] = as_pack<C::BF>(x, y);
-                    }
+                    if (C::NP == 2) as_split(x, y, ph[i], pl[i]);
+                    else ph[i] = as_pack<C::BF>(x, y);
                 }
                 as_st8(sb + (half * HC + k) / 2, ph);
                 if (C::NP == 2) as_st8(sb + KT / 2 + (half * HC + k) / 2, pl);
@@ -919,32 +889,28 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             lsum += x + y;
             return cnew;
         };
-
-        // what becomes of a tile's O: added to o[] while the next tile is worked on;
-        // ACC: left in tensor memory (prefix), or brought from there (the last prefix tile)
-        enum { ADD = 0, LEAVE = 1, BRING = 2 };
-        int kind = ADD, acc_buf = 0;
-        float x[HD];
-        auto fetch_o = [&](int i) {  // tile i's O on its way to x
+        // the O of tile i (of the prefix, or not) joins the row's
+        auto take_o = [&](int i, bool of_prefix) {
             as_wait(m, &m->o_full[i & 1], (i >> 1) & 1, ok);
             as_tc_after();
-            if (prev_any && kind != LEAVE) {
-                const uint32_t src = lane_base + C::O_COL + (C::ACC && kind == BRING ? acc_buf : i & 1) * DP + half * HD;
+            if constexpr (C::ACC) {
+                if (!of_prefix && prev_any) rescale(cprev, true, prev_act);
+            } else if (prev_any) {
+                // (an f32 tile's values come back to their scale here)
+                const float vs = C::KF32 ? m->vsc[i & 3] : 1.f;
+                const f2 c2 = as_f2(cprev, cprev), v2 = as_f2(vs, vs);
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) as_ld32(src + c, x + c);
-            }
-        };
-        auto take_o = [&](int i) {  // o = o * cprev + x
-            if (prev_any && kind != LEAVE) {
-                as_wait_ld();
-                if (prev_act) {
-                    const f2 c2 = as_f2(cprev, cprev);
-                    if (C::ACC && kind == BRING) {
+                for (int c = 0; c < HD; c += 32) {
+                    float x[32];
+                    as_ld32(o_base + (i & 1) * DP + c, x);
+                    as_wait_ld();
+                    if (prev_act) {
 #pragma unroll
-                        for (int k = 0; k < HD / 2; ++k) o[k] = as_f2(x[2 * k], x[2 * k + 1]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < HD / 2; ++k) o[k] = as_fma2(o[k], c2, as_f2(x[2 * k], x[2 * k + 1]));
+                        for (int k = 0; k < 16; ++k) {
+                            f2& d = o[c / 2 + k];
+                            const f2 xx = as_f2(x[2 * k], x[2 * k + 1]);
+                            d = C::KF32 ? as_fma2(xx, v2, as_mul2(d, c2)) : as_fma2(d, c2, xx);
+                        }
                     }
                 }
             }
@@ -954,20 +920,29 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         };
 
         int j = 0, cur = -1, seg_t0 = t0;
+        bool prev_pre = false;
         for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t, ++j) {
-            const bool first = kvh != cur;
+            const bool first = kvh != cur, of_prefix = off < ntp;
             if (first) {
                 cur = kvh, seg_t0 = t;
                 if constexpr (C::QF32) load_q(kvh);  // (the segment before is done with the last ones)
+                if constexpr (C::ACC) {
+                    if (!of_prefix) {  // no product of the prefix sets O
+                        const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+                        for (int k = 0; k < HD; k += 8) as_st8(o_base + k, zero);
+                        as_wait_st();
+                    }
+                } else {
 #pragma unroll
-                for (int k = 0; k < HD / 2; ++k) o[k] = 0ull;
-                mrun = Mrun = -INFINITY;
+                    for (int k = 0; k < HD / 2; ++k) o[k] = 0ull;
+                }
+                mrun = -INFINITY;
                 lsum = 0.f;
-                if (C::ACC) acc_buf = (j + (off < ntp ? min(ntp - off, t1 - t) : 0) + 1) & 1;
             }
             // the row's keys of this tile: the first hi
             int hi = 0;
-            if (off < ntp) {
+            if (of_prefix) {
                 if (live) hi = min(KT, prefix - off * KT);
             } else if (off - ntp >= own0) {
                 hi = (int)min((long long)KT, own - (long long)(off - ntp - own0) * KT);
@@ -976,72 +951,69 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             const bool any = __any_sync(0xffffffffu, act);
             const uint32_t bf = j & 1;
             as_wait(m, &m->s_full[bf], (j >> 1) & 1, ok);
-            if (C::KF32) as_wait(m, &m->v_full[bf], (j >> 1) & 1, ok);  // the values' exponents
             as_tc_after();
             float cnew = 1.f;
             if (any) {
-                const int h0 = hi - half * HC, rb = off < ntp && !first ? acc_buf : -1;
-                if (__all_sync(0xffffffffu, h0 >= HC)) cnew = weigh(std::true_type{}, j, act, h0, rb);
-                else cnew = weigh(std::false_type{}, j, act, h0, rb);
+                const int h0 = hi - half * HC;
+                const float kq = C::KF32 ? qs * m->ksc[j & 3] : qs;
+                const bool fix = of_prefix && !first;
+                if (__all_sync(0xffffffffu, h0 >= HC)) cnew = weigh(std::true_type{}, j, act, h0, kq, fix);
+                else cnew = weigh(std::false_type{}, j, act, h0, kq, fix);
             }
-            if (!first) fetch_o(j - 1);
             as_wait_st();
             as_tc_before();
             __syncwarp();
             if (lane == 0) as_arrive(&m->p_full[bf], ok);
-            if (!first) take_o(j - 1);
-            cprev = cnew, prev_act = act, prev_any = any;
+            if (!first) take_o(j - 1, prev_pre);
+            cprev = cnew, prev_act = act, prev_any = any, prev_pre = of_prefix;
             const bool end = t + 1 == t1 || off + 1 == tpg;
-            if (C::ACC) {
-                kind = off >= ntp ? ADD : (end || off + 1 == ntp ? BRING : LEAVE);
-            }
             if (++off == tpg) off = 0, ++kvh;
             if (!end) continue;
 
             // ---- the segment's last tile: add it, then the output or a partial
-            fetch_o(j);
-            take_o(j);
+            take_o(j, prev_pre);
             m->lx[half][row] = lsum;
             as_pair_sync(1 + q4);
             float l = lsum + m->lx[half ^ 1][row];
             as_pair_sync(1 + q4);
             if (*(volatile int*)&m->fail) l = NAN;
-            if (!live) continue;
             const int d0 = half * HD;
-            if (seg_t0 == cur * tpg && t + 1 == (cur + 1) * tpg) {
-                float inv = l == 0.f ? 0.f : 1.f / l;
-                if (C::KF32 && l != 0.f) inv *= exp2f(Mrun - mrun - OFF);
-                const f2 inv2 = as_f2(inv, inv);
-                const size_t at = (size_t)(seq0 + sq) * a.out_sn + (size_t)(cur * G + row % G) * a.out_sh + d0;
+            const bool whole = seg_t0 == cur * tpg && t + 1 == (cur + 1) * tpg;
+            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const f2 inv2 = as_f2(inv, inv);
+            // slot 1: a run that began in an earlier kv head; slot 0: the others
+            const size_t ps = (size_t)blockIdx.x * 2 + (t0 < cur * tpg ? 1 : 0);
+            const size_t at = (size_t)(seq0 + sq) * a.out_sn + (size_t)(cur * G + row % G) * a.out_sh + d0;
+            if (!whole && live && half == 0) a.part_ml[ps * AS_ROWS + row] = make_float2(mrun, l);
+            // (a row without keys here has no partial: mrun tells)
+            const bool put = live && (whole || mrun != -INFINITY || isnan(l));
 #pragma unroll
-                for (int k = 0; k < HD; k += 8) {
-                    float x[8];
+            for (int k = 0; k < HD; k += 8) {
+                float x[8];
+                if constexpr (C::ACC) {
+                    as_ld8(o_base + k, reinterpret_cast<uint32_t*>(x));
+                    as_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = l == 0.f ? 0.f : x[i] * inv;
+                } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) as_un2(as_mul2(o[k / 2 + i], inv2), x[2 * i], x[2 * i + 1]);
-                    if constexpr (C::QF32) {
-                        float* dst = (float*)a.out + at + k;
-                        if (d0 + k < a.hd) *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
-                        if (d0 + k + 4 < a.hd) *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
-                    } else if (d0 + k < a.hd) {
-                        *(uint4*)((uint16_t*)a.out + at + k) =
-                            make_uint4(as_pack<C::BF>(x[0], x[1]), as_pack<C::BF>(x[2], x[3]),
-                                       as_pack<C::BF>(x[4], x[5]), as_pack<C::BF>(x[6], x[7]));
-                    }
                 }
-            } else {
-                // slot 1: a run that began in an earlier kv head; slot 0: the others
-                const size_t ps = (size_t)blockIdx.x * 2 + (t0 < cur * tpg ? 1 : 0);
-                if (half == 0) a.part_ml[ps * AS_ROWS + row] = make_float4(mrun, l, C::KF32 ? Mrun - OFF : mrun, 0.f);
-                if (mrun != -INFINITY || isnan(l)) {
+                if (!put || d0 + k >= a.hd) continue;
+                const bool two = d0 + k + 4 < a.hd;
+                if (!whole) {
                     // [4 dims][128 rows]: neighbouring lanes write neighbouring addresses
-                    float4* dst = (float4*)a.part_o + (ps * 32 + d0 / 4) * AS_ROWS + row;
-#pragma unroll
-                    for (int k = 0; k < HD; k += 4)
-                        if (d0 + k < a.hd) {
-                            float x, y, z, w;
-                            as_un2(o[k / 2], x, y), as_un2(o[k / 2 + 1], z, w);
-                            dst[k / 4 * AS_ROWS] = make_float4(x, y, z, w);
-                        }
+                    float4* dst = a.part_o + (ps * 32 + (d0 + k) / 4) * AS_ROWS + row;
+                    dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    if (two) dst[AS_ROWS] = make_float4(x[4], x[5], x[6], x[7]);
+                } else if constexpr (C::QF32) {
+                    float* dst = (float*)a.out + at + k;
+                    *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
+                    if (two) *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+                    *(uint4*)((uint16_t*)a.out + at + k) =
+                        make_uint4(as_pack<C::BF>(x[0], x[1]), as_pack<C::BF>(x[2], x[3]), as_pack<C::BF>(x[4], x[5]),
+                                   as_pack<C::BF>(x[6], x[7]));
                 }
             }
         }
@@ -1056,9 +1028,9 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
 }
 
 // Adds the partials of a (row tile, kv head) that several CTAs share, in CTA
-// order: out = sum O_i 2^(M_i - M) / sum l_i 2^(m_i - m) * 2^(M - m) (integer
-// exponents). A warp takes 4 dims of 32 rows, a lane one row.
-template <typename OT, bool KF32>
+// order: out = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m) (integer exponents). A
+// warp takes 4 dims of 32 rows, a lane one row.
+template <typename OT>
 __global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ AttnSharedArgs a, int KT) {
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -1077,25 +1049,23 @@ __global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ Attn
     const int i0 = as_part_of(g0, total, nb), i1 = as_part_of(g1 - 1, total, nb);
     if (as_part(i0, total, nb) <= g0 && as_part(i0 + 1, total, nb) >= g1) return;  // written by its one CTA
     if (row >= spt * G || seq >= n) return;
-    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = i0; i <= i1; ++i) {
         const int s0 = as_part(i, total, nb), s1 = as_part(i + 1, total, nb);
         if (s0 >= s1) continue;
         const size_t ps = (size_t)(b0 + i) * 2 + (s0 < g0 ? 1 : 0);
-        const float4 x = a.part_ml[ps * AS_ROWS + row];
+        const float2 x = a.part_ml[ps * AS_ROWS + row];
         if (x.x == -INFINITY && !isnan(x.y)) continue;
-        const float4 v = ((const float4*)a.part_o)[(ps * 32 + d4) * AS_ROWS + row];
-        const float mn = fmaxf(m, x.x), Mn = fmaxf(M, x.z);
-        l = l * exp2f(m - mn) + x.y * exp2f(x.x - mn);
-        const float c = exp2f(M - Mn), cv = exp2f(x.z - Mn);
+        const float4 v = a.part_o[(ps * 32 + d4) * AS_ROWS + row];
+        const float mn = fmaxf(m, x.x), c = exp2f(m - mn), cv = exp2f(x.x - mn);
+        l = l * c + x.y * cv;
         o.x = fmaf(v.x, cv, o.x * c), o.y = fmaf(v.y, cv, o.y * c);
         o.z = fmaf(v.z, cv, o.z * c), o.w = fmaf(v.w, cv, o.w * c);
-        m = mn, M = Mn;
+        m = mn;
     }
-    float inv = l == 0.f ? 0.f : 1.f / l;
-    if (KF32 && l != 0.f) inv *= exp2f(M - m);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     const size_t at = (size_t)seq * a.out_sn + (size_t)(kvh * G + row % G) * a.out_sh + 4 * d4;
     if constexpr (sizeof(OT) == 4) {
         *(float4*)((float*)a.out + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -1123,10 +1093,10 @@ static int as_grid(int n, int group, int sms) {
     return r > sms ? r : sms;
 }
 
-// Workspace: [2 per CTA][128 rows] (m, l, M), the same rows' O, the row tiles' plan.
+// Workspace: [2 per CTA][128 rows] (m, l), the same rows' O, the row tiles' plan.
 size_t attn_shared_work_bytes(int n, int group, int sms) {
     const size_t cta = as_grid(n, group, sms);
-    return cta * 2 * AS_ROWS * (16 + 128 * 4) + (size_t)as_row_tiles(n, group) * 8 + 256;
+    return cta * 2 * AS_ROWS * (8 + 128 * 4) + (size_t)as_row_tiles(n, group) * 8 + 256;
 }
 
 typedef CUresult (*AsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -1201,14 +1171,14 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
     cfg.numAttrs = 1;
     using OT = typename std::conditional<MODE <= 1, float,
                                          typename std::conditional<MODE == 2, __half, __nv_bfloat16>::type>::type;
-    return cudaLaunchKernelEx(&cfg, k_attn_merge<OT, MODE == 0>, a, (int)C::KT);
+    return cudaLaunchKernelEx(&cfg, k_attn_merge<OT>, a, (int)C::KT);
 }
 
 cudaError_t launch_attn_shared(AttnSharedArgs a, int q_type, int kv_type, void* work, int sms, cudaStream_t s) {
     const size_t cta = as_grid(a.n, a.group, sms);
-    a.part_ml = (float4*)work;
-    a.part_o = (float*)((uint8_t*)work + cta * 2 * AS_ROWS * 16);
-    a.plan = (int*)((uint8_t*)work + cta * 2 * AS_ROWS * (16 + 128 * 4));
+    a.part_ml = (float2*)work;
+    a.part_o = (float4*)((uint8_t*)work + cta * 2 * AS_ROWS * 8);
+    a.plan = (int*)((uint8_t*)work + cta * 2 * AS_ROWS * (8 + 128 * 4));
     const bool wide = a.hd > 64;
     switch (as_mode(q_type, kv_type)) {
         case 0: return wide ? as_launch<0, 128>(a, sms, s) : as_launch<0, 64>(a, sms, s);

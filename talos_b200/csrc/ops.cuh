@@ -82,8 +82,8 @@ struct AttnSharedArgs {
     uint32_t* error;
     // set by launch_attn_shared
     int whole, div_g;
-    float4* part_ml;
-    float* part_o;
+    float2* part_ml;
+    float4* part_o;
     int* plan;
 };
 bool attn_shared_types(int q_type, int kv_type);
