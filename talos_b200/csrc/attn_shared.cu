@@ -36,19 +36,25 @@
 // Roles (one CTA per SM):
 //  * warps 0-7: softmax. Warps w and w + 4 share the rows 32 w .. 32 w + 31 (their
 //    TMEM lanes), one half of the tile's keys and of the head's dims each; they
-//    exchange row maxima in shared memory. f32 queries are scaled and split by them.
+//    exchange row maxima in shared memory. f32 queries come as they are; these warps
+//    scale and split them into tensor memory (as an operand from shared memory Q
+//    would be read again for every product: 6 KB instead of 2 per 128 x 64 x 16).
 //  * 16-bit caches, 12 warps: warp 8 issues the TMA copies of the K tiles and the
-//    queries, warp 9 those of the V tiles (both straight into the swizzled operand
-//    tiles; separate, so that K runs ahead of V), warp 10 clears the V rows behind a
-//    suffix's last key, which the copy brought along and which may hold anything.
-//  * f32 cache, 16 warps: warp 14 issues TMA copies of half tiles (32 rows) into a
-//    ring, warps 8-13 scale and split them into the operand tiles.
-//  * the last warp: TMEM allocation, and the MMAs: QK of tile j ahead of PV of tile
-//    j - 1, so that the softmax of one tile runs beside the products of its neighbours.
+//    queries, warp 9 those of the V tiles, straight into the swizzled operand tiles
+//    (separate, so that K runs ahead of V).
+//  * f32 cache, 16 warps: warp 13 fills a ring of 16 KB slots by TMA (the queries of a
+//    kv head, then half tiles, or whole ones of heads up to 64). Warps 8-12 scale and
+//    split the K tiles into the operand tile, the softmax warps the V tiles while they
+//    wait for a tile's scores (one group for both took 6600 cycles a tile).
+//  * the last two warps issue the MMAs: the last one (which allocates TMEM) S = Q K^T,
+//    a tile ahead of the other's O = P V, so that the softmax of one tile runs beside
+//    the products of its neighbours. Tiles that end early take fewer of both. The
+//    copies bring along the rows behind a suffix's last key, which may hold anything:
+//    the PV warp clears those V rows that its product reads.
 // Bound: HBM (the keys once) up to one row tile; above, the exponentials and the
 // tensor cores.
 //
-// Every wait is bounded (2 s); on expiry a CTA flag makes all roles run on without
+// Every wait is bounded; on expiry a CTA flag makes all roles run on without
 // waiting or multiplying, and the rows come out as NaN.
 #include <cuda.h>
 #include <math.h>
@@ -62,8 +68,8 @@ namespace talos {
 
 constexpr int AS_ROWS = 128;   // rows per tile = TMEM lanes
 constexpr int AS_SOFT = 8;     // softmax warps
-constexpr int AS_CONV = 6;     // f32: converter warps
-constexpr int AS_HALF = 32;    // f32: rows of a half tile
+constexpr int AS_CONV = 5;     // f32: converter warps
+constexpr int AS_SLOT = 16 * 1024;  // f32: one slot of the ring
 constexpr int AS_MISC = 12 * 1024;
 constexpr int AS_SMEM = 227 * 1024;
 constexpr float AS_LOG2E = 1.4426950408889634f;
@@ -80,36 +86,40 @@ struct AsCfg {
     static constexpr int THREADS = WARPS * 32;   // x 128 or 168 registers: the register file
     // registers after the split: 256 x 168 + 256 x 88 = 512 x 128, 256 x 208 + 128 x 88 = 384 x 168
     static constexpr int SOFT_REGS = KF32 ? 168 : 208, REST_REGS = 88;
-    static constexpr int QPLANE = AS_ROWS * DP * 2, KPLANE = KT * DP * 2;
-    static constexpr int RAW_HALF = AS_HALF * DP * 4;  // f32: one ring slot
-    static constexpr int NR = KF32 ? 5 : 0;
+    static constexpr int Q_BYTES = AS_ROWS * DP * (QF32 ? 4 : 2), KPLANE = KT * DP * 2;
+    static constexpr int HALF = AS_SLOT / (DP * 4);  // f32: rows of a ring slot, 32 or 64
+    static constexpr int NR = KF32 ? 7 : 0;
+    static constexpr int QB = Q_BYTES / AS_SLOT;     // f32: slots of the queries
     // 16-bit outputs: O is added up in tensor memory, in O buffer 0 (prefix tiles by
     // the tensor core; suffix tiles go to buffer 1 and are added by their rows' warps,
     // so that no other row meets their values)
     static constexpr bool ACC = !QF32;
-    static constexpr int FIT = (AS_SMEM - AS_MISC - NQ * QPLANE) / KPLANE;  // 16-bit: operand tiles that fit
-    static constexpr int NSV = KF32 ? 1 : (FIT / 2 > 4 ? 4 : FIT / 2);
+    static constexpr int Q_OWN = KF32 ? 0 : Q_BYTES;  // (f32: in the ring)
+    static constexpr int FIT = (AS_SMEM - AS_MISC - Q_OWN) / KPLANE;  // 16-bit: operand tiles that fit
+    static constexpr int NSV = KF32 ? 2 : (FIT / 2 > 4 ? 4 : FIT / 2);
     static constexpr int NSK = KF32 ? 1 : (FIT - NSV > 4 ? 4 : FIT - NSV);
-    static constexpr int SMEM = NQ * QPLANE + (NSK + NSV) * NK * KPLANE + NR * RAW_HALF + AS_MISC;
+    static constexpr int SMEM = Q_OWN + (NSK + NSV) * NK * KPLANE + NR * AS_SLOT + AS_MISC;
     static constexpr int S_COLS = KT;          // TMEM columns of one S buffer; P lies over it
-    static constexpr int O_COL = 2 * KT;       // first column of the two O buffers
+    static constexpr int O_COL = 2 * KT;       // first column of the O buffers
+    static constexpr int NOB = MODE == 1 ? 1 : 2;
+    static constexpr int Q_COL = O_COL + NOB * DP;  // f32 queries: hi, then lo
     static_assert(NSV >= 1 && SMEM <= AS_SMEM, "shared memory");
-    static_assert(2 * KT + 2 * DP <= 512, "tensor memory");
+    static_assert(Q_COL + (QF32 ? DP : 0) <= 512, "tensor memory");
 };
 
 struct AsMisc {
-    uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], v_raw[4], r_full[5], r_empty[5];
+    uint64_t q_raw[2], q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], r_full[8], r_empty[8];
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], done;
     uint32_t tmem;
     int fail;
+    uint32_t q_slot[2], q_par[2];  // f32: the first ring slot of the queries, its parity (two segments in flight at most)
     int rt, b0, nb, tpg;     // row tile of this CTA, its first CTA and CTA count, tiles per kv head
     int cum[AS_ROWS + 1];    // suffix tiles before each of the row tile's sequences
     int len[AS_ROWS], slot[AS_ROWS];
-    float qsc[AS_ROWS];      // f32 queries: scale * log2(e) * 2^(exponent of the row)
     float mx[2][2][AS_ROWS];  // [tile parity][half] row maxima
     float lx[2][AS_ROWS];
-    float ksc[4], vsc[4];     // f32 cache: 2^exponent of a tile's keys, values
-    uint32_t cmax[2][8];      // f32 cache: largest |element| per converter warp (K, V)
+    float ksc[4];             // f32 cache: 2^exponent of a tile's keys
+    alignas(16) uint32_t kmax[2][8], vmax[2][8];  // f32 cache: [tile parity] largest |element| of each converting warp
 };
 static_assert(sizeof(AsMisc) <= AS_MISC, "misc area");
 
@@ -266,26 +276,23 @@ __device__ __forceinline__ int as_exponent(uint32_t abs_bits) {
 }
 __device__ __forceinline__ float as_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// Bounded wait (2 s; the timer is read only after many polls, one read of it takes
-// about a microsecond). On expiry it marks the CTA as failed and `ok` as false:
-// the role then runs its loops to their end without waiting, copying, multiplying
-// or signalling (the pair barriers still match), and the others follow when their
-// own waits find the mark.
+// Bounded wait (4 M polls, each of which the hardware suspends for a while: a
+// second or so). On expiry it marks the CTA as failed and `ok` as false: the role
+// then runs its loops to their end without waiting, copying, multiplying or
+// signalling (the pair barriers still match), and the others follow when their own
+// waits find the mark. Kept small: it is inlined some thirty times, and what runs
+// in the roles' loops has to stay near in the instruction caches.
 __device__ __forceinline__ void as_wait(AsMisc* m, uint64_t* bar, uint32_t parity, bool& ok) {
     if (!ok) return;
-#pragma unroll 1
-    for (int i = 0; i < 4096; ++i)
-        if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = globaltimer_ns();
-    for (;;) {
-        if (*(volatile int*)&m->fail) break;
-#pragma unroll 1
-        for (int i = 0; i < 256; ++i)
-            if (mbar_try_wait(bar, parity)) return;
-        if (globaltimer_ns() - t0 > 2000000000ull) break;
+    uint32_t polls = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if (++polls & 4095) continue;
+        if (polls >= 1u << 22 || *(volatile int*)&m->fail) {
+            *(volatile int*)&m->fail = 1;
+            ok = false;
+            break;
+        }
     }
-    *(volatile int*)&m->fail = 1;
-    ok = false;
 }
 __device__ __forceinline__ void as_arrive(uint64_t* bar, bool ok) {
     if (ok) mbar_arrive(bar);
@@ -319,17 +326,27 @@ __device__ __forceinline__ int as_slot(const AttnSharedArgs& a, int seq) {
     return s >= 0 && s < a.n_slots ? s : -1;
 }
 
-// The sequence (within its row tile) that suffix tile t belongs to: the last one
-// that starts at or before it and has any (empty suffixes start where the next does).
-__device__ __forceinline__ int as_owner(const AsMisc* m, int nseq, int t) {
-    int lo = 0, hi = nseq;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (m->cum[mid] <= t) lo = mid;
-        else hi = mid;
+// A role's walk over its CTA's tiles: tile `off` of kv head `kvh`; its first key (of
+// the prefix, or of sequence i's suffix) and the number of its keys.
+struct AsWalk {
+    int off, kvh, i, key, valid;
+    __device__ __forceinline__ void start(int t0, int tpg) {
+        kvh = t0 / tpg, off = t0 - kvh * tpg, i = 0;
     }
-    return lo;
-}
+    __device__ __forceinline__ void tile(const AsMisc* m, int ntp, int prefix, int KT) {
+        if (off < ntp) {
+            key = off * KT;
+            valid = min(KT, prefix - key);
+        } else {
+            while (m->cum[i + 1] <= off - ntp) ++i;  // (past sequences without a suffix)
+            key = (off - ntp - m->cum[i]) * KT;
+            valid = min(KT, m->len[i] - key);
+        }
+    }
+    __device__ __forceinline__ void next(int tpg) {
+        if (++off == tpg) off = 0, ++kvh, i = 0;
+    }
+};
 // Suffix tiles of sequences seq0 .. seq0 + ns - 1, summed by a warp.
 __device__ __forceinline__ int as_suffix_tiles(const AttnSharedArgs& a, int seq0, int ns, int prefix, int KT) {
     int t = 0;
@@ -340,6 +357,55 @@ __device__ __forceinline__ int as_suffix_tiles(const AttnSharedArgs& a, int seq0
     return t;
 }
 
+// f32 tiles: NW warps take the rows of a raw tile (two ring slots of HALF rows, or
+// one) into registers, find the largest element, and store the tile scaled by
+// 2^(14 - e) as f16 hi and lo operand tiles.
+template <int DP, int KT, int NW>
+struct AsConv {
+    static constexpr int QC = DP / 4, QR = 32 / QC;  // float4 chunks of a row, rows per warp step
+    static constexpr int NI = (KT / QR + NW - 1) / NW, HALF = AS_SLOT / (DP * 4);
+    float4 v[NI];
+    // the warp's largest |element| as bits; rows behind the last key (the next ones of
+    // the slot, or stale) become zeros
+    __device__ __forceinline__ uint32_t load(const uint8_t* raw0, const uint8_t* raw1, int w, int lane, int valid) {
+        const int ch = lane % QC, sub = lane / QC;
+        float mx = 0.f;
+#pragma unroll
+        for (int q = 0; q < NI; ++q) {
+            const int r = (w + NW * q) * QR + sub;
+            v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < valid) v[q] = *(const float4*)((r < HALF ? raw0 : raw1) + r % HALF * (QC * 16) + ch * 16);
+        }
+#pragma unroll
+        for (int q = 0; q < NI; ++q) {
+            mx = as_max3(mx, fabsf(v[q].x), fabsf(v[q].y));
+            mx = as_max3(mx, fabsf(v[q].z), fabsf(v[q].w));
+        }
+        return __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+    }
+    __device__ __forceinline__ void store(uint8_t* tile, int w, int lane, int e) {
+        const int ch = lane % QC, sub = lane / QC;
+        const float f = as_pow2(14 - e);
+        const f2 ff = as_f2(f, f);
+        uint8_t* dst0 = tile + (ch / 16) * (KT * 128) + (ch & 1) * 8;
+#pragma unroll
+        for (int q = 0; q < NI; ++q) {
+            const int r = (w + NW * q) * QR + sub;
+            if (NI * NW * QR > KT && r >= KT) continue;
+            float x, y, z, u;
+            as_un2(as_mul2(as_f2(v[q].x, v[q].y), ff), x, y), as_un2(as_mul2(as_f2(v[q].z, v[q].w), ff), z, u);
+            uint2 hi, lo;
+            as_split_cut(x, y, hi.x, lo.x);
+            as_split_cut(z, u, hi.y, lo.y);
+            uint8_t* dst = dst0 + r * 128 + (((ch % 16 / 2) ^ (r & 7)) << 4);
+            *(uint2*)dst = hi;
+            *(uint2*)(dst + KT * DP * 2) = lo;
+        }
+        as_fence_async();
+        __syncwarp();
+    }
+};
+
 // ---------------------------------------------------------------- the kernel
 
 template <int MODE, int DP>
@@ -348,11 +414,11 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
     using C = AsCfg<MODE, DP>;
     constexpr int KT = C::KT, NB = DP / 64;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* sQ = smem;
-    uint8_t* sK = sQ + C::NQ * C::QPLANE;            // [NSK][planes]
+    uint8_t* sQ = smem;                              // f32 queries: [DP / 32][128 rows][32], else the operand
+    uint8_t* sK = sQ + C::Q_OWN;            // [NSK][planes]
     uint8_t* sV = sK + C::NSK * C::NK * C::KPLANE;   // [NSV][planes]
-    uint8_t* sR = sV + C::NSV * C::NK * C::KPLANE;   // f32: [NR] half tiles
-    AsMisc* m = (AsMisc*)(sR + C::NR * C::RAW_HALF);
+    uint8_t* sR = sV + C::NSV * C::NK * C::KPLANE;   // f32: [NR] ring slots
+    AsMisc* m = (AsMisc*)(sR + C::NR * AS_SLOT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const int n = a.n_dev ? *a.n_dev : a.n;
@@ -372,25 +438,26 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
     }
     if (tid >= 96 && tid < 101) {  // the call's tensor maps (those that it has)
         const int i = tid - 96;
-        if (i == 0 ? !C::QF32 : i < 3 ? a.prefix > 0 : a.slot_len > 0)
+        if (i == 0 || (i < 3 ? a.prefix > 0 : a.slot_len > 0))
             asm volatile("prefetch.tensormap [%0];" ::"l"((const CUtensorMap*)&maps + i) : "memory");
     }
     if (tid == 64) {
         m->fail = 0;
         mbar_init(&m->q_full, C::QF32 ? AS_SOFT : 1);
-        mbar_init(&m->q_empty, 1);
+        mbar_init(&m->q_raw[0], 1);
+        mbar_init(&m->q_raw[1], 1);
+        mbar_init(&m->q_empty, C::QF32 ? AS_SOFT : 1);
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             mbar_init(&m->k_full[i], C::KF32 ? AS_CONV : 1);
             mbar_init(&m->k_empty[i], 1);
-            mbar_init(&m->v_full[i], C::KF32 ? AS_CONV : 1);
+            mbar_init(&m->v_full[i], C::KF32 ? AS_SOFT : 1);
             mbar_init(&m->v_empty[i], 1);
-            mbar_init(&m->v_raw[i], 1);
         }
 #pragma unroll 1
-        for (int i = 0; i < 5; ++i) {
+        for (int i = 0; i < 8; ++i) {
             mbar_init(&m->r_full[i], 1);
-            mbar_init(&m->r_empty[i], AS_CONV);
+            mbar_init(&m->r_empty[i], 1);
         }
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -399,23 +466,19 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             mbar_init(&m->o_full[i], 1);
             mbar_init(&m->o_empty[i], AS_SOFT);
         }
-        mbar_init(&m->done, 1);
+        mbar_init(&m->done, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     int rt = 0, b0 = 0, nb = (int)gridDim.x;
     if (a.whole) {  // one CTA per (row tile, kv head)
         rt = (int)blockIdx.x / a.n_kv, b0 = rt * a.n_kv, nb = a.n_kv;
-    } else if (R == 1) {
-        if (blockIdx.x == 0 && tid == 0) a.plan[0] = 0, a.plan[1] = nb;
-    } else {
+    } else if (R > 1) {
         // CTAs in proportion to the row tiles' work: row tile r has CTAs b(r) ..
         // b(r + 1) - 1, b(r) = r + (N - R) * (tiles before r) / (all tiles)
         int* cnt = (int*)smem;  // [R] suffix tiles, before the operand tiles are used
-        for (int r = tid; r < R; r += C::THREADS) cnt[r] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += C::THREADS) {
-            const int len = as_len(a, i, prefix);
-            if (as_slot(a, i) >= 0 && len > 0) atomicAdd(&cnt[i / spt], (len + KT - 1) / KT);
+        for (int r = warp; r < R; r += C::WARPS) {
+            const int own = as_suffix_tiles(a, r * spt, min(spt, n - r * spt), prefix, KT);
+            if (lane == 0) cnt[r] = own;
         }
         __syncthreads();
         if (warp == 0) {
@@ -438,7 +501,6 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 }
                 const int lo = r + (int)(per * (double)(before + x - t)), hi = r + 1 + (int)(per * (double)(before + x));
                 if (r < R) {
-                    if (blockIdx.x == 0) a.plan[2 * r] = lo, a.plan[2 * r + 1] = hi - lo;
                     if ((int)blockIdx.x >= lo && (int)blockIdx.x < hi) m->rt = r, m->b0 = lo, m->nb = hi - lo;
                 }
                 before += __shfl_sync(0xffffffffu, x, 31);
@@ -482,6 +544,8 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
     const int rank = (int)blockIdx.x - b0;
     const int t0 = mine ? as_part(rank, total, nb) : 0, t1 = mine ? as_part(rank + 1, total, nb) : 0;
     const int rows = nseq * G;  // live rows
+    if (mine && rank == 0 && tid == 0 && !a.whole)
+        a.plan[3 * rt] = b0, a.plan[3 * rt + 1] = nb, a.plan[3 * rt + 2] = tpg;  // for k_attn_merge
     if (mine && tpg == 0 && rank == 0) {
         // no key in the whole row tile: zeros
         for (int i = tid; i < rows * a.n_kv * a.hd; i += C::THREADS) {
@@ -491,103 +555,138 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             else ((uint16_t*)a.out)[at] = 0;
         }
     }
-    // the sequence and the first key of suffix tile off (from a kv head's first tile), its valid keys
-    auto suffix = [&](int off, int& i, int& key) {
-        i = as_owner(m, nseq, off - ntp);
-        key = (off - ntp - m->cum[i]) * KT;
-        return min(KT, m->len[i] - key);
+    auto ring_step = [&](uint32_t& st, uint32_t& par, uint32_t by) {  // f32: on by up to NR slots
+        st += by;
+        if (st >= (uint32_t)(C::NR ? C::NR : 1)) st -= C::NR, par ^= 1;
     };
-
     bool ok = true;
+    // the queries of kv head kvh: their live rows, 128 bytes of each at a time
+    auto copy_q = [&](int kvh, int seg) {
+        constexpr int W = C::QF32 ? 32 : 64;
+        uint64_t* bar = C::QF32 ? &m->q_raw[seg & 1] : &m->q_full;
+        if (seg > 0) as_wait(m, &m->q_empty, (seg - 1) & 1, ok);
+        if (!ok) return;
+        mbar_expect_tx(bar, (uint32_t)(min(spt, a.n) * G) * 128 * (DP / W));
+#pragma unroll
+        for (int b = 0; b < DP / W; ++b)
+            as_tma3(smem_u32(sQ) + b * (AS_ROWS * 128), &maps.q, W * b, kvh * G, seq0, bar);
+    };
     if (t0 >= t1) {
         // nothing to do (TMEM is freed below)
     } else if (warp >= AS_SOFT) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
     if (warp == C::WARPS - 1) {
-        // ---------------------------------------------------- MMA issuer: the warp walks the
-        // tiles together (uniform control flow and descriptors), one lane issues
+        // ---------------------------------------------------- S = Q K^T: the warp walks the tiles
+        // together (uniform control flow and descriptors), one lane issues
         const bool lead = as_elect();
         const int ksteps = (a.hd + 15) / 16;
-        const uint32_t id_qk = as_idesc(KT, C::BF, false), id_pv = as_idesc(ksteps * 16, C::BF, true);
-        const uint64_t dq = as_desc(smem_u32(sQ), 16), dk0 = as_desc(smem_u32(sK), 16),
-                       dv0 = as_desc(smem_u32(sV), KT * 128);
+        const uint64_t dq = as_desc(smem_u32(sQ), 16), dk0 = as_desc(smem_u32(sK), 16);
         int j = 0, seg = -1, cur = -1;
-        uint32_t sk = 0, pk = 0, sv = 0, pv = 0;  // stage and its parity
-        bool pre = false, pre0 = false;  // the tile whose PV comes next: of the prefix, the segment's first
-        auto issue_pv = [&](int i) {  // tile i (counted from the CTA's first)
-            const uint32_t bf = i & 1, par = (i >> 1) & 1;
-            as_wait(m, &m->p_full[bf], par, ok);
-            as_wait(m, &m->v_full[sv], pv, ok);
-            as_wait(m, &m->o_empty[bf], par ^ 1, ok);
-            if (C::ACC && !pre && i > 0) as_wait(m, &m->o_empty[bf ^ 1], ((i - 1) >> 1) & 1, ok);  // one buffer
-            as_tc_after();
-            if (lead && ok) {
-                const uint32_t d = tmem + C::O_COL + (C::ACC ? !pre : bf) * DP, p = tmem + bf * C::S_COLS;
-                const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
-                const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
-                // the small terms first
-#pragma unroll
-                for (int pr = C::NP + C::NK - 2; pr >= 0; --pr) {
-                    const bool p_lo = C::NP == 2 && pr == 1, v_lo = pr == 2;
-                    const uint32_t pa = p + (p_lo ? KT / 2 : 0);
-                    const uint64_t vd = v + (v_lo ? C::KPLANE >> 4 : 0);
-#pragma unroll
-                    for (int ks = 0; ks < KT / 16; ++ks)
-                        as_mma_ts(d, pa + 8 * ks, vd + (uint64_t)(ks * 2048 >> 4), id_pv,
-                                  pr == C::NP + C::NK - 2 && ks == 0 ? keep : 1u);
-                }
-            }
-            __syncwarp();
-            if (lead && ok) {
-                as_commit(&m->v_empty[sv]);
-                as_commit(&m->o_full[bf]);
-            }
-            if (++sv == C::NSV) sv = 0, pv ^= 1;
-        };
-        for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t, ++j) {
-            const bool fresh = kvh != cur;
-            if (fresh) {
-                // the softmax warps finish a segment before they load the next one's queries
-                if (j > 0) issue_pv(j - 1);
-                cur = kvh, ++seg;
+        uint32_t sk = 0, pk = 0;  // stage and its parity
+        AsWalk w;
+        w.start(t0, tpg);
+        for (int t = t0; t < t1; ++t, ++j) {
+            if (w.kvh != cur) {
+                cur = w.kvh, ++seg;
                 as_wait(m, &m->q_full, seg & 1, ok);
             }
             const uint32_t bf = j & 1;
-            const bool is_pre = off < ntp;
+            w.tile(m, ntp, prefix, KT);
+            const uint32_t idesc = as_idesc((w.valid + 15) & ~15, C::BF, false);
             as_wait(m, &m->k_full[sk], pk, ok);
             if (j >= 2) as_wait(m, &m->o_full[bf], ((j - 2) >> 1) & 1, ok);  // P over this S buffer was read
             as_tc_after();
             if (lead && ok) {
                 const uint32_t d = tmem + bf * C::S_COLS;
                 const uint64_t k = dk0 + (uint64_t)(sk * (C::NK * C::KPLANE >> 4));
+                // the small terms first
 #pragma unroll
                 for (int pr = C::NQ + C::NK - 2; pr >= 0; --pr) {
                     const bool ql = C::NQ == 2 && pr == 1, kl = pr == 2;
-                    const uint64_t qd = dq + (ql ? C::QPLANE >> 4 : 0), kd = k + (kl ? C::KPLANE >> 4 : 0);
+                    const uint32_t first = pr == C::NQ + C::NK - 2 ? 0u : 1u;
+                    const uint64_t kd = k + (kl ? C::KPLANE >> 4 : 0);
 #pragma unroll
-                    for (int ks = 0; ks < DP / 16; ++ks)
-                        if (ks < ksteps)
-                            as_mma_ss(d, qd + (uint64_t)(((ks >> 2) * (AS_ROWS * 128) + (ks & 3) * 32) >> 4),
-                                      kd + (uint64_t)(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), id_qk,
-                                      pr == C::NQ + C::NK - 2 && ks == 0 ? 0u : 1u);
+                    for (int ks = 0; ks < DP / 16; ++ks) {
+                        if (ks >= ksteps) continue;
+                        const uint64_t ka = kd + (uint64_t)(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4);
+                        if (C::QF32)
+                            as_mma_ts(d, tmem + C::Q_COL + (ql ? DP / 2 : 0) + 8 * ks, ka, idesc, ks ? 1u : first);
+                        else
+                            as_mma_ss(d, dq + (uint64_t)(((ks >> 2) * (AS_ROWS * 128) + (ks & 3) * 32) >> 4), ka, idesc,
+                                      ks ? 1u : first);
+                    }
                 }
-            }
-            __syncwarp();
-            if (++off == tpg) off = 0, ++kvh;
-            if (lead && ok) {
                 as_commit(&m->k_empty[sk]);
                 as_commit(&m->s_full[bf]);
-                if (t + 1 == t1 || off == 0) as_commit(&m->q_empty);  // the queries may be replaced
+                if (!C::QF32 && (t + 1 == t1 || w.off + 1 == tpg)) as_commit(&m->q_empty);  // the queries may be replaced
             }
+            __syncwarp();
+            w.next(tpg);
             if (++sk == C::NSK) sk = 0, pk ^= 1;
-            if (!fresh) issue_pv(j - 1);
-            pre = is_pre, pre0 = fresh;
         }
-        issue_pv(j - 1);
         // nothing in flight when TMEM is freed (also after a failure: a wait of its own)
         if (lead) as_commit(&m->done);
         bool end_ok = true;
         as_wait(m, &m->done, 0, end_ok);
+    } else if (warp == C::WARPS - 2) {
+        // ---------------------------------------------------- O = P V
+        const bool lead = as_elect();
+        const uint32_t idesc = as_idesc((a.hd + 15) / 16 * 16, C::BF, true);
+        const uint64_t dv0 = as_desc(smem_u32(sV), KT * 128);
+        int j = 0, cur = -1, nsuf = 0;  // nsuf: ACC, suffix tiles so far
+        uint32_t sv = 0, pv = 0;
+        AsWalk w;
+        w.start(t0, tpg);
+        for (int t = t0; t < t1; ++t, ++j) {
+            const uint32_t bf = j & 1, par = (j >> 1) & 1;
+            const bool pre = w.off < ntp, pre0 = w.kvh != cur;
+            cur = w.kvh;
+            w.tile(m, ntp, prefix, KT);
+            const int valid = w.valid, ksteps = (valid + 15) / 16;
+            as_wait(m, &m->v_full[sv], pv, ok);
+            if (!C::KF32 && !pre && (valid & 15)) {
+                uint8_t* v = sV + sv * C::KPLANE;
+                for (int c = valid * 8 + lane; c < ksteps * 128; c += 32)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) *(uint4*)(v + b * (KT * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                as_fence_async();
+                __syncwarp();
+            }
+            // the O buffer is free: two in turn, one for all, or (ACC) one for the suffix tiles
+            if (C::ACC) {
+                if (!pre && nsuf > 0) as_wait(m, &m->o_empty[0], (nsuf - 1) & 1, ok);
+                nsuf += !pre;
+            } else if (C::NOB == 2) {
+                as_wait(m, &m->o_empty[bf], par ^ 1, ok);
+            } else if (j > 0) {
+                as_wait(m, &m->o_empty[0], (j - 1) & 1, ok);
+            }
+            as_wait(m, &m->p_full[bf], par, ok);
+            as_tc_after();
+            if (lead && ok) {
+                const uint32_t d = tmem + C::O_COL + (C::ACC ? !pre : C::NOB == 2 ? bf : 0) * DP, p = tmem + bf * C::S_COLS;
+                const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
+                const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
+                // the small terms first
+#pragma unroll
+                for (int pr = C::NP + C::NK - 2; pr >= 0; --pr) {
+                    const bool p_lo = C::NP == 2 && pr == 1, v_lo = pr == 2;
+                    const uint32_t pa = p + (p_lo ? KT / 2 : 0), first = pr == C::NP + C::NK - 2 ? keep : 1u;
+                    const uint64_t vd = v + (v_lo ? C::KPLANE >> 4 : 0);
+#pragma unroll
+                    for (int ks = 0; ks < KT / 16; ++ks) {
+                        if (ks >= ksteps) continue;
+                        as_mma_ts(d, pa + 8 * ks, vd + (uint64_t)(ks * 2048 >> 4), idesc, ks ? 1u : first);
+                    }
+                }
+                as_commit(&m->v_empty[sv]);
+                as_commit(&m->o_full[bf]);
+            }
+            __syncwarp();
+            w.next(tpg);
+            if (++sv == C::NSV) sv = 0, pv ^= 1;
+        }
+        if (lead) as_commit(&m->done);
     } else if (!C::KF32 && (warp == 8 || warp == 9)) {
         // ---------------------------------------------------- TMA: K (and 16-bit queries), V
         if (as_elect()) {
@@ -596,155 +695,132 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             uint64_t *full = is_v ? m->v_full : m->k_full, *empty = is_v ? m->v_empty : m->k_empty;
             const uint32_t ns = is_v ? C::NSV : C::NSK;
             const uint32_t base = smem_u32(is_v ? sV : sK);
-            const int q_box = min(spt, a.n) * G;  // rows of the query box
             uint32_t st = 0, par = 1;
             int seg = -1, cur = -1;
-            for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t) {
+            AsWalk w;
+            w.start(t0, tpg);
+            for (int t = t0; t < t1; ++t) {
+                w.tile(m, ntp, prefix, KT);
                 as_wait(m, &empty[st], par, ok);
-                int i = 0, key = 0, valid = KT;
-                if (off >= ntp) valid = suffix(off, i, key);
-                // rows behind the suffix's last one that the copy brings along: warp 10 clears them first
-                const bool fix = is_v && valid < KT && key + valid < a.slot_len;
-                uint64_t* bar = fix ? &m->v_raw[st] : &full[st];
                 if (ok) {
-                mbar_expect_tx(bar, C::KPLANE);
+                    mbar_expect_tx(&full[st], C::KPLANE);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint32_t dst = base + st * C::KPLANE + b * (KT * 128);
-                    if (off < ntp) as_tma3(dst, mp, 64 * b, kvh, off * KT, bar);
-                    else as_tma4(dst, ms, 64 * b, kvh, key, m->slot[i], bar);
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t dst = base + st * C::KPLANE + b * (KT * 128);
+                        if (w.off < ntp) as_tma3(dst, mp, 64 * b, w.kvh, w.key, &full[st]);
+                        else as_tma4(dst, ms, 64 * b, w.kvh, w.key, m->slot[w.i], &full[st]);
+                    }
                 }
-                }
-                if (!C::QF32 && !is_v && kvh != cur) {
-                    cur = kvh, ++seg;
-                    if (seg > 0) as_wait(m, &m->q_empty, (seg - 1) & 1, ok);
-                    if (ok) mbar_expect_tx(&m->q_full, (uint32_t)q_box * 128 * NB);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        if (ok) as_tma3(smem_u32(sQ) + b * (AS_ROWS * 128), &maps.q, 64 * b, kvh * G, seq0, &m->q_full);
-                }
+                if (!is_v && w.kvh != cur) cur = w.kvh, copy_q(w.kvh, ++seg);
                 if (++st == ns) st = 0, par ^= 1;
-                if (++off == tpg) off = 0, ++kvh;
+                w.next(tpg);
             }
             as_settle(ok);
         }
         __syncwarp();
-    } else if (!C::KF32 && warp == 10) {
-        // ---------------------------------------------------- V rows behind a suffix's last key: zeros
-        uint32_t st = 0, raw_par = 0;  // bit s: parity of v_raw[s]
-        for (int t = t0, off = t0 % tpg; t < t1; ++t) {
-            int i = 0, key = 0, valid = KT;
-            if (off >= ntp) valid = suffix(off, i, key);
-            if (valid < KT && key + valid < a.slot_len) {
-                as_wait(m, &m->v_raw[st], (raw_par >> st) & 1, ok);
-                raw_par ^= 1u << st;
-                uint8_t* v = sV + st * C::KPLANE;
-                for (int c = valid * 8 + lane; c < KT * 8; c += 32)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) *(uint4*)(v + b * (KT * 128) + c * 16) = make_uint4(0, 0, 0, 0);
-                as_fence_async();
-                __syncwarp();
-                if (lane == 0) as_arrive(&m->v_full[st], ok);
-            }
-            if (++st == C::NSV) st = 0;
-            if (++off == tpg) off = 0;
-        }
-    } else if (C::KF32 && warp == 14) {
-        // ---------------------------------------------------- f32 rows: TMA of half tiles into the ring
+    } else if (C::KF32 && warp == 13) {
+        // ---------------------------------------------------- f32: the ring's copies
         if (as_elect()) {
-            uint32_t st = 0, par = 1;
-            for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t) {
-                int i = 0, key = off * KT, valid = min(KT, prefix - off * KT);
-                if (off >= ntp) valid = suffix(off, i, key);
-#pragma unroll 1
-                for (int h = 0; h < 4; ++h) {  // K, K, V, V
-                    if ((h & 1) * AS_HALF >= valid) continue;
-                    as_wait(m, &m->r_empty[st], par, ok);
-                    if (!ok) continue;
-                    mbar_expect_tx(&m->r_full[st], C::RAW_HALF);
-                    const uint32_t dst = smem_u32(sR) + st * C::RAW_HALF;
-                    const int row = key + (h & 1) * AS_HALF;
-                    if (off < ntp) as_tma3(dst, h < 2 ? &maps.kp : &maps.vp, 0, kvh, row, &m->r_full[st]);
-                    else
-                        as_tma4(dst, h < 2 ? &maps.k : &maps.v, 0, kvh, row + a.slot_row0 * prefix, m->slot[i],
-                                &m->r_full[st]);
-                    if (++st == C::NR) st = 0, par ^= 1;
+            uint32_t st = 0, par = 0;            // the next slot, the parity of its data
+            uint32_t used = 0, re_par = 0;       // bit s: slot s held a tile before; parity of r_empty[s]
+            uint32_t held_q = 0, first_q = 0;    // bit s: it held queries (the first of them)
+            int seg = -1, cur = -1, q_done = 0;
+            auto slot_free = [&]() {
+                const uint32_t b = 1u << st;
+                if (held_q & b) {
+                    if (first_q & b) as_wait(m, &m->q_empty, q_done++ & 1, ok);
+                    held_q &= ~b, first_q &= ~b;
+                } else if (used & b) {
+                    as_wait(m, &m->r_empty[st], re_par >> st & 1, ok);
+                    re_par ^= b;
                 }
-                if (++off == tpg) off = 0, ++kvh;
+                used |= b;
+            };
+            auto next = [&]() {
+                if (++st == (uint32_t)C::NR) st = 0, par ^= 1;
+            };
+            AsWalk w;
+            w.start(t0, tpg);
+            for (int t = t0; t < t1; ++t) {
+                if (w.kvh != cur) {  // the queries of a kv head, 32 dims per slot
+                    cur = w.kvh, ++seg;
+#pragma unroll 1
+                    for (int b = 0; b < C::QB; ++b) {
+                        slot_free();
+                        if (b == 0) {
+                            m->q_slot[seg & 1] = st, m->q_par[seg & 1] = par;
+                            as_arrive(&m->q_raw[seg & 1], ok);
+                            first_q |= 1u << st;
+                        }
+                        held_q |= 1u << st;
+                        if (ok) {
+                            mbar_expect_tx(&m->r_full[st], (uint32_t)(min(spt, a.n) * G) * 128);
+                            as_tma3(smem_u32(sR) + st * AS_SLOT, &maps.q, 32 * b, w.kvh * G, seq0, &m->r_full[st]);
+                        }
+                        next();
+                    }
+                }
+                w.tile(m, ntp, prefix, KT);
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {  // K, then V
+                    if ((h & 1) * C::HALF >= w.valid) continue;
+                    slot_free();
+                    if (ok) {
+                        mbar_expect_tx(&m->r_full[st], AS_SLOT);
+                        const uint32_t dst = smem_u32(sR) + st * AS_SLOT;
+                        const int row = w.key + (h & 1) * C::HALF;
+                        if (w.off < ntp) as_tma3(dst, h < 2 ? &maps.kp : &maps.vp, 0, w.kvh, row, &m->r_full[st]);
+                        else
+                            as_tma4(dst, h < 2 ? &maps.k : &maps.v, 0, w.kvh, row + a.slot_row0 * prefix, m->slot[w.i],
+                                    &m->r_full[st]);
+                    }
+                    next();
+                }
+                w.next(tpg);
             }
             as_settle(ok);
         }
         __syncwarp();
-    } else if (C::KF32 && warp >= 8) {
-        // ---------------------------------------------------- converters: ring -> registers,
-        // the tile's largest element, -> scaled f16 hi + lo
-        constexpr int QC = DP / 4, QR = 32 / QC;               // float4 chunks of a row, rows per warp step
-        constexpr int NI = (KT / QR + AS_CONV - 1) / AS_CONV;
-        const int w = warp - 8, ch = lane % QC, sub = lane / QC;
-        uint8_t* dst0 = (ch / 16) * (KT * 128) + (ch & 1) * 8 + sK;
+    } else if constexpr (C::KF32) {
+        // ---------------------------------------------------- K tiles: ring -> operand tile
+        const int w = warp - 8;
+        int cur = -1, j = 0;
         uint32_t st = 0, par = 0;
-        int j = 0;
-        for (int t = t0, off = t0 % tpg; t < t1; ++t, ++j) {
-            int i = 0, key = 0, valid = min(KT, prefix - off * KT);
-            if (off >= ntp) valid = suffix(off, i, key);
-#pragma unroll 1
-            for (int is_v = 0; is_v < 2; ++is_v) {
-                const uint32_t s0 = st;
+        AsConv<DP, KT, AS_CONV> cv;
+        AsWalk wk;
+        wk.start(t0, tpg);
+        for (int t = t0; t < t1; ++t, ++j) {
+            wk.tile(m, ntp, prefix, KT);
+            const int valid = wk.valid;
+            const bool two = C::HALF < valid;
+            if (wk.kvh != cur) cur = wk.kvh, ring_step(st, par, C::QB);  // the queries' slots: the softmax warps'
+            const uint32_t s0 = st;
+            as_wait(m, &m->r_full[st], par, ok);
+            ring_step(st, par, 1);
+            const uint32_t s1 = st;
+            if (two) {
                 as_wait(m, &m->r_full[st], par, ok);
-                if (++st == C::NR) st = 0, par ^= 1;
-                const uint32_t s1 = st;
-                if (AS_HALF < valid) {
-                    as_wait(m, &m->r_full[st], par, ok);
-                    if (++st == C::NR) st = 0, par ^= 1;
-                }
-                const uint8_t *raw0 = sR + s0 * C::RAW_HALF + ch * 16, *raw1 = sR + s1 * C::RAW_HALF + ch * 16;
-                float4 v[NI];
-                float mx = 0.f;
-#pragma unroll
-                for (int q = 0; q < NI; ++q) {
-                    const int r = (w + AS_CONV * q) * QR + sub;
-                    v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    // rows behind the last key (the next ones of the slot, or stale) become zeros
-                    if (r < valid) v[q] = *(const float4*)((r < AS_HALF ? raw0 : raw1) + r % AS_HALF * (QC * 16));
-                    mx = as_max3(mx, fabsf(v[q].x), fabsf(v[q].y));
-                    mx = as_max3(mx, fabsf(v[q].z), fabsf(v[q].w));
-                }
-                const uint32_t own = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-                if (lane == 0) m->cmax[is_v][w] = own;
-                asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
-                // the ring's slots are free once their values have arrived, which the reduction
-                // waited for (an arrival may overtake loads that are still under way)
-                if (lane == 0) {
-                    as_arrive(&m->r_empty[s0], ok);
-                    if (AS_HALF < valid) as_arrive(&m->r_empty[s1], ok);
-                }
-                uint32_t all = m->cmax[is_v][0];
-#pragma unroll
-                for (int q = 1; q < AS_CONV; ++q) all = max(all, m->cmax[is_v][q]);
-                const int e = as_exponent(all);
-                const float f = as_pow2(14 - e);
-                const f2 ff = as_f2(f, f);
-                if (tid == 8 * 32) (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
-                if (j > 0) as_wait(m, is_v ? &m->v_empty[0] : &m->k_empty[0], (j - 1) & 1, ok);
-                uint8_t* base = dst0 + (is_v ? C::NSK * C::NK * C::KPLANE : 0);
-#pragma unroll
-                for (int q = 0; q < NI; ++q) {
-                    const int r = (w + AS_CONV * q) * QR + sub;
-                    if (r >= KT) continue;
-                    float x, y, z, u;
-                    as_un2(as_mul2(as_f2(v[q].x, v[q].y), ff), x, y), as_un2(as_mul2(as_f2(v[q].z, v[q].w), ff), z, u);
-                    uint2 hi, lo;
-                    as_split_cut(x, y, hi.x, lo.x);
-                    as_split_cut(z, u, hi.y, lo.y);
-                    uint8_t* dst = base + r * 128 + (((ch % 16 / 2) ^ (r & 7)) << 4);
-                    *(uint2*)dst = hi;
-                    *(uint2*)(dst + C::KPLANE) = lo;
-                }
-                as_fence_async();
-                __syncwarp();
-                if (lane == 0) as_arrive(is_v ? &m->v_full[0] : &m->k_full[0], ok);
+                ring_step(st, par, 1);
             }
-            if (++off == tpg) off = 0;
+            const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
+            if (lane == 0) m->kmax[j & 1][w] = own;
+            // (the slots are free once every warp's values have arrived, which the reductions
+            // waited for: an arrival may overtake loads that are still under way)
+            asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
+            uint32_t all = m->kmax[j & 1][0];
+#pragma unroll
+            for (int q = 1; q < AS_CONV; ++q) all = max(all, m->kmax[j & 1][q]);
+            const int e = as_exponent(all);
+            if (w == 0 && lane == 0) {
+                as_arrive(&m->r_empty[s0], ok);
+                if (two) as_arrive(&m->r_empty[s1], ok);
+                m->ksc[j & 3] = as_pow2(e - 14);
+            }
+            if (j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
+            cv.store(sK, w, lane, e);
+            if (lane == 0) as_arrive(&m->k_full[0], ok);
+            ring_step(st, par, two ? 2 : 1);  // the V tile's slots: the softmax warps'
+            wk.next(tpg);
         }
     }
     } else {
@@ -755,92 +831,95 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const bool live = row < rows;
         const uint32_t lane_base = tmem + ((uint32_t)(q4 * 32) << 16);
         constexpr int HC = KT / 2, HD = DP / 2;  // this thread's keys of a tile, dims of the output
-        constexpr float OFF = C::BF ? 0.f : 14.f;  // f16 weights: 2^14 at the maximum keeps small ones normal
+        constexpr float OFF = C::BF ? 0.f : C::ACC ? 6.f : 14.f;  // f16 weights: at most 2^14, small ones stay normal
         f2 o[C::ACC ? 1 : HD / 2];
         float mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = a.scale * AS_LOG2E;
         bool prev_act = false, prev_any = false;
-        const int own0 = live ? m->cum[sq] : 0, own = live ? m->len[sq] : 0;  // its first suffix tile, its keys
         const uint32_t o_base = lane_base + C::O_COL + half * HD;
 
-        // the queries of kv head kvh, scaled per row and split: 16 rows per warp
-        auto load_q = [&](int kvh) {
-            constexpr int QC = DP / 4, QR = 32 / QC, QI = 16 / QR, QB = 8;
-            const int ch = lane % QC;
-            const int r0 = q4 * 32 + half * 16 + lane / QC;
-            uint8_t* dst0 = sQ + (ch / 16) * (AS_ROWS * 128) + (ch & 1) * 8;
-#pragma unroll 1
-            for (int i0 = 0; i0 < QI; i0 += QB) {
-                float4 v[QB];
+        // the row's f32 queries (this thread's half of the dims), scaled and split into TMEM
+        auto load_q = [&](int seg) {
+            float4 v[HD / 4];
+            float mx = 0.f;
+            as_wait(m, &m->q_raw[seg & 1], (seg >> 1) & 1, ok);
+            const uint8_t* src[HD / 32];
 #pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    const int r = r0 + (i0 + i) * QR, rs = (r * a.div_g) >> 16;  // r / G
-                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < rows && 4 * ch < a.hd)
-                        v[i] = *(const float4*)((const float*)a.q + (size_t)(seq0 + rs) * a.q_sn +
-                                                (size_t)(kvh * G + r - rs * G) * a.q_sh + 4 * ch);
-                }
-#pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    const int r = r0 + (i0 + i) * QR;
-                    uint32_t b = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
-                    if constexpr (QR == 1) {
-                        b = __reduce_max_sync(0xffffffffu, b);
-                    } else {
-#pragma unroll
-                        for (int d = QC / 2; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
-                    }
-                    const int e = as_exponent(b);
-                    const float f = as_pow2(14 - e);
-                    uint2 hi, lo;
-                    as_split(v[i].x * f, v[i].y * f, hi.x, lo.x);
-                    as_split(v[i].z * f, v[i].w * f, hi.y, lo.y);
-                    uint8_t* dst = dst0 + r * 128 + (((ch % 16 / 2) ^ (r & 7)) << 4);
-                    *(uint2*)dst = hi;
-                    *(uint2*)(dst + C::QPLANE) = lo;
-                    if (ch == 0) m->qsc[r] = as_pow2(e - 14) * (a.scale * AS_LOG2E);
+            for (int b = 0; b < HD / 32; ++b) {
+                const uint32_t blk = half * (HD / 32) + b;
+                src[b] = sQ + blk * (AS_ROWS * 128);
+                if (C::KF32) {  // a ring slot
+                    uint32_t at = m->q_slot[seg & 1] + blk, par = m->q_par[seg & 1];
+                    ring_step(at, par, 0);
+                    as_wait(m, &m->r_full[at], par, ok);
+                    src[b] = sR + at * AS_SLOT;
                 }
             }
-            as_fence_async();
-            __syncwarp();
-            if (lane == 0) as_arrive(&m->q_full, ok);
+#pragma unroll
+            for (int c = 0; c < HD / 4; ++c) {
+                v[c] = *(const float4*)(src[c / 8] + row * 128 + ((c % 8 ^ (row & 7)) << 4));
+                mx = as_max3(mx, fabsf(v[c].x), fabsf(v[c].y));
+                mx = as_max3(mx, fabsf(v[c].z), fabsf(v[c].w));
+            }
+            m->mx[0][half][row] = mx;
             as_pair_sync(1 + q4);
-            qs = m->qsc[row];
+            mx = fmaxf(mx, m->mx[0][half ^ 1][row]);
+            const int e = as_exponent(__float_as_uint(mx));
+            const float f = as_pow2(14 - e);
+            qs = as_pow2(e - 14) * (a.scale * AS_LOG2E);
+            const uint32_t dst = lane_base + C::Q_COL + half * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < HD / 4; c += 4) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    as_split(v[c + i].x * f, v[c + i].y * f, hi[2 * i], lo[2 * i]);
+                    as_split(v[c + i].z * f, v[c + i].w * f, hi[2 * i + 1], lo[2 * i + 1]);
+                }
+                as_st8(dst + 2 * c, hi);
+                as_st8(dst + DP / 2 + 2 * c, lo);
+            }
+            as_wait_st();
+            as_tc_before();
+            __syncwarp();
+            if (lane == 0) {
+                as_arrive(&m->q_full, ok);
+                as_arrive(&m->q_empty, ok);
+            }
         };
         // ACC: O (buffer 0) = O * c, or O * c + buffer 1 where `act`
         auto rescale = [&](float c, bool add, bool act) {
             const f2 c2 = as_f2(c, c);
-#pragma unroll 1
-            for (int k = 0; k < HD; k += 8) {
-                uint32_t x[8], y[8];
-                as_ld8(o_base + k, x);
-                if (add) as_ld8(o_base + DP + k, y);
+#pragma unroll
+            for (int k = 0; k < HD; k += 32) {
+                float x[32], y[32];
+                as_ld32(o_base + k, x);
+                if (add) as_ld32(o_base + DP + k, y);
                 as_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const f2 v = as_f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    f2 r = as_mul2(v, c2);
-                    if (add && act) r = as_fma2(v, c2, as_f2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
-                    float p, q;
-                    as_un2(r, p, q);
-                    x[i] = __float_as_uint(p), x[i + 1] = __float_as_uint(q);
+                for (int i = 0; i < 32; i += 2) {
+                    f2 r = as_f2(x[i], x[i + 1]);
+                    if (add) r = act ? as_fma2(r, c2, as_f2(y[i], y[i + 1])) : r;
+                    else r = as_mul2(r, c2);
+                    as_un2(r, x[i], x[i + 1]);
                 }
-                as_st8(o_base + k, x);
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) as_st8(o_base + k + i, reinterpret_cast<uint32_t*>(x) + i);
             }
             as_wait_st();
         };
-        // scores of tile j -> weights; FULL: every row of the warp has all of its half's keys.
+        // scores of tile j -> weights of the rows that act, for the first h0 of this half's keys.
         // kq: the row's score factor (qs, times 2^exponent of an f32 tile); fix: an ACC prefix
         // tile behind the segment's first, whose O so far is rescaled when a maximum grows
-        auto weigh = [&](auto full_c, int j, bool act, int h0, float kq, bool fix) {
-            constexpr bool FULL = decltype(full_c)::value;
+        auto weigh = [&](int j, bool act, int h0, float kq, bool fix) {
             const uint32_t bf = j & 1, sb = lane_base + bf * C::S_COLS;
             float s[HC];
 #pragma unroll
             for (int c = 0; c < HC; c += 32) as_ld32(sb + half * HC + c, s + c);
             as_wait_ld();
-            if (!FULL) {
+            if (h0 < HC || !act) {
+                const int h = act ? h0 : 0;
 #pragma unroll
-                for (int k = 0; k < HC; ++k) s[k] = k < h0 ? s[k] : -INFINITY;
+                for (int k = 0; k < HC; ++k) s[k] = k < h ? s[k] : -INFINITY;
             }
             // (s stays unscaled; the scaled maximum is the maximum of the scaled, kq > 0)
             float m2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -853,8 +932,10 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_pair_sync(1 + q4);  // (also: both halves of S are read, P may overwrite them)
             float cnew = 1.f;
             if (act) {
-                // integer exponents: exact powers of two (0 on the first tile)
-                const float mnew = fmaxf(mrun, ceilf(fmaxf(mt, m->mx[bf][half ^ 1][row])));
+                // integer exponents: exact powers of two (0 on the first tile). ACC: the reference
+                // only moves when it is passed by 2^8, as O in tensor memory then moves too
+                const float top = ceilf(fmaxf(mt, m->mx[bf][half ^ 1][row]));
+                const float mnew = top > mrun + (C::ACC ? 8.f : 0.f) ? top : mrun;
                 cnew = as_ex2(mrun - mnew);
                 lsum *= cnew;
                 mrun = mnew;
@@ -864,7 +945,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_tc_after();
                 rescale(cnew, false, false);
             }
-            const float sub = OFF - mrun;
+            const float sub = act ? OFF - mrun : 0.f;  // (no weight where -inf)
             const f2 q2 = as_f2(kq, kq), sub2 = as_f2(sub, sub);
             f2 l2[2] = {0ull, 0ull};
             // P over S: hi planes in the first half of the columns, lo in the second
@@ -876,7 +957,6 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                     float x, y;
                     as_un2(as_fma2(as_f2(s[k + 2 * i], s[k + 2 * i + 1]), q2, sub2), x, y);
                     x = as_ex2(x), y = as_ex2(y);
-                    if (!FULL) x = k + 2 * i < h0 ? x : 0.f, y = k + 2 * i + 1 < h0 ? y : 0.f;
                     l2[i & 1] = as_add2(l2[i & 1], as_f2(x, y));
                     if (C::NP == 2) as_split(x, y, ph[i], pl[i]);
                     else ph[i] = as_pack<C::BF>(x, y);
@@ -890,19 +970,20 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             return cnew;
         };
         // the O of tile i (of the prefix, or not) joins the row's
+        float vscale = 1.f;  // f32: 2^exponent of the values of the tile that is taken
         auto take_o = [&](int i, bool of_prefix) {
+            if (C::ACC && of_prefix) return;
             as_wait(m, &m->o_full[i & 1], (i >> 1) & 1, ok);
             as_tc_after();
             if constexpr (C::ACC) {
-                if (!of_prefix && prev_any) rescale(cprev, true, prev_act);
+                if (prev_any) rescale(cprev, true, prev_act);
             } else if (prev_any) {
                 // (an f32 tile's values come back to their scale here)
-                const float vs = C::KF32 ? m->vsc[i & 3] : 1.f;
-                const f2 c2 = as_f2(cprev, cprev), v2 = as_f2(vs, vs);
+                const f2 c2 = as_f2(cprev, cprev), v2 = as_f2(vscale, vscale);
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {
                     float x[32];
-                    as_ld32(o_base + (i & 1) * DP + c, x);
+                    as_ld32(o_base + (C::NOB == 2 ? i & 1 : 0) * DP + c, x);
                     as_wait_ld();
                     if (prev_act) {
 #pragma unroll
@@ -916,16 +997,21 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             }
             as_tc_before();
             __syncwarp();
-            if (lane == 0) as_arrive(&m->o_empty[i & 1], ok);
+            if (lane == 0) as_arrive(&m->o_empty[C::ACC || C::NOB == 1 ? 0 : i & 1], ok);
         };
 
-        int j = 0, cur = -1, seg_t0 = t0;
+        int j = 0, cur = -1, seg = -1, seg_t0 = t0;
         bool prev_pre = false;
-        for (int t = t0, off = t0 % tpg, kvh = t0 / tpg; t < t1; ++t, ++j) {
-            const bool first = kvh != cur, of_prefix = off < ntp;
+        uint32_t st = 0, rpar = 0;       // f32: the ring
+        float vnext = 1.f;
+        AsWalk w;
+        w.start(t0, tpg);
+        for (int t = t0; t < t1; ++t, ++j) {
+            const bool first = w.kvh != cur, of_prefix = w.off < ntp;
+            w.tile(m, ntp, prefix, KT);
             if (first) {
-                cur = kvh, seg_t0 = t;
-                if constexpr (C::QF32) load_q(kvh);  // (the segment before is done with the last ones)
+                cur = w.kvh, seg_t0 = t;
+                if constexpr (C::QF32) load_q(++seg);  // (the segment before is done with the last ones)
                 if constexpr (C::ACC) {
                     if (!of_prefix) {  // no product of the prefix sets O
                         const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -940,38 +1026,61 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 mrun = -INFINITY;
                 lsum = 0.f;
             }
-            // the row's keys of this tile: the first hi
-            int hi = 0;
-            if (of_prefix) {
-                if (live) hi = min(KT, prefix - off * KT);
-            } else if (off - ntp >= own0) {
-                hi = (int)min((long long)KT, own - (long long)(off - ntp - own0) * KT);
+            if constexpr (C::KF32) {
+                const int valid = w.valid;
+                const bool two = C::HALF < valid;
+                if (first) ring_step(st, rpar, C::QB);
+                ring_step(st, rpar, two ? 2 : 1);  // the K tile's slots
+                const uint32_t s0 = st;
+                as_wait(m, &m->r_full[st], rpar, ok);
+                ring_step(st, rpar, 1);
+                const uint32_t s1 = st;
+                if (two) {
+                    as_wait(m, &m->r_full[st], rpar, ok);
+                    ring_step(st, rpar, 1);
+                }
+                AsConv<DP, KT, AS_SOFT> cv;
+                const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, warp, lane, valid);
+                if (lane == 0) m->vmax[j & 1][warp] = own;
+                asm volatile("bar.sync 6, %0;" ::"n"(AS_SOFT * 32) : "memory");
+                const uint4 v0 = *(const uint4*)&m->vmax[j & 1][0], v1 = *(const uint4*)&m->vmax[j & 1][4];
+                const int e = as_exponent(max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w))));
+                if (tid == 0) {
+                    as_arrive(&m->r_empty[s0], ok);
+                    if (two) as_arrive(&m->r_empty[s1], ok);
+                }
+                if (j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+                cv.store(sV + (j & 1) * (C::NK * C::KPLANE), warp, lane, e);
+                if (lane == 0) as_arrive(&m->v_full[j & 1], ok);
+                vnext = as_pow2(e - 14);
             }
-            const bool act = hi > 0;
+            // the row's keys of this tile: all, or none
+            const bool act = live && (of_prefix || sq == w.i);
             const bool any = __any_sync(0xffffffffu, act);
             const uint32_t bf = j & 1;
             as_wait(m, &m->s_full[bf], (j >> 1) & 1, ok);
             as_tc_after();
             float cnew = 1.f;
             if (any) {
-                const int h0 = hi - half * HC;
-                const float kq = C::KF32 ? qs * m->ksc[j & 3] : qs;
-                const bool fix = of_prefix && !first;
-                if (__all_sync(0xffffffffu, h0 >= HC)) cnew = weigh(std::true_type{}, j, act, h0, kq, fix);
-                else cnew = weigh(std::false_type{}, j, act, h0, kq, fix);
+                const float kq = C::KF32 ? fmaxf(qs * m->ksc[j & 3], 1e-37f) : qs;  // (above 0: -inf stays -inf)
+                cnew = weigh(j, act, w.valid - half * HC, kq, of_prefix && !first);
             }
             as_wait_st();
             as_tc_before();
             __syncwarp();
             if (lane == 0) as_arrive(&m->p_full[bf], ok);
             if (!first) take_o(j - 1, prev_pre);
-            cprev = cnew, prev_act = act, prev_any = any, prev_pre = of_prefix;
-            const bool end = t + 1 == t1 || off + 1 == tpg;
-            if (++off == tpg) off = 0, ++kvh;
+            cprev = cnew, prev_act = act, prev_any = any, prev_pre = of_prefix, vscale = vnext;
+            const bool end = t + 1 == t1 || w.off + 1 == tpg;
+            w.next(tpg);
             if (!end) continue;
 
             // ---- the segment's last tile: add it, then the output or a partial
             take_o(j, prev_pre);
+            if (C::ACC && prev_pre) {
+                as_wait(m, &m->o_full[j & 1], (j >> 1) & 1, ok);
+                as_tc_after();
+            }
             m->lx[half][row] = lsum;
             as_pair_sync(1 + q4);
             float l = lsum + m->lx[half ^ 1][row];
@@ -1031,7 +1140,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
 // order: out = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m) (integer exponents). A
 // warp takes 4 dims of 32 rows, a lane one row.
 template <typename OT>
-__global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ AttnSharedArgs a, int KT) {
+__global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ AttnSharedArgs a) {
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int nd4 = (a.hd + 3) / 4;
@@ -1039,30 +1148,47 @@ __global__ void __launch_bounds__(256) k_attn_merge(const __grid_constant__ Attn
     const int d4 = gw % nd4, rb = gw / nd4 % (AS_ROWS / 32), g = gw / nd4 / (AS_ROWS / 32);
     const int kvh = g % a.n_kv, rt = g / a.n_kv, row = rb * 32 + lane;
     const int n = a.n_dev ? *a.n_dev : a.n;
-    const int prefix = a.prefix_dev ? (int)*a.prefix_dev : a.prefix;
     const int G = a.group, spt = AS_ROWS / G, seq = rt * spt + row / G;
     if (rt * spt >= n || rb * 32 >= min(spt, n - rt * spt) * G) return;
-    const int tpg = (prefix + KT - 1) / KT + as_suffix_tiles(a, rt * spt, min(spt, n - rt * spt), prefix, KT);
+    const int b0 = a.plan[3 * rt], nb = a.plan[3 * rt + 1], tpg = a.plan[3 * rt + 2];
     if (tpg == 0) return;
-    const int b0 = a.plan[2 * rt], nb = a.plan[2 * rt + 1], total = tpg * a.n_kv;
+    const int total = tpg * a.n_kv;
     const int g0 = kvh * tpg, g1 = g0 + tpg;
     const int i0 = as_part_of(g0, total, nb), i1 = as_part_of(g1 - 1, total, nb);
     if (as_part(i0, total, nb) <= g0 && as_part(i0 + 1, total, nb) >= g1) return;  // written by its one CTA
     if (row >= spt * G || seq >= n) return;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = i0; i <= i1; ++i) {
-        const int s0 = as_part(i, total, nb), s1 = as_part(i + 1, total, nb);
-        if (s0 >= s1) continue;
-        const size_t ps = (size_t)(b0 + i) * 2 + (s0 < g0 ? 1 : 0);
-        const float2 x = a.part_ml[ps * AS_ROWS + row];
-        if (x.x == -INFINITY && !isnan(x.y)) continue;
-        const float4 v = a.part_o[(ps * 32 + d4) * AS_ROWS + row];
-        const float mn = fmaxf(m, x.x), c = exp2f(m - mn), cv = exp2f(x.x - mn);
-        l = l * c + x.y * cv;
-        o.x = fmaf(v.x, cv, o.x * c), o.y = fmaf(v.y, cv, o.y * c);
-        o.z = fmaf(v.z, cv, o.z * c), o.w = fmaf(v.w, cv, o.w * c);
+    // eight partials at a time, all their loads in flight (one that its CTA did not write is
+    // read and not used)
+    constexpr int MB = 8;
+    const int q = total / nb, rem = total - q * nb;
+    for (int i = i0; i <= i1; i += MB) {
+        float2 x[MB];
+        float4 v[MB];
+#pragma unroll
+        for (int k = 0; k < MB; ++k) {
+            const int ii = min(i + k, i1), s0 = ii * q + min(ii, rem);
+            const size_t ps = (size_t)(b0 + ii) * 2 + (s0 < g0 ? 1 : 0);
+            x[k] = a.part_ml[ps * AS_ROWS + row];
+            v[k] = a.part_o[(ps * 32 + d4) * AS_ROWS + row];
+            if (i + k > i1 || (q == 0 && ii >= rem)) x[k] = make_float2(-INFINITY, 0.f);  // none, or a CTA without tiles
+        }
+        float mn = m;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < MB; ++k) mn = fmaxf(mn, x[k].x), bad |= isnan(x[k].y);
+        const float c = mn == m ? 1.f : exp2f(m - mn);
+        l *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
+#pragma unroll
+        for (int k = 0; k < MB; ++k) {
+            const float cv = exp2f(x[k].x - mn);
+            if (x[k].x == -INFINITY) continue;
+            l = fmaf(x[k].y, cv, l);
+            o.x = fmaf(v[k].x, cv, o.x), o.y = fmaf(v[k].y, cv, o.y);
+            o.z = fmaf(v[k].z, cv, o.z), o.w = fmaf(v[k].w, cv, o.w);
+        }
+        if (bad) l = NAN;  // a CTA's wait ran out
         m = mn;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1096,7 +1222,7 @@ static int as_grid(int n, int group, int sms) {
 // Workspace: [2 per CTA][128 rows] (m, l), the same rows' O, the row tiles' plan.
 size_t attn_shared_work_bytes(int n, int group, int sms) {
     const size_t cta = as_grid(n, group, sms);
-    return cta * 2 * AS_ROWS * (8 + 128 * 4) + (size_t)as_row_tiles(n, group) * 8 + 256;
+    return cta * 2 * AS_ROWS * (8 + 128 * 4) + (size_t)as_row_tiles(n, group) * 12 + 256;
 }
 
 typedef CUresult (*AsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -1128,12 +1254,12 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     AsMaps maps{};
     const int es = C::KF32 ? 4 : 2;
-    const uint32_t rows = C::KF32 ? AS_HALF : C::KT, cols = C::KF32 ? DP : 64;
+    const uint32_t rows = C::KF32 ? C::HALF : C::KT, cols = C::KF32 ? DP : 64;
     cudaError_t e = cudaSuccess;
-    if (!C::QF32) {
+    {
         const uint64_t d[3] = {(uint64_t)a.hd, (uint64_t)a.n_kv * a.group, (uint64_t)a.n}, st[3] = {1, a.q_sh, a.q_sn};
-        const uint32_t box[3] = {64, (uint32_t)a.group, (uint32_t)(spt < a.n ? spt : a.n)};
-        e = as_map(&maps.q, type, es, true, a.q, 3, d, st, box);
+        const uint32_t box[3] = {C::QF32 ? 32u : 64u, (uint32_t)a.group, (uint32_t)(spt < a.n ? spt : a.n)};
+        e = as_map(&maps.q, C::QF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type, C::QF32 ? 4 : 2, true, a.q, 3, d, st, box);
     }
     if (e == cudaSuccess && a.prefix) {
         const uint64_t d[3] = {(uint64_t)a.hd, (uint64_t)a.n_kv, (uint64_t)a.prefix}, st[3] = {1, a.pre_sh, a.pre_st};
@@ -1153,7 +1279,6 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
     // tile takes a CTA about 1 us with its latencies, the second kernel about 3.
     const long long most = (a.prefix + C::KT - 1) / C::KT +
                            (long long)(a.n < spt ? a.n : spt) * ((a.slot_len + C::KT - 1) / C::KT);
-    a.div_g = 65536 / a.group + 1;  // r * div_g >> 16 == r / group for r <= 128
     a.whole = !a.prefix_dev && most <= 4 && (long long)R * a.n_kv <= 0x7fffffff;
     const int grid = a.whole ? R * a.n_kv : as_grid(a.n, a.group, sms);
     k_attn_shared<MODE, DP><<<grid, C::THREADS, C::SMEM, s>>>(a, maps);
@@ -1171,7 +1296,7 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
     cfg.numAttrs = 1;
     using OT = typename std::conditional<MODE <= 1, float,
                                          typename std::conditional<MODE == 2, __half, __nv_bfloat16>::type>::type;
-    return cudaLaunchKernelEx(&cfg, k_attn_merge<OT>, a, (int)C::KT);
+    return cudaLaunchKernelEx(&cfg, k_attn_merge<OT>, a);
 }
 
 cudaError_t launch_attn_shared(AttnSharedArgs a, int q_type, int kv_type, void* work, int sms, cudaStream_t s) {

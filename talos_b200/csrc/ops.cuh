@@ -81,7 +81,7 @@ struct AttnSharedArgs {
     int slot_row0;
     uint32_t* error;
     // set by launch_attn_shared
-    int whole, div_g;
+    int whole;
     float2* part_ml;
     float4* part_o;
     int* plan;
