@@ -42,10 +42,9 @@
 //  * 16-bit caches, 12 warps: warp 8 issues the TMA copies of the K tiles and the
 //    queries, warp 9 those of the V tiles, straight into the swizzled operand tiles
 //    (separate, so that K runs ahead of V).
-//  * f32 cache, 16 warps: warp 13 fills a ring of 16 KB slots by TMA (the queries of a
-//    kv head, then half tiles, or whole ones of heads up to 64). Warps 8-12 scale and
-//    split the K tiles into the operand tile, the softmax warps the V tiles while they
-//    wait for a tile's scores (one group for both took 6600 cycles a tile).
+//  * f32 cache, 20 warps: warp 17 fills a ring of 16 KB slots by TMA (the queries of a
+//    kv head, then half tiles, or whole ones of heads up to 64); warps 8-16 scale and
+//    split the tiles into the operand tiles.
 //  * the last two warps issue the MMAs: the last one (which allocates TMEM) S = Q K^T,
 //    a tile ahead of the other's O = P V, so that the softmax of one tile runs beside
 //    the products of its neighbours. Tiles that end early take fewer of both. The
@@ -68,7 +67,7 @@ namespace talos {
 
 constexpr int AS_ROWS = 128;   // rows per tile = TMEM lanes
 constexpr int AS_SOFT = 8;     // softmax warps
-constexpr int AS_CONV = 5;     // f32: converter warps
+constexpr int AS_CONV = 9;     // f32: converter warps
 constexpr int AS_SLOT = 16 * 1024;  // f32: one slot of the ring
 constexpr int AS_MISC = 12 * 1024;
 constexpr int AS_SMEM = 227 * 1024;
@@ -82,17 +81,17 @@ struct AsCfg {
     static constexpr int NP = QF32 ? 2 : 1;  // of P
     static constexpr int NK = KF32 ? 2 : 1;  // of K and V
     static constexpr int KT = KF32 ? 64 : 128;   // keys per tile
-    static constexpr int WARPS = KF32 ? 16 : 12;
-    static constexpr int THREADS = WARPS * 32;   // x 128 or 168 registers: the register file
-    // registers after the split: 256 x 168 + 256 x 88 = 512 x 128, 256 x 208 + 128 x 88 = 384 x 168
-    static constexpr int SOFT_REGS = KF32 ? 168 : 208, REST_REGS = 88;
+    static constexpr int WARPS = KF32 ? 20 : 12;
+    static constexpr int THREADS = WARPS * 32;   // x 96 or 168 registers at launch
+    // registers after the split: 256 x 152 + 384 x 56 <= 640 x 96, 256 x 208 + 128 x 88 = 384 x 168
+    static constexpr int SOFT_REGS = KF32 ? 152 : 208, REST_REGS = KF32 ? 56 : 88;
     static constexpr int Q_BYTES = AS_ROWS * DP * (QF32 ? 4 : 2), KPLANE = KT * DP * 2;
     static constexpr int HALF = AS_SLOT / (DP * 4);  // f32: rows of a ring slot, 32 or 64
     static constexpr int NR = KF32 ? 7 : 0;
     static constexpr int QB = Q_BYTES / AS_SLOT;     // f32: slots of the queries
-    // 16-bit outputs: O is added up in tensor memory, in O buffer 0 (prefix tiles by
-    // the tensor core; suffix tiles go to buffer 1 and are added by their rows' warps,
-    // so that no other row meets their values)
+    // 16-bit outputs: the prefix's O is added up in tensor memory, in O buffer 0. The
+    // rows' warps take it from there before their suffix tiles, whose products go to
+    // buffers 1, 0, 1, ... and are added in registers: no other row meets their values
     static constexpr bool ACC = !QF32;
     static constexpr int Q_OWN = KF32 ? 0 : Q_BYTES;  // (f32: in the ring)
     static constexpr int FIT = (AS_SMEM - AS_MISC - Q_OWN) / KPLANE;  // 16-bit: operand tiles that fit
@@ -118,8 +117,8 @@ struct AsMisc {
     int len[AS_ROWS], slot[AS_ROWS];
     float mx[2][2][AS_ROWS];  // [tile parity][half] row maxima
     float lx[2][AS_ROWS];
-    float ksc[4];             // f32 cache: 2^exponent of a tile's keys
-    alignas(16) uint32_t kmax[2][8], vmax[2][8];  // f32 cache: [tile parity] largest |element| of each converting warp
+    float ksc[4], vsc[4];     // f32 cache: 2^exponent of a tile's keys, values
+    uint32_t cmax[2][AS_CONV];  // f32 cache: largest |element| of each converter warp (K, V)
 };
 static_assert(sizeof(AsMisc) <= AS_MISC, "misc area");
 
@@ -451,7 +450,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         for (int i = 0; i < 4; ++i) {
             mbar_init(&m->k_full[i], C::KF32 ? AS_CONV : 1);
             mbar_init(&m->k_empty[i], 1);
-            mbar_init(&m->v_full[i], C::KF32 ? AS_SOFT : 1);
+            mbar_init(&m->v_full[i], C::KF32 ? AS_CONV : 1);
             mbar_init(&m->v_empty[i], 1);
         }
 #pragma unroll 1
@@ -633,7 +632,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const bool lead = as_elect();
         const uint32_t idesc = as_idesc((a.hd + 15) / 16 * 16, C::BF, true);
         const uint64_t dv0 = as_desc(smem_u32(sV), KT * 128);
-        int j = 0, cur = -1, nsuf = 0;  // nsuf: ACC, suffix tiles so far
+        int j = 0, cur = -1, nsuf = 0, ntaken = 0;  // ACC: suffix tiles of the segment, hand-overs before it
         uint32_t sv = 0, pv = 0;
         AsWalk w;
         w.start(t0, tpg);
@@ -654,8 +653,13 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             }
             // the O buffer is free: two in turn, one for all, or (ACC) one for the suffix tiles
             if (C::ACC) {
-                if (!pre && nsuf > 0) as_wait(m, &m->o_empty[0], (nsuf - 1) & 1, ok);
-                nsuf += !pre;
+                // hand-overs of a buffer, counted over the CTA: the prefix's O, then each suffix
+                // tile's; suffix tile k of a segment waits for hand-over k - 1
+                if (pre0) ntaken += nsuf ? nsuf + 1 : 0, nsuf = 0;
+                if (!pre && nsuf > 0) {
+                    const int h = ntaken + nsuf - 1;
+                    as_wait(m, &m->o_empty[h & 1], (h >> 1) & 1, ok);
+                }
             } else if (C::NOB == 2) {
                 as_wait(m, &m->o_empty[bf], par ^ 1, ok);
             } else if (j > 0) {
@@ -664,7 +668,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_wait(m, &m->p_full[bf], par, ok);
             as_tc_after();
             if (lead && ok) {
-                const uint32_t d = tmem + C::O_COL + (C::ACC ? !pre : C::NOB == 2 ? bf : 0) * DP, p = tmem + bf * C::S_COLS;
+                const uint32_t d = tmem + C::O_COL + (C::ACC ? (pre ? 0 : (nsuf & 1) ^ 1) : C::NOB == 2 ? bf : 0) * DP, p = tmem + bf * C::S_COLS;
                 const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
                 const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
                 // the small terms first
@@ -682,6 +686,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_commit(&m->v_empty[sv]);
                 as_commit(&m->o_full[bf]);
             }
+            if (C::ACC) nsuf += !pre;
             __syncwarp();
             w.next(tpg);
             if (++sv == C::NSV) sv = 0, pv ^= 1;
@@ -718,7 +723,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_settle(ok);
         }
         __syncwarp();
-    } else if (C::KF32 && warp == 13) {
+    } else if (C::KF32 && warp == 8 + AS_CONV) {
         // ---------------------------------------------------- f32: the ring's copies
         if (as_elect()) {
             uint32_t st = 0, par = 0;            // the next slot, the parity of its data
@@ -782,7 +787,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         }
         __syncwarp();
     } else if constexpr (C::KF32) {
-        // ---------------------------------------------------- K tiles: ring -> operand tile
+        // ---------------------------------------------------- ring -> operand tiles
         const int w = warp - 8;
         int cur = -1, j = 0;
         uint32_t st = 0, par = 0;
@@ -794,32 +799,33 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             const int valid = wk.valid;
             const bool two = C::HALF < valid;
             if (wk.kvh != cur) cur = wk.kvh, ring_step(st, par, C::QB);  // the queries' slots: the softmax warps'
-            const uint32_t s0 = st;
-            as_wait(m, &m->r_full[st], par, ok);
-            ring_step(st, par, 1);
-            const uint32_t s1 = st;
-            if (two) {
+#pragma unroll 1
+            for (int is_v = 0; is_v < 2; ++is_v) {
+                const uint32_t s0 = st;
                 as_wait(m, &m->r_full[st], par, ok);
                 ring_step(st, par, 1);
+                const uint32_t s1 = st;
+                if (two) {
+                    as_wait(m, &m->r_full[st], par, ok);
+                    ring_step(st, par, 1);
+                }
+                const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
+                if (lane == 0) m->cmax[is_v][w] = own;
+                // (the slots are free once every warp's values have arrived, which the reductions
+                // waited for: an arrival may overtake loads that are still under way)
+                asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
+                const uint32_t all = __reduce_max_sync(0xffffffffu, m->cmax[is_v][lane < AS_CONV ? lane : 0]);
+                const int e = as_exponent(all);
+                if (w == 0 && lane == 0) {
+                    as_arrive(&m->r_empty[s0], ok);
+                    if (two) as_arrive(&m->r_empty[s1], ok);
+                    (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
+                }
+                if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
+                if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+                cv.store(is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK, w, lane, e);
+                if (lane == 0) as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
             }
-            const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
-            if (lane == 0) m->kmax[j & 1][w] = own;
-            // (the slots are free once every warp's values have arrived, which the reductions
-            // waited for: an arrival may overtake loads that are still under way)
-            asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
-            uint32_t all = m->kmax[j & 1][0];
-#pragma unroll
-            for (int q = 1; q < AS_CONV; ++q) all = max(all, m->kmax[j & 1][q]);
-            const int e = as_exponent(all);
-            if (w == 0 && lane == 0) {
-                as_arrive(&m->r_empty[s0], ok);
-                if (two) as_arrive(&m->r_empty[s1], ok);
-                m->ksc[j & 3] = as_pow2(e - 14);
-            }
-            if (j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
-            cv.store(sK, w, lane, e);
-            if (lane == 0) as_arrive(&m->k_full[0], ok);
-            ring_step(st, par, two ? 2 : 1);  // the V tile's slots: the softmax warps'
             wk.next(tpg);
         }
     }
@@ -832,7 +838,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const uint32_t lane_base = tmem + ((uint32_t)(q4 * 32) << 16);
         constexpr int HC = KT / 2, HD = DP / 2;  // this thread's keys of a tile, dims of the output
         constexpr float OFF = C::BF ? 0.f : C::ACC ? 6.f : 14.f;  // f16 weights: at most 2^14, small ones stay normal
-        f2 o[C::ACC ? 1 : HD / 2];
+        f2 o[HD / 2];
         float mrun = -INFINITY, lsum = 0.f, cprev = 1.f, qs = a.scale * AS_LOG2E;
         bool prev_act = false, prev_any = false;
         const uint32_t o_base = lane_base + C::O_COL + half * HD;
@@ -886,26 +892,31 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_arrive(&m->q_empty, ok);
             }
         };
-        // ACC: O (buffer 0) = O * c, or O * c + buffer 1 where `act`
-        auto rescale = [&](float c, bool add, bool act) {
+        // ACC: the prefix's O (buffer 0) times c
+        auto rescale = [&](float c) {
             const f2 c2 = as_f2(c, c);
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < HD; k += 32) {
-                float x[32], y[32];
+                float x[32];
                 as_ld32(o_base + k, x);
-                if (add) as_ld32(o_base + DP + k, y);
                 as_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    f2 r = as_f2(x[i], x[i + 1]);
-                    if (add) r = act ? as_fma2(r, c2, as_f2(y[i], y[i + 1])) : r;
-                    else r = as_mul2(r, c2);
-                    as_un2(r, x[i], x[i + 1]);
-                }
+                for (int i = 0; i < 32; i += 2) as_un2(as_mul2(as_f2(x[i], x[i + 1]), c2), x[i], x[i + 1]);
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) as_st8(o_base + k + i, reinterpret_cast<uint32_t*>(x) + i);
             }
             as_wait_st();
+        };
+        // ACC: the prefix's O into registers
+        auto bring = [&]() {
+#pragma unroll
+            for (int k = 0; k < HD; k += 32) {
+                float x[32];
+                as_ld32(o_base + k, x);
+                as_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[k / 2 + i] = as_f2(x[2 * i], x[2 * i + 1]);
+            }
         };
         // scores of tile j -> weights of the rows that act, for the first h0 of this half's keys.
         // kq: the row's score factor (qs, times 2^exponent of an f32 tile); fix: an ACC prefix
@@ -943,7 +954,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             if (C::ACC && fix && __any_sync(0xffffffffu, cnew != 1.f)) {
                 as_wait(m, &m->o_full[bf ^ 1], ((j - 1) >> 1) & 1, ok);
                 as_tc_after();
-                rescale(cnew, false, false);
+                rescale(cnew);
             }
             const float sub = act ? OFF - mrun : 0.f;  // (no weight where -inf)
             const f2 q2 = as_f2(kq, kq), sub2 = as_f2(sub, sub);
@@ -969,21 +980,22 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             lsum += x + y;
             return cnew;
         };
-        // the O of tile i (of the prefix, or not) joins the row's
-        float vscale = 1.f;  // f32: 2^exponent of the values of the tile that is taken
-        auto take_o = [&](int i, bool of_prefix) {
-            if (C::ACC && of_prefix) return;
+        // the O of tile i, in buffer buf, joins the row's; or (ACC) stays, where i is of the prefix
+        // and not its last tile before a suffix or the segment's end
+        int taken = 0;  // ACC: hand-overs
+        auto take_o = [&](int i, int buf, bool of_prefix) {
             as_wait(m, &m->o_full[i & 1], (i >> 1) & 1, ok);
             as_tc_after();
-            if constexpr (C::ACC) {
-                if (prev_any) rescale(cprev, true, prev_act);
+            if (C::ACC && of_prefix) {
+                bring();
             } else if (prev_any) {
                 // (an f32 tile's values come back to their scale here)
-                const f2 c2 = as_f2(cprev, cprev), v2 = as_f2(vscale, vscale);
+                const float vs = C::KF32 ? m->vsc[i & 3] : 1.f;
+                const f2 c2 = as_f2(cprev, cprev), v2 = as_f2(vs, vs);
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {
                     float x[32];
-                    as_ld32(o_base + (C::NOB == 2 ? i & 1 : 0) * DP + c, x);
+                    as_ld32(o_base + buf * DP + c, x);
                     as_wait_ld();
                     if (prev_act) {
 #pragma unroll
@@ -995,15 +1007,16 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                     }
                 }
             }
+        };
+        auto hand_over = [&](int b) {
             as_tc_before();
             __syncwarp();
-            if (lane == 0) as_arrive(&m->o_empty[C::ACC || C::NOB == 1 ? 0 : i & 1], ok);
+            if (lane == 0) as_arrive(&m->o_empty[b], ok);
         };
 
         int j = 0, cur = -1, seg = -1, seg_t0 = t0;
         bool prev_pre = false;
-        uint32_t st = 0, rpar = 0;       // f32: the ring
-        float vnext = 1.f;
+        int nsuf = 0;  // ACC: suffix tiles of the segment so far
         AsWalk w;
         w.start(t0, tpg);
         for (int t = t0; t < t1; ++t, ++j) {
@@ -1012,47 +1025,11 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             if (first) {
                 cur = w.kvh, seg_t0 = t;
                 if constexpr (C::QF32) load_q(++seg);  // (the segment before is done with the last ones)
-                if constexpr (C::ACC) {
-                    if (!of_prefix) {  // no product of the prefix sets O
-                        const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 1
-                        for (int k = 0; k < HD; k += 8) as_st8(o_base + k, zero);
-                        as_wait_st();
-                    }
-                } else {
 #pragma unroll
-                    for (int k = 0; k < HD / 2; ++k) o[k] = 0ull;
-                }
+                for (int k = 0; k < HD / 2; ++k) o[k] = 0ull;
+                nsuf = 0;
                 mrun = -INFINITY;
                 lsum = 0.f;
-            }
-            if constexpr (C::KF32) {
-                const int valid = w.valid;
-                const bool two = C::HALF < valid;
-                if (first) ring_step(st, rpar, C::QB);
-                ring_step(st, rpar, two ? 2 : 1);  // the K tile's slots
-                const uint32_t s0 = st;
-                as_wait(m, &m->r_full[st], rpar, ok);
-                ring_step(st, rpar, 1);
-                const uint32_t s1 = st;
-                if (two) {
-                    as_wait(m, &m->r_full[st], rpar, ok);
-                    ring_step(st, rpar, 1);
-                }
-                AsConv<DP, KT, AS_SOFT> cv;
-                const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, warp, lane, valid);
-                if (lane == 0) m->vmax[j & 1][warp] = own;
-                asm volatile("bar.sync 6, %0;" ::"n"(AS_SOFT * 32) : "memory");
-                const uint4 v0 = *(const uint4*)&m->vmax[j & 1][0], v1 = *(const uint4*)&m->vmax[j & 1][4];
-                const int e = as_exponent(max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w))));
-                if (tid == 0) {
-                    as_arrive(&m->r_empty[s0], ok);
-                    if (two) as_arrive(&m->r_empty[s1], ok);
-                }
-                if (j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
-                cv.store(sV + (j & 1) * (C::NK * C::KPLANE), warp, lane, e);
-                if (lane == 0) as_arrive(&m->v_full[j & 1], ok);
-                vnext = as_pow2(e - 14);
             }
             // the row's keys of this tile: all, or none
             const bool act = live && (of_prefix || sq == w.i);
@@ -1069,17 +1046,28 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_tc_before();
             __syncwarp();
             if (lane == 0) as_arrive(&m->p_full[bf], ok);
-            if (!first) take_o(j - 1, prev_pre);
-            cprev = cnew, prev_act = act, prev_any = any, prev_pre = of_prefix, vscale = vnext;
+            if (C::ACC) {
+                // (the first suffix tile of a segment without prefix tiles hands over all the same)
+                if (!of_prefix) {
+                    if (!first) take_o(j - 1, nsuf & 1, prev_pre);
+                    hand_over(taken++ & 1);
+                    ++nsuf;
+                }
+            } else if (!first) {
+                take_o(j - 1, C::NOB == 2 ? (j - 1) & 1 : 0, false);
+                hand_over(C::NOB == 2 ? (j - 1) & 1 : 0);
+            }
+            cprev = cnew, prev_act = act, prev_any = any, prev_pre = of_prefix;
             const bool end = t + 1 == t1 || w.off + 1 == tpg;
             w.next(tpg);
             if (!end) continue;
 
             // ---- the segment's last tile: add it, then the output or a partial
-            take_o(j, prev_pre);
-            if (C::ACC && prev_pre) {
-                as_wait(m, &m->o_full[j & 1], (j >> 1) & 1, ok);
-                as_tc_after();
+            take_o(j, C::ACC ? nsuf & 1 : C::NOB == 2 ? j & 1 : 0, C::ACC && prev_pre);
+            if (C::ACC) {
+                if (!prev_pre) hand_over(taken++ & 1);
+            } else {
+                hand_over(C::NOB == 2 ? j & 1 : 0);
             }
             m->lx[half][row] = lsum;
             as_pair_sync(1 + q4);
@@ -1099,15 +1087,8 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
 #pragma unroll
             for (int k = 0; k < HD; k += 8) {
                 float x[8];
-                if constexpr (C::ACC) {
-                    as_ld8(o_base + k, reinterpret_cast<uint32_t*>(x));
-                    as_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = l == 0.f ? 0.f : x[i] * inv;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) as_un2(as_mul2(o[k / 2 + i], inv2), x[2 * i], x[2 * i + 1]);
-                }
+                for (int i = 0; i < 4; ++i) as_un2(as_mul2(o[k / 2 + i], inv2), x[2 * i], x[2 * i + 1]);
                 if (!put || d0 + k >= a.hd) continue;
                 const bool two = d0 + k + 4 < a.hd;
                 if (!whole) {
