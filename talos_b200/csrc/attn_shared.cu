@@ -25,8 +25,8 @@
 // accumulation truncates); for 16-bit outputs it stays in tensor memory.
 //
 // Precision. f16 / bf16 queries: one product each, P rounded to 16 bits (half a
-// step of 2^-11 / 2^-8 relative per weight, averaged by the sum; the row sum uses
-// the unrounded weights), f32 everywhere else. f32 queries: q is scaled by a power
+// step of 2^-11 / 2^-8 relative per weight, averaged by the sum; the row's sum is that
+// of the rounded weights), f32 everywhere else. f32 queries: q is scaled by a power
 // of two into [2^14, 2^15) at its row's largest element and split into f16 hi + lo
 // (22 bits), and so is P. An f32 cache's tiles are scaled (one power of two for 64
 // keys of K, and of V) and split too, so no input overflows f16; an element keeps
@@ -968,9 +968,20 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                     float x, y;
                     as_un2(as_fma2(as_f2(s[k + 2 * i], s[k + 2 * i + 1]), q2, sub2), x, y);
                     x = as_ex2(x), y = as_ex2(y);
+                    if (C::NP == 2) {
+                        as_split(x, y, ph[i], pl[i]);
+                    } else {
+                        // the sum of the weights that V is multiplied by: where one of them dominates
+                        // its rounding cancels
+                        ph[i] = as_pack<C::BF>(x, y);
+                        if (C::BF) {
+                            x = __uint_as_float(ph[i] << 16), y = __uint_as_float(ph[i] & 0xffff0000u);
+                        } else {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ph[i]));
+                            x = f.x, y = f.y;
+                        }
+                    }
                     l2[i & 1] = as_add2(l2[i & 1], as_f2(x, y));
-                    if (C::NP == 2) as_split(x, y, ph[i], pl[i]);
-                    else ph[i] = as_pack<C::BF>(x, y);
                 }
                 as_st8(sb + (half * HC + k) / 2, ph);
                 if (C::NP == 2) as_st8(sb + KT / 2 + (half * HC + k) / 2, pl);
