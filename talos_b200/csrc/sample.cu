@@ -13,8 +13,11 @@
 //
 // Exactness. An answer is a border between cumulative sums, so weights are
 // computed in f64 and summed as 64-bit integers in units of 2^-42: sums do not
-// depend on their order, and a weight is off by at most 2^-43 (a million weights
-// add up to less than 2^63).
+// depend on their order, and a weight is off by at most 2^-42 (a million weights
+// add up to less than 2^63). w = 2^-(k / 64) 2^(r / 64) with k the nearest integer
+// to 64 log2(e) (max - l) / T: a table of 64 powers and the exponential's series to
+// the fourth power (|r| <= 1/2: the fifth is below 4e-14), eleven f64 operations
+// where exp() took about a hundred instructions (64 rows of 128256: 117 -> @@ us).
 //
 // Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
 // shared memory, so the row is read from HBM once. No sort of the row: a
@@ -69,6 +72,7 @@ struct SpSmem {
     uint32_t f_cnt, f_bin;
     u64 f_bc, f_bw;
     uint32_t keep;     // elements of the list with w >= min_p
+    double pow[64];    // sp_pow
 };
 
 __device__ __forceinline__ float sp_load(float v) { return isnan(v) ? -INFINITY : v + 0.0f; }  // -0 -> +0
@@ -82,11 +86,46 @@ __device__ __forceinline__ float sp_key_value(u64 k) {
     return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
 
-// w of value v as f64 (1 at the maximum, +inf included).
-__device__ __forceinline__ double sp_weight(float v, float vmax, double inv_t) {
-    return v == vmax ? 1.0 : exp(((double)v - (double)vmax) * inv_t);
+// 2^42 2^(-i / 64), i < 64: the product of 2^(-1 / 2) to 2^(-1 / 64) over i's bits.
+__device__ __forceinline__ double sp_pow(int i) {
+    constexpr double root[6] = {0.98922801319397548, 0.97857206208770013, 0.95760328069857365,
+                                0.91700404320467123, 0.84089641525371454, 0.70710678118654752};
+    double w = SP_ONE;
+#pragma unroll
+    for (int b = 0; b < 6; ++b)
+        if (i >> b & 1) w *= root[b];
+    return w;
 }
-__device__ __forceinline__ u64 sp_fixed(double w) { return (u64)__double2ll_rn(w * SP_ONE); }
+
+struct SpScale {
+    float vmax, inv_t;
+    double vmax_d, c;  // c: 64 log2(e) / T
+};
+// f32 -> f64 by its bits (two integer operations where the conversion runs at a quarter
+// of their rate). Zeros and denormals become 2^-126 to 2^-125, which matters below a
+// temperature of 1e-24 only.
+__device__ __forceinline__ double sp_f64(float v) {
+    const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
+    return __hiloint2double((int)((b & 0x80000000u) | ((m >> 3) + (896u << 20))), (int)(m << 29));
+}
+// 2^42 w of a finite value v whose bin is below SP_NB (2^42 at the maximum, +inf included).
+__device__ __forceinline__ double sp_weight(float v, const SpScale& q, const double* pow) {
+    if (v == q.vmax) return SP_ONE;
+    const double t = (q.vmax_d - sp_f64(v)) * q.c;
+    const double round = 6755399441055744.0;  // 1.5 2^52: the sum's low word is the nearest integer
+    const double tm = t + round;
+    const int k = __double2loint(tm);
+    const double r = (tm - round) - t, h = 0.010830424696249145;  // ln 2 / 64
+    const double z = r * h;
+    const double e = fma(z, fma(z, fma(z, fma(z, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
+    const double w = pow[k & 63] * e;
+    return __hiloint2double(__double2hiint(w) - ((k >> 6) << 20), __double2loint(w));  // times 2^-(k / 64)
+}
+// To the nearest integer (w <= 2^42).
+__device__ __forceinline__ u64 sp_fixed(double w) {
+    const double x = w + 4503599627370496.0;  // 2^52
+    return (u64)__double_as_longlong(x) & 0xfffffffffffffull;
+}
 // Bin of value v, SP_NB for weight 0. Non-decreasing as v falls: every rounding here is monotone.
 __device__ __forceinline__ int sp_bin(float v, float vmax, float inv_t) {
     if (v == vmax) return 0;
@@ -175,6 +214,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     if (!(temp > 0.f)) temp = 1.f, topk = 1;
     const double inv_t = fmin(1.0 / (double)temp, 1e30);
     const float inv_tf = (float)inv_t;
+    if (tid < 64) s.pow[tid] = sp_pow(tid);
 
     // the row's maximum
     mx = warp_max(mx);
@@ -195,6 +235,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         }
         return;
     }
+
+    const SpScale q{vmax, inv_tf, sp_f64(vmax), inv_t * 92.332482616893656};  // 64 log2(e)
+    const double min_w = (double)minp * SP_ONE;
 
     auto zero_hist = [&]() {
         for (int b = tid; b < SP_NB; b += SP_THREADS) s.cnt[b] = 0, s.wlo[b] = 0, s.whi[b] = 0;
@@ -220,7 +263,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                     const int b = sp_bin(v, vmax, inv_tf);
                     if (b < SP_NB) {
                         atomicAdd(&s.cnt[b], 1u);
-                        if (c.op == SP_WEIGH) add_hist(b, sp_fixed(sp_weight(v, vmax, inv_t)));
+                        if (c.op == SP_WEIGH) add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
                     }
                 });
                 break;
@@ -271,7 +314,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                     if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, inv_tf) < SP_NB) {
                         const int b = (int)((k - c.k0) >> c.shift);
                         atomicAdd(&s.cnt[b], 1u);
-                        add_hist(b, sp_fixed(sp_weight(v, vmax, inv_t)));
+                        add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
                     }
                 });
                 break;
@@ -279,8 +322,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                 u64 sum = 0;
                 each([&](float v, uint32_t) {
                     if (sp_bin(v, vmax, inv_tf) < SP_NB) {
-                        const double w = sp_weight(v, vmax, inv_t);
-                        if (w >= (double)minp) sum += sp_fixed(w);
+                        const double w = sp_weight(v, q, s.pow);
+                        if (w >= min_w) sum += sp_fixed(w);
                     }
                 });
 #pragma unroll
@@ -351,13 +394,30 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     };
     // rank the gathered list (keys are unique) and sum its weights
     auto rank_list = [&](int n) {
-        __syncthreads();
-        for (int i = tid; i < n; i += SP_THREADS) {
-            const u64 k = s.list[i];
-            int pos = 0;
+        if (n <= 256) {  // count the smaller keys
+            __syncthreads();
+            if (tid < n) {
+                const u64 k = s.list[tid];
+                int pos = 0;
 #pragma unroll 8
-            for (int j = 0; j < n; ++j) pos += s.list[j] < k ? 1 : 0;
-            s.key[pos] = k;
+                for (int j = 0; j < n; ++j) pos += s.list[j] < k ? 1 : 0;
+                s.key[pos] = k;
+            }
+        } else {  // sort (bitonic; 600 keys: 45 steps instead of 1200 comparisons a thread)
+            const int len = n <= 512 ? 512 : 1024;
+            __syncthreads();
+            for (int i = tid; i < len; i += SP_THREADS) s.key[i] = i < n ? s.list[i] : ~0ull;
+#pragma unroll 1
+            for (int k = 2; k <= len; k *= 2)
+#pragma unroll 1
+                for (int j = k / 2; j > 0; j /= 2) {
+                    __syncthreads();
+                    if (tid < len / 2) {
+                        const int i = 2 * tid - (tid & (j - 1)), l = i + j;
+                        const u64 x = s.key[i], y = s.key[l];
+                        if ((x > y) == ((i & k) == 0)) s.key[i] = y, s.key[l] = x;
+                    }
+                }
         }
         if (tid == 0) s.keep = 0;
         __syncthreads();
@@ -367,9 +427,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         for (int j = 0; j < 2; ++j) {
             const int i = 2 * tid + j;
             if (i < n) {
-                const double w = sp_weight(sp_key_value(s.key[i]), vmax, inv_t);
+                const double w = sp_weight(sp_key_value(s.key[i]), q, s.pow);
                 x[j] = sp_fixed(w);
-                keep += !(w < (double)minp) ? 1u : 0u;
+                keep += w >= min_w ? 1u : 0u;
             }
         }
         u64 ex = x[0] + x[1], dummy = 0, t1, t2;
@@ -505,7 +565,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     if (tid == 0) {
         a.tokens[row] = (int32_t)(chosen & (SAMPLE_MAX_VOCAB - 1));
         if (a.probs)
-            a.probs[row] = (float)(sp_weight(sp_key_value(chosen), vmax, inv_t) / ((double)W / SP_ONE));
+            a.probs[row] = (float)(sp_weight(sp_key_value(chosen), q, s.pow) / (double)W);
     }
     __syncthreads();
     if (tid < C) cluster.map_shared_rank(&s, tid)->cmd.op = SP_DONE;
