@@ -17,11 +17,11 @@
 // add up to less than 2^63). w = 2^-(k / 64) 2^(r / 64) with k the nearest integer
 // to 64 log2(e) (max - l) / T: a table of 64 powers and the exponential's series to
 // the fourth power (|r| <= 1/2: the fifth is below 4e-14), eleven f64 operations
-// where exp() took about a hundred instructions (64 rows of 128256: 117 -> @@ us).
+// where exp() took about a hundred instructions (64 rows of 128256: 117 -> 99 us).
 //
 // Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
 // shared memory, so the row is read from HBM once. No sort of the row: a
-// histogram over 1024 bins of (max - l) / T (1/32 nat each; beyond 32 nats the
+// histogram over 1024 bins of (max - l) / T (1/32 nat each or less; beyond 32 nats the
 // weight is 0) counts and sums the weights per bin in shared memory, the leading
 // CTA adds the cluster's histograms through distributed shared memory, scans
 // them, and finds the bins of the borders. When the elements up to the first
@@ -59,17 +59,18 @@ struct SpCmd {
 
 struct SpSmem {
     uint32_t cnt[SP_NB], wlo[SP_NB], whi[SP_NB];
-    u64 list[SP_CAP];  // gathered keys (leader)
-    u64 key[SP_CAP];   // ranked
+    u64 list[SP_CAP];  // leader: gathered keys, then the ranked ones
+    u64 key[SP_CAP];   // this CTA's gathered keys; leader: keys by bucket
     u64 cum[SP_CAP];   // cumulative weights of the ranked list
-    float cmax[8];     // each CTA's maximum
+    float cmax[8], cmin[8];  // each CTA's largest and smallest finite logit
     SpCmd cmd;
     uint32_t nlist;    // leader: gathered so far
+    uint32_t mine, at; // gathered by this CTA, their place in the leader's list
     u64 ra, rb;        // this CTA's SP_RANGE (smallest, largest key) or SP_SUM_MIN (sum)
     u64 wa[SP_WARPS], wb[SP_WARPS];  // block scans
-    float fa[SP_WARPS];
+    float fa[SP_WARPS], fb[SP_WARPS];
     // result of a search
-    uint32_t f_cnt, f_bin;
+    uint32_t f_cnt, f_bin, f_at;
     u64 f_bc, f_bw;
     uint32_t keep;     // elements of the list with w >= min_p
     double pow[64];    // sp_pow
@@ -98,7 +99,7 @@ __device__ __forceinline__ double sp_pow(int i) {
 }
 
 struct SpScale {
-    float vmax, inv_t;
+    float vmax;
     double vmax_d, c;  // c: 64 log2(e) / T
 };
 // f32 -> f64 by its bits (two integer operations where the conversion runs at a quarter
@@ -127,10 +128,12 @@ __device__ __forceinline__ u64 sp_fixed(double w) {
     return (u64)__double_as_longlong(x) & 0xfffffffffffffull;
 }
 // Bin of value v, SP_NB for weight 0. Non-decreasing as v falls: every rounding here is monotone.
-__device__ __forceinline__ int sp_bin(float v, float vmax, float inv_t) {
-    if (v == vmax) return 0;
-    const float z = __fmul_rn(__fmul_rn(__fsub_rn(vmax, v), inv_t), SP_PER_NAT);
-    return z < (float)SP_NB ? (int)z : SP_NB;  // NaN (-inf * 0) gives SP_NB
+__device__ __forceinline__ float sp_z(float v, float vmax, float scale) {
+    return v == vmax ? 0.f : __fmul_rn(__fsub_rn(vmax, v), scale);
+}
+__device__ __forceinline__ int sp_bin(float v, float vmax, float scale) {
+    const float z = sp_z(v, vmax, scale);
+    return z < (float)SP_NB ? (int)z : SP_NB;  // NaN (-inf at a scale of 0) gives SP_NB
 }
 
 // Exclusive block scan of (a, b); returns the totals through ta, tb.
@@ -158,7 +161,7 @@ __device__ __forceinline__ void sp_scan(SpSmem& s, u64& a, u64& b, u64& ta, u64&
 
 // RES: the CTA's slice of the row stays in shared memory (up to SP_SLICE
 // logits as f32); otherwise every pass reads it again (vocabularies above
-// 8 x SP_SLICE). (In registers, 32 logits a thread, the f64 weights spilled.)
+// 8 x SP_SLICE, or fewer CTAs a row). (In registers, 32 logits a thread, the f64 weights spilled.)
 template <typename T, bool RES, bool VEC>
 __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant__ SampleArgs a, int slice) {
     __shared__ SpSmem s;
@@ -172,7 +175,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     const int i0 = min(a.vocab, rank * slice), n_own = min(a.vocab, i0 + slice) - i0;
     const T* lg = (const T*)a.logits + (size_t)row * a.stride + i0;
 
-    float mx = -INFINITY;
+    float mx = -INFINITY, mn = INFINITY;
+    auto minmax = [&](float v) {
+        mx = fmaxf(mx, v);
+        mn = fminf(mn, v > -INFINITY ? v : INFINITY);
+    };
     if (VEC) {  // slice is a multiple of VW, so lg is 16-byte aligned
 #pragma unroll 4
         for (int i = tid * VW; i < n_own; i += SP_THREADS * VW) {
@@ -187,7 +194,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                 for (int k = 0; k < VW; ++k) v[k] = i + k < n_own ? sp_load(lg[i + k]) : -INFINITY;
             }
 #pragma unroll
-            for (int k = 0; k < VW; ++k) mx = fmaxf(mx, v[k]);
+            for (int k = 0; k < VW; ++k) minmax(v[k]);
 #pragma unroll
             for (int k = 0; k < VW; k += 4)
                 if (RES) *(float4*)(vals + i + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
@@ -197,12 +204,35 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         for (int i = tid; i < n_own; i += SP_THREADS) {
             const float v = sp_load(lg[i]);
             if (RES) vals[i] = v;
-            mx = fmaxf(mx, v);
+            minmax(v);
         }
     }
+    // the slice's last four start on a multiple of four (-inf has weight 0)
+    if (RES && tid < 4 && n_own + tid < (n_own + 3) / 4 * 4) vals[n_own + tid] = -INFINITY;
     auto each = [&](auto&& f) {  // (after the barriers of the maximum)
+        if (RES) {
+#pragma unroll 2
+            for (int i = 4 * tid; i < n_own; i += 4 * SP_THREADS) {
+                const float4 v = *(const float4*)(vals + i);
+                f(v.x, (uint32_t)(i0 + i));
+                f(v.y, (uint32_t)(i0 + i + 1));
+                f(v.z, (uint32_t)(i0 + i + 2));
+                f(v.w, (uint32_t)(i0 + i + 3));
+            }
+        } else if (VEC) {
+            const int nv = n_own / VW * VW;
+#pragma unroll 2
+            for (int i = tid * VW; i < nv; i += SP_THREADS * VW) {
+                const uint4 x = __ldg((const uint4*)(lg + i));
+                const T* t = reinterpret_cast<const T*>(&x);
+#pragma unroll
+                for (int k = 0; k < VW; ++k) f(sp_load(t[k]), (uint32_t)(i0 + i + k));
+            }
+            if (tid < n_own - nv) f(sp_load(lg[nv + tid]), (uint32_t)(i0 + nv + tid));
+        } else {
 #pragma unroll 4
-        for (int i = tid; i < n_own; i += SP_THREADS) f(RES ? vals[i] : sp_load(lg[i]), (uint32_t)(i0 + i));
+            for (int i = tid; i < n_own; i += SP_THREADS) f(sp_load(lg[i]), (uint32_t)(i0 + i));
+        }
     };
 
     // settings of the row; T <= 0 (or NaN) is the greedy choice: the first of the order
@@ -213,21 +243,24 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     minp = minp > 0.f ? fminf(minp, 1.0f) : 0.f;  // NaN: off
     if (!(temp > 0.f)) temp = 1.f, topk = 1;
     const double inv_t = fmin(1.0 / (double)temp, 1e30);
-    const float inv_tf = (float)inv_t;
     if (tid < 64) s.pow[tid] = sp_pow(tid);
 
-    // the row's maximum
+    // the row's largest and smallest finite logit
     mx = warp_max(mx);
-    if (lane == 0) s.fa[warp] = mx;
+    mn = -warp_max(-mn);
+    if (lane == 0) s.fa[warp] = mx, s.fb[warp] = mn;
     __syncthreads();
-    if (tid < C) {
-        float m = s.fa[0];
-        for (int w = 1; w < SP_WARPS; ++w) m = fmaxf(m, s.fa[w]);
-        cluster.map_shared_rank(&s, tid)->cmax[rank] = m;
+    if (warp == 0) {
+        mx = warp_max(lane < SP_WARPS ? s.fa[lane] : -INFINITY);
+        mn = -warp_max(lane < SP_WARPS ? -s.fb[lane] : -INFINITY);
+        if (lane < C) {
+            SpSmem* o = cluster.map_shared_rank(&s, lane);
+            o->cmax[rank] = mx, o->cmin[rank] = mn;
+        }
     }
     cluster.sync();
-    float vmax = s.cmax[0];
-    for (int c = 1; c < C; ++c) vmax = fmaxf(vmax, s.cmax[c]);
+    float vmax = s.cmax[0], vmin = s.cmin[0];
+    for (int c = 1; c < C; ++c) vmax = fmaxf(vmax, s.cmax[c]), vmin = fminf(vmin, s.cmin[c]);
     if (vmax == -INFINITY) {  // nothing to choose from; the whole cluster agrees
         if (rank == 0 && tid == 0) {
             a.tokens[row] = -1;
@@ -236,7 +269,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         return;
     }
 
-    const SpScale q{vmax, inv_tf, sp_f64(vmax), inv_t * 92.332482616893656};  // 64 log2(e)
+    const SpScale q{vmax, sp_f64(vmax), inv_t * 92.332482616893656};  // 64 log2(e)
+    // Bins per logit: the row's range over all bins, at most 32 nats (the smallest logit's
+    // bin is below SP_NB for every rounding; an infinite or empty range leaves the 32 nats).
+    // With 32 nats always, rows of 128256 with a deviation of 1.5 nats had bins of more than
+    // SP_CAP and took 193,000 clocks instead of 85,000 (64 rows with top-p: 105 -> 63 us).
+    const float scale = fmaxf((float)inv_t * SP_PER_NAT, (float)(SP_NB - 1) / (vmax - vmin));
     const double min_w = (double)minp * SP_ONE;
 
     auto zero_hist = [&]() {
@@ -249,9 +287,39 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
         if (hi) atomicAdd(&s.whi[b], hi);
     };
+    // matches are collected here and handed to the leader at once (one atomic on the
+    // leader's counter for each took 8,000 clocks for 600 keys, this 3,000)
     auto gather = [&](u64 k) {
-        const uint32_t at = atomicAdd(&lead->nlist, 1u);
-        if (at < SP_CAP) lead->list[at] = k;
+        const uint32_t at = atomicAdd(&s.mine, 1u);
+        if (at < SP_CAP) s.key[at] = k;
+    };
+    auto hand_over = [&]() {
+        __syncthreads();
+        const uint32_t n = s.mine;
+        if (tid == 0 && n) s.at = atomicAdd(&lead->nlist, n);
+        __syncthreads();
+        if (tid == 0) s.mine = 0;
+        for (uint32_t i = tid; i < n && i < SP_CAP && s.at + i < SP_CAP; i += SP_THREADS)
+            lead->list[s.at + i] = s.key[i];
+    };
+    // Each CTA adds its share of the bins over the cluster and hands the sums to the
+    // leader, in place of its list and cum (the leader alone, reading 8 x 12 KB, took
+    // 4,500 clocks; this and its barrier 4,000, beside the others' work).
+    auto sum_hist = [&]() {
+        cluster.sync();
+        const int nb = SP_NB / C;  // C is a power of two
+        for (int b = rank * nb + tid; b < (rank + 1) * nb; b += SP_THREADS) {
+            uint32_t n = 0;
+            u64 w = 0;
+#pragma unroll 8
+            for (int c = 0; c < C; ++c) {
+                const SpSmem* o = cluster.map_shared_rank(&s, c);
+                n += o->cnt[b];
+                w += ((u64)o->whi[b] << 32) + o->wlo[b];
+            }
+            ((uint32_t*)lead->cum)[b] = n;
+            lead->list[b] = w;
+        }
     };
     // one command, by every CTA of the cluster
     auto execute = [&](const SpCmd& c) {
@@ -260,29 +328,34 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             case SP_WEIGH:
                 zero_hist();
                 each([&](float v, uint32_t) {
-                    const int b = sp_bin(v, vmax, inv_tf);
+                    const int b = sp_bin(v, vmax, scale);
                     if (b < SP_NB) {
                         atomicAdd(&s.cnt[b], 1u);
                         if (c.op == SP_WEIGH) add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
                     }
                 });
+                sum_hist();
                 break;
-            case SP_GATHER_BINS:
+            case SP_GATHER_BINS: {
+                const float z0 = (float)c.b0, z1 = (float)(c.b1 + 1);  // b0 <= bin <= b1
                 each([&](float v, uint32_t i) {
-                    const int b = sp_bin(v, vmax, inv_tf);
-                    if (b >= c.b0 && b <= c.b1) gather(sp_key(v, i));
+                    const float z = sp_z(v, vmax, scale);
+                    if (z >= z0 && z < z1) gather(sp_key(v, i));
                 });
+                hand_over();
                 break;
+            }
             case SP_GATHER_KEYS:
                 each([&](float v, uint32_t i) {
                     const u64 k = sp_key(v, i);
-                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, inv_tf) < SP_NB) gather(k);
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, scale) < SP_NB) gather(k);
                 });
+                hand_over();
                 break;
             case SP_RANGE: {
                 u64 lo = ~0ull, hi = 0ull;
                 each([&](float v, uint32_t i) {
-                    if (sp_bin(v, vmax, inv_tf) == c.b0) {
+                    if (sp_bin(v, vmax, scale) == c.b0) {
                         const u64 k = sp_key(v, i);
                         lo = k < lo ? k : lo;
                         hi = k > hi ? k : hi;
@@ -311,17 +384,18 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                 zero_hist();
                 each([&](float v, uint32_t i) {
                     const u64 k = sp_key(v, i);
-                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, inv_tf) < SP_NB) {
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, scale) < SP_NB) {
                         const int b = (int)((k - c.k0) >> c.shift);
                         atomicAdd(&s.cnt[b], 1u);
                         add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
                     }
                 });
+                sum_hist();
                 break;
             case SP_SUM_MIN: {
                 u64 sum = 0;
                 each([&](float v, uint32_t) {
-                    if (sp_bin(v, vmax, inv_tf) < SP_NB) {
+                    if (sp_bin(v, vmax, scale) < SP_NB) {
                         const double w = sp_weight(v, q, s.pow);
                         if (w >= min_w) sum += sp_fixed(w);
                     }
@@ -343,7 +417,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     // weights of all elements are only needed without one
     const bool count_only = topk > 0 && topk <= SP_CAP / 2;
     const SpCmd first{count_only ? SP_COUNT : SP_WEIGH, 0, 0, 0, 0, 0};
-    if (tid == 0) s.nlist = 0;
+    if (tid == 0) s.nlist = s.mine = 0;
     execute(first);
     cluster.sync();
     if (rank != 0) {
@@ -369,15 +443,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     uint32_t c0, c1;
     u64 w0, w1, bc, bw, tc, tw;
     auto load_hist = [&]() {
-        c0 = c1 = 0;
-        w0 = w1 = 0;
-        for (int q = 0; q < C; ++q) {
-            const SpSmem* o = cluster.map_shared_rank(&s, q);
-            const uint2 n = *(const uint2*)&o->cnt[2 * tid], lo = *(const uint2*)&o->wlo[2 * tid],
-                        hi = *(const uint2*)&o->whi[2 * tid];
-            c0 += n.x, c1 += n.y;
-            w0 += ((u64)hi.x << 32) + lo.x, w1 += ((u64)hi.y << 32) + lo.y;
-        }
+        const uint2 n = *(const uint2*)((const uint32_t*)s.cum + 2 * tid);
+        c0 = n.x, c1 = n.y;
+        w0 = s.list[2 * tid], w1 = s.list[2 * tid + 1];
         bc = (u64)c0 + c1, bw = w0 + w1;
         sp_scan(s, bc, bw, tc, tw);
     };
@@ -392,34 +460,57 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             s.f_bin = 2 * tid + 1, s.f_cnt = c1, s.f_bc = xc + bc + c0, s.f_bw = xw + bw + w0;
         __syncthreads();
     };
-    // rank the gathered list (keys are unique) and sum its weights
+    // sort the gathered list (keys are unique) and sum its weights. The keys are put into
+    // 1024 buckets by their leading bits and each counts the smaller ones of its own bucket
+    // (600 keys: 2,500 clocks; counting over the whole list or a sorting network: 15,000)
+    u64 lx = 0, l0 = 0, l1 = 0;  // this thread's two: weights, and the sum before them
     auto rank_list = [&](int n) {
-        if (n <= 256) {  // count the smaller keys
-            __syncthreads();
-            if (tid < n) {
-                const u64 k = s.list[tid];
-                int pos = 0;
-#pragma unroll 8
-                for (int j = 0; j < n; ++j) pos += s.list[j] < k ? 1 : 0;
-                s.key[pos] = k;
-            }
-        } else {  // sort (bitonic; 600 keys: 45 steps instead of 1200 comparisons a thread)
-            const int len = n <= 512 ? 512 : 1024;
-            __syncthreads();
-            for (int i = tid; i < len; i += SP_THREADS) s.key[i] = i < n ? s.list[i] : ~0ull;
-#pragma unroll 1
-            for (int k = 2; k <= len; k *= 2)
-#pragma unroll 1
-                for (int j = k / 2; j > 0; j /= 2) {
-                    __syncthreads();
-                    if (tid < len / 2) {
-                        const int i = 2 * tid - (tid & (j - 1)), l = i + j;
-                        const u64 x = s.key[i], y = s.key[l];
-                        if ((x > y) == ((i & k) == 0)) s.key[i] = y, s.key[l] = x;
-                    }
-                }
+        u64 k[2], lo = ~0ull, hi = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = tid + j * SP_THREADS;
+            k[j] = i < n ? s.list[i] : 0;
+            if (i < n) lo = k[j] < lo ? k[j] : lo, hi = k[j] > hi ? k[j] : hi;
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const u64 x = __shfl_xor_sync(0xffffffffu, lo, o), y = __shfl_xor_sync(0xffffffffu, hi, o);
+            lo = x < lo ? x : lo;
+            hi = y > hi ? y : hi;
+        }
+        __syncthreads();
+        if (lane == 0) s.wa[warp] = lo, s.wb[warp] = hi;
+        *(uint2*)&s.cnt[2 * tid] = make_uint2(0, 0);
         if (tid == 0) s.keep = 0;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SP_WARPS; ++w) {
+            lo = s.wa[w] < lo ? s.wa[w] : lo;
+            hi = s.wb[w] > hi ? s.wb[w] : hi;
+        }
+        const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
+        uint32_t at[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (tid + j * SP_THREADS < n) at[j] = atomicAdd(&s.cnt[(k[j] - lo) >> shift], 1u);
+        __syncthreads();
+        const uint2 c = *(const uint2*)&s.cnt[2 * tid];
+        u64 ex = c.x + c.y, dummy = 0, t1, t2;
+        sp_scan(s, ex, dummy, t1, t2);
+        *(uint2*)&s.wlo[2 * tid] = make_uint2((uint32_t)ex, (uint32_t)ex + c.x);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (tid + j * SP_THREADS < n) s.key[s.wlo[(k[j] - lo) >> shift] + at[j]] = k[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (tid + j * SP_THREADS < n) {
+                const uint32_t b = (uint32_t)((k[j] - lo) >> shift), b0 = s.wlo[b], nb = s.cnt[b];
+                uint32_t pos = b0;
+                for (uint32_t i = 0; i < nb; ++i) pos += s.key[b0 + i] < k[j] ? 1 : 0;
+                s.list[pos] = k[j];
+            }
         __syncthreads();
         u64 x[2] = {0, 0};
         uint32_t keep = 0;
@@ -427,27 +518,29 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         for (int j = 0; j < 2; ++j) {
             const int i = 2 * tid + j;
             if (i < n) {
-                const double w = sp_weight(sp_key_value(s.key[i]), q, s.pow);
+                const double w = sp_weight(sp_key_value(s.list[i]), q, s.pow);
                 x[j] = sp_fixed(w);
                 keep += w >= min_w ? 1u : 0u;
             }
         }
-        u64 ex = x[0] + x[1], dummy = 0, t1, t2;
-        sp_scan(s, ex, dummy, t1, t2);
-        if (2 * tid < n) s.cum[2 * tid] = ex + x[0];
-        if (2 * tid + 1 < n) s.cum[2 * tid + 1] = ex + x[0] + x[1];
+        l0 = x[0], l1 = x[1];
+        lx = l0 + l1, dummy = 0;
+        sp_scan(s, lx, dummy, t1, t2);
+        if (2 * tid < n) s.cum[2 * tid] = lx + l0;
+        if (2 * tid + 1 < n) s.cum[2 * tid + 1] = lx + l0 + l1;
         if (keep) atomicAdd(&s.keep, keep);
         __syncthreads();
     };
-    // first of the ranked list with base + cum >= x (all threads get it)
+    // first of the ranked list with base + cum >= x, else its last (all threads get it)
     auto list_find = [&](int n, u64 base, u64 x) {
-        int lo = 0, hi = n - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (base + s.cum[mid] >= x) hi = mid;
-            else lo = mid + 1;
-        }
-        return lo;
+        if (tid == 0) s.f_at = n - 1;
+        __syncthreads();
+        if (base + lx < x && x <= base + lx + l0) s.f_at = 2 * tid;
+        if (base + lx + l0 < x && x <= base + lx + l0 + l1) s.f_at = 2 * tid + 1;
+        __syncthreads();
+        const int j = (int)s.f_at;
+        __syncthreads();
+        return j;
     };
     auto p_target = [&](u64 z) {  // smallest integer >= p * z, within 1 .. z
         const double t = ceil((double)topp * (double)z);
@@ -471,8 +564,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     // (top-p is a share of the top-k's weight: with both, the list holds the whole top-k)
     const bool sum_known = !k_active && !count_only;
     if (minp > 0.f && (sum_known || !(topp < 1.f))) {
-        // w < m beyond bin -32 ln m; one bin more covers the roundings of both
-        const float zb = -logf(minp) * SP_PER_NAT + 2.0f;
+        // w < m beyond -ln m nats; one bin more covers the roundings of both
+        const float zb = -logf(minp) * (scale / (float)inv_t) + 2.0f;
         const int b = zb < (float)(SP_NB - 1) ? (int)zb : SP_NB - 1;
         if (b < bcut) {
             __syncthreads();
@@ -505,7 +598,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         if (keep < 1) keep = 1;
         W = s.cum[keep - 1];
         const int j = list_find(n, 0, draw_target(W));
-        chosen = s.key[j];
+        chosen = s.list[j];
     } else {
         if (count_only) {  // more equal logits at the border than the list holds
             step(SpCmd{SP_WEIGH, 0, 0, 0, 0, 0});
@@ -546,7 +639,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             }
             rank_list((int)n);
             const int j = by_count ? (int)(x - xc) - 1 : list_find((int)n, xw, x);
-            chosen = s.key[j];
+            chosen = s.list[j];
             const u64 cum = xw + s.cum[j];
             __syncthreads();
             return cum;
@@ -597,6 +690,10 @@ static cudaError_t launch_type(const SampleArgs& a, int sms, cudaStream_t s) {
     int C = 1;
     while (C < 8 && (long)C * SP_SLICE < a.vocab) C *= 2;
     while (C < 8 && (long)C * 4096 < a.vocab && 2L * C * a.n <= 2L * sms) C *= 2;
+    // Rows that would not all run at once take half as many CTAs where those do, which read
+    // their slices again from L2 where they no longer fit (64 rows of 128256, plain
+    // temperature: 8 CTAs a row in two waves 60 us, 4 in one 50).
+    if (C > 1 && (long)C * a.n > 2L * sms && (long)C / 2 * a.n <= 2L * sms) C /= 2;
     const int slice = ((a.vocab + C - 1) / C + 15) / 16 * 16;
     const bool res = slice <= SP_SLICE;
     const bool vec = ((uintptr_t)a.logits % 16 == 0) && (a.stride * sizeof(T)) % 16 == 0;
