@@ -6,12 +6,17 @@
 // the data from before the call. The host orders them so that each slot is read
 // by all its readers before it is overwritten, and groups them into components
 // that touch disjoint slots; a cycle of slots keeps one chunk aside (MOVE_TMP).
-// A thread takes one offset of a component (array, layer, row, 16 bytes of the
-// row) and carries out all of the component's moves at that offset, so the
+// A thread takes offsets of a component (array, layer, row, 16 bytes of the
+// row) and carries out all of the component's moves at each of them, so the
 // order between them is its own program order: no barrier, no second buffer,
 // and a slot copied to many others is read once.
 //
 // Bound: HBM. Each source row is read once, each destination row written once.
+// What carries it is warps in flight (one 16-byte load a thread, 32 registers, 8
+// blocks an SM) and long runs within a slot. One prompt of 512 rows into 31 slots
+// (1.07 GB with 8 layers of 2 x 4 KB rows): 173 us, 6.2 TB/s; 40 slots of up to 1000 rows
+// moved to the front (1.64 GB, f16): 246 us, 6.7 TB/s. With 16 loads a thread in
+// flight (199 registers, one block an SM) they took 298 and 870 us.
 #include <string.h>
 
 #include "ops.cuh"
@@ -23,7 +28,7 @@ constexpr int MV_THREADS = 256;
 template <int CAP>
 struct MoveProg {
     MoveGeom g;
-    int n_comp;
+    int n_comp, iter;          // iter: offsets a thread takes
     uint32_t comp[CAP + 1];    // first instruction of each component
     uint32_t block[CAP + 1];   // first block of each component
     uint32_t row0[CAP];        // rows the component touches: row0 ..
@@ -54,12 +59,8 @@ struct MvWord<1> {
     using T = uint8_t;
 };
 
-// OFF offsets per thread, BAT instructions whose loads are in flight together:
-// loads may run ahead of earlier stores because no slot is read after it was written.
-constexpr int MV_OFF = 4, MV_BAT = 4;
-
 template <int VEC, int CAP>
-__global__ void __launch_bounds__(MV_THREADS) k_kv_move(const __grid_constant__ MoveProg<CAP> p) {
+__global__ void __launch_bounds__(MV_THREADS, 8) k_kv_move(const __grid_constant__ MoveProg<CAP> p) {
     using T = typename MvWord<VEC>::T;
     int lo = 0, hi = p.n_comp;  // the component of this block
     while (hi - lo > 1) {
@@ -69,54 +70,45 @@ __global__ void __launch_bounds__(MV_THREADS) k_kv_move(const __grid_constant__ 
     }
     const uint32_t cpr = (uint32_t)(p.g.row_bytes / VEC);  // chunks per row
     const unsigned long long span = (unsigned long long)p.rows[lo] * cpr;
-    const uint32_t per_outer = (uint32_t)((span + MV_THREADS * MV_OFF - 1) / (MV_THREADS * MV_OFF));
+    const uint32_t per_block = MV_THREADS * (uint32_t)p.iter;
+    const uint32_t per_outer = (uint32_t)((span + per_block - 1) / per_block);
     const uint32_t b = blockIdx.x - p.block[lo];
     const uint32_t outer = b / per_outer;  // (array, layer)
     uint8_t* base = p.g.base[outer / p.g.n_outer] + (size_t)(outer % p.g.n_outer) * p.g.outer_stride;
-    const unsigned long long i0 = (unsigned long long)(b % per_outer) * (MV_THREADS * MV_OFF) + threadIdx.x;
-    uint32_t row[MV_OFF];
-    size_t off[MV_OFF];
-    bool live[MV_OFF];
-#pragma unroll
-    for (int k = 0; k < MV_OFF; ++k) {
-        const unsigned long long i = i0 + k * MV_THREADS;
-        live[k] = i < span;
-        const uint32_t r = (uint32_t)(i / cpr);
-        row[k] = p.row0[lo] + r;
-        off[k] = (size_t)row[k] * p.g.row_stride + (size_t)(i - (unsigned long long)r * cpr) * VEC;
-    }
-    T tmp[MV_OFF];
+    const unsigned long long i0 = (unsigned long long)(b % per_outer) * per_block + threadIdx.x;
     const uint32_t e = p.comp[lo + 1];
-    for (uint32_t j0 = p.comp[lo]; j0 < e; j0 += MV_BAT) {
-        T v[MV_BAT][MV_OFF];
-#pragma unroll
-        for (int j = 0; j < MV_BAT; ++j)
-            if (j0 + j < e) {
-                const MoveIns in = p.ins[j0 + j];
-#pragma unroll
-                for (int k = 0; k < MV_OFF; ++k) {
-                    if (in.src == MOVE_TMP) {
-                        v[j][k] = tmp[k];
-                    } else if (live[k] && row[k] - in.start < in.len) {
-                        if (j > 0 && p.ins[j0 + j - 1].src == in.src && p.ins[j0 + j - 1].start == in.start &&
-                            p.ins[j0 + j - 1].len == in.len)
-                            v[j][k] = v[j > 0 ? j - 1 : 0][k];
-                        else
-                            v[j][k] = *(const T*)(base + (size_t)in.src * p.g.slot_stride + off[k]);
-                    }
-                    if (in.dst == MOVE_TMP) tmp[k] = v[j][k];
-                }
+    if (p.iter == 1) {
+        const uint32_t r = span <= 0xffffffffull ? (uint32_t)i0 / cpr : (uint32_t)(i0 / cpr);
+        const uint32_t row = p.row0[lo] + r;
+        if (i0 >= span) return;
+        uint8_t* at = base + (size_t)row * p.g.row_stride + (size_t)(i0 - (unsigned long long)r * cpr) * VEC;
+        T v = {}, tmp = {};
+        MoveIns last{MOVE_TMP, MOVE_TMP, 0, 0};
+#pragma unroll 4
+        for (uint32_t j = p.comp[lo]; j < e; ++j) {
+            const MoveIns in = p.ins[j];
+            if (row - in.start < in.len) {
+                if (in.src == MOVE_TMP) v = tmp;
+                else if (in.src != last.src || in.start != last.start || in.len != last.len)
+                    v = *(const T*)(at + (size_t)in.src * p.g.slot_stride);
+                if (in.dst == MOVE_TMP) tmp = v;
+                else *(T*)(at + (size_t)in.dst * p.g.slot_stride) = v;
             }
-#pragma unroll
-        for (int j = 0; j < MV_BAT; ++j)
-            if (j0 + j < e) {
-                const MoveIns in = p.ins[j0 + j];
-                if (in.dst == MOVE_TMP) continue;
-#pragma unroll
-                for (int k = 0; k < MV_OFF; ++k)
-                    if (live[k] && row[k] - in.start < in.len)
-                        *(T*)(base + (size_t)in.dst * p.g.slot_stride + off[k]) = v[j][k];
-            }
+            last = in;
+        }
+        return;
+    }
+    for (uint32_t j = p.comp[lo]; j < e; ++j) {
+        const MoveIns in = p.ins[j];
+#pragma unroll 1
+        for (int it = 0; it < p.iter; ++it) {
+            const unsigned long long i = i0 + (uint32_t)it * MV_THREADS;
+            const uint32_t r = span <= 0xffffffffull ? (uint32_t)i / cpr : (uint32_t)(i / cpr);
+            const uint32_t row = p.row0[lo] + r;
+            if (i >= span || row - in.start >= in.len) continue;
+            uint8_t* at = base + (size_t)row * p.g.row_stride + (size_t)(i - (unsigned long long)r * cpr) * VEC;
+            *(T*)(at + (size_t)in.dst * p.g.slot_stride) = *(const T*)(at + (size_t)in.src * p.g.slot_stride);
+        }
     }
 }
 
@@ -132,19 +124,32 @@ static cudaError_t launch_cap(const MoveGeom& g, const MoveIns* ins, const uint3
     size_t all = g.slot_stride | g.outer_stride | g.row_stride | g.row_bytes;
     for (int i = 0; i < g.n_base; ++i) all |= (size_t)g.base[i];
     const int vec = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+    // Offsets of a thread: one where a source is copied to several slots in a row or a chunk
+    // is kept aside; else up to 8, so that a block reads and writes 32 KB of a slot at a
+    // stretch (40 slots: 382 -> 267 us; a fork, reading its source for each copy, would take
+    // 245 instead of 173), as long as the blocks fill 148 SMs twice.
+    bool one = false;
     unsigned long long blocks = 0;
     for (int c = 0; c < n_comp; ++c) {
         uint32_t r0 = 0xffffffffu, r1 = 0;
         for (uint32_t j = comp[c]; j < comp[c + 1]; ++j) {
             r0 = ins[j].start < r0 ? ins[j].start : r0;
             r1 = ins[j].start + ins[j].len > r1 ? ins[j].start + ins[j].len : r1;
+            one |= ins[j].src == MOVE_TMP || ins[j].dst == MOVE_TMP || (j > comp[c] && ins[j].src == ins[j - 1].src);
         }
         p.row0[c] = r0;
         p.rows[c] = r1 - r0;
-        p.block[c] = (uint32_t)blocks;
-        const unsigned long long span = (unsigned long long)(r1 - r0) * (g.row_bytes / vec);
-        blocks += (span + MV_THREADS * MV_OFF - 1) / (MV_THREADS * MV_OFF) * g.n_outer * g.n_base;
-        if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+    }
+    for (p.iter = one ? 1 : 8;; p.iter /= 2) {
+        const unsigned long long per_block = (unsigned long long)MV_THREADS * p.iter;
+        blocks = 0;
+        for (int c = 0; c < n_comp; ++c) {
+            p.block[c] = (uint32_t)blocks;
+            blocks += (p.rows[c] * (unsigned long long)(g.row_bytes / vec) + per_block - 1) / per_block * g.n_outer *
+                      g.n_base;
+            if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+        }
+        if (p.iter == 1 || blocks >= 2 * 8 * 148) break;
     }
     p.block[n_comp] = (uint32_t)blocks;
     if (blocks == 0) return cudaSuccess;
