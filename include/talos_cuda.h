@@ -266,6 +266,56 @@ talos_status talos_generate_batch_greedy(talos_ctx* ctx, const uint32_t* tokens,
                                          size_t steps, uint32_t* tokens_out);
 
 /*
+ * Batched decode with drawn tokens: as talos_generate_batch_greedy, but step k's
+ * token of sequence i is talos_sample_dev's choice from its logits with settings[i]
+ * and the random number u[k * n + i] (host, in [0, 1)). A temperature of 0 is the
+ * greedy choice (the lowest index among equal logits, where talos_sample_dev's order
+ * starts; talos_generate_batch_greedy takes the highest). The same numbers give the
+ * same tokens. A row whose logits are all NaN or -inf ends the call with
+ * TALOS_ERR_OOB. The reference draws one sequence's tokens on the host
+ * (src/sample.rs:19-76).
+ */
+typedef struct talos_sampling {
+    float temperature; /* <= 0: the first of the order */
+    int32_t top_k;     /* 0: off */
+    float top_p;       /* >= 1: off */
+    float min_p;       /* 0: off */
+} talos_sampling;
+talos_status talos_generate_batch_sample(talos_ctx* ctx, const uint32_t* tokens, const size_t* pos, int n,
+                                         size_t steps, const talos_sampling* settings, const float* u,
+                                         uint32_t* tokens_out);
+
+/*
+ * A prefix shared by every sequence of the batch: positions 0 .. n-1 of slot `slot`
+ * (filled before, talos_prefill_slot) become positions 0 .. n-1 of all of them. Their
+ * rows are kept once, beside the slots; talos_forward_batch, talos_prefill_slot and the
+ * batched generation then attend to them once for all sequences (the tensor-core
+ * attention of talos_attention_shared_dev) and to the slots' own rows from position n
+ * on, and refuse positions below n. The slots keep rows by their absolute positions.
+ * A call with a prefix in place extends it from the slot's rows behind it, or cuts it;
+ * n = 0 ends the sharing (the slots' rows below the old prefix are then what they were
+ * before it, so only slots that were filled themselves can go on). Takes the memory of
+ * one more slot, from the first call to the release of the slots. The attention's
+ * scores and weights are exact to about 22 bits, like the f32 path's own roundings;
+ * results with and without sharing differ in their last bits. Under tensor parallelism
+ * every rank makes the call. No reference counterpart.
+ */
+talos_status talos_batch_share(talos_ctx* ctx, int slot, size_t n);
+
+/*
+ * Copies of rows between the batch's cache slots, all at once (talos_kv_move_dev on the
+ * context's cache): the rows of positions start .. start+len-1 of slot src, in every
+ * layer, to slot dst. A prompt forked into other slots, live sequences moved to the
+ * front (decode steps take slots 0 .. n-1), or slots exchanged; every source is read as
+ * it was before the call, no slot may be the destination of two copies. Under tensor
+ * parallelism every rank makes the call. No reference counterpart.
+ */
+typedef struct talos_kv_copy {
+    uint32_t src, dst, start, len;
+} talos_kv_copy;
+talos_status talos_batch_move(talos_ctx* ctx, const talos_kv_copy* moves, size_t n);
+
+/*
  * Teacher-forced perplexity of tokens[0..n) (n >= 2): eval::perplexity
  * (src/eval.rs:35-52). The tokens are scored in chunks of the context length,
  * each from an empty KV cache; at each position the negative log-likelihood of
@@ -521,9 +571,6 @@ typedef struct talos_kv_slots {
     size_t slot_stride, outer_stride, row_stride; /* bytes */
     size_t row_bytes;
 } talos_kv_slots;
-typedef struct talos_kv_copy {
-    uint32_t src, dst, start, len;
-} talos_kv_copy;
 talos_status talos_kv_move_dev(const talos_kv_slots* slots, const talos_kv_copy* moves, size_t n, void* stream);
 
 #ifdef __cplusplus

@@ -62,6 +62,18 @@ class KvSlots(C.Structure):
                 ("outer_stride", C.c_size_t), ("row_stride", C.c_size_t), ("row_bytes", C.c_size_t)]
 
 
+class Sampling(C.Structure):
+    """``talos_sampling``."""
+
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
+class KvCopy(C.Structure):
+    """``talos_kv_copy``."""
+
+    _fields_ = [(n, C.c_uint32) for n in ("src", "dst", "start", "len")]
+
+
 # Every symbol include/talos_cuda.h declares, with its ctypes signature.
 _vp, _sz, _u32, _i = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int
 SIGNATURES = {
@@ -81,6 +93,10 @@ SIGNATURES = {
     "talos_prefill_slot": (_i, [_vp, _i, C.POINTER(C.c_uint32), _sz, _sz, C.POINTER(C.c_float)]),
     "talos_generate_batch_greedy": (_i, [_vp, C.POINTER(C.c_uint32), C.POINTER(_sz), _i, _sz,
                                          C.POINTER(C.c_uint32)]),
+    "talos_generate_batch_sample": (_i, [_vp, C.POINTER(C.c_uint32), C.POINTER(_sz), _i, _sz, C.POINTER(Sampling),
+                                         C.POINTER(C.c_float), C.POINTER(C.c_uint32)]),
+    "talos_batch_share": (_i, [_vp, _i, _sz]),
+    "talos_batch_move": (_i, [_vp, C.POINTER(KvCopy), _sz]),
     "talos_ctx_kv_dtype": (_i, [_vp, C.POINTER(_i)]),
     "talos_ctx_device_bytes": (_i, [_vp, C.POINTER(_sz)]),
     "talos_ctx_stream": (_i, [_vp, C.POINTER(_vp)]),

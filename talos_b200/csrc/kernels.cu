@@ -577,6 +577,30 @@ cudaError_t launch_greedy_advance_b(const float* logits, int V, BatchParams* bp,
     return cudaGetLastError();
 }
 
+__global__ void k_sample_advance_b(const int32_t* chosen, const float* u_all, float* u_cur, BatchParams* bp,
+                                   uint32_t* gen, int cap) {
+    const int s = threadIdx.x;
+    if (s >= bp->n) return;
+    int32_t tok = chosen[s];
+    if (tok < 0) {  // no finite logit, nothing to choose
+        atomicOr(&bp->error, 1u);
+        tok = 0;
+    }
+    const uint32_t n = bp->ngen[s];
+    if (n < (uint32_t)cap) gen[(size_t)s * cap + n] = (uint32_t)tok;
+    if (n + 1 < (uint32_t)cap) u_cur[s] = u_all[(size_t)s * cap + n + 1];
+    bp->ngen[s] = n + 1;
+    bp->token[s] = (uint32_t)tok;
+    bp->pos[s] += 1;
+    if (s == 0) bp->tpstep += 1;  // read only by the next step's kernels
+}
+
+cudaError_t launch_sample_advance_b(const int32_t* tok, const float* u_all, float* u_cur, BatchParams* bp,
+                                    uint32_t* gen, int cap, cudaStream_t s) {
+    k_sample_advance_b<<<1, MB_SEQ, 0, s>>>(tok, u_all, u_cur, bp, gen, cap);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_swiglu_b(const float* g, const float* u, float* h, int ld, int n_ff, const BatchParams* bp,
                             cudaStream_t s) {
     k_swiglu_b<<<dim3((n_ff + 255) / 256, MB_SEQ), 256, 0, s>>>(g, u, h, ld, n_ff, bp);

@@ -92,6 +92,7 @@ struct BatchParams {
     uint32_t ngen[MB_SEQ];     // batched greedy: tokens chosen so far per column
     uint32_t error;            // device-side error bits (1: token out of range, 2: a bounded wait expired)
     uint32_t tpstep;           // tensor parallel: earlier batched steps of the context (k_tp_join_b targets)
+    uint32_t prefix;           // positions 0 .. prefix-1 of every column are the shared prefix's rows
 };
 
 // Batched epilogues: store / add rows; RoPE of q rows (stored to y); RoPE of k
@@ -184,6 +185,11 @@ cudaError_t launch_embed_b(const uint8_t* embd_raw, int type, int cols, int voca
 // appended to gen[s * cap + ngen[s]]; then tpstep advances by one.
 cudaError_t launch_greedy_advance_b(const float* logits, int V, BatchParams* bp, uint32_t* gen, int cap,
                                     cudaStream_t s);
+// Batched sampling: column s's chosen token tok[s] becomes its next token as above; its
+// next random number u_cur[s] is u_all[s * cap + ngen[s]]. A row without a choice
+// (tok < 0) sets error bit 1.
+cudaError_t launch_sample_advance_b(const int32_t* tok, const float* u_all, float* u_cur, BatchParams* bp,
+                                    uint32_t* gen, int cap, cudaStream_t s);
 cudaError_t launch_swiglu_b(const float* g, const float* u, float* h, int ld, int n_ff, const BatchParams* bp,
                             cudaStream_t s);
 // GQA attention per (head, sequence) over positions 0 .. pos[s] (src/model/llama.rs:135-155)

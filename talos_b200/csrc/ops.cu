@@ -35,8 +35,11 @@ talos_status on_device(const OnDevice& d, int device) {
                    cudaGetErrorString(d.err));
 }
 
-// Kernel attributes of the current device, set on its first call.
-talos_status configured(int device) {
+bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
+
+}  // namespace
+
+talos_status talos::ops_configured(int device) {
     static std::mutex mu;
     static bool done[64];
     if (device < 0 || device >= 64) return set_err(TALOS_ERR_INVALID_ARG, "device %d", device);
@@ -47,10 +50,6 @@ talos_status configured(int device) {
     done[device] = true;
     return TALOS_OK;
 }
-
-bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
-
-}  // namespace
 
 // ------------------------------------------------------------------ token choice
 
@@ -72,7 +71,7 @@ extern "C" talos_status talos_sample_dev(const talos_sample_args* a, void* strea
     if (!a->top_k_dev && a->top_k < 0) return set_err(TALOS_ERR_INVALID_ARG, "top_k %d", a->top_k);
     OnDevice d(a->device);
     TRY(on_device(d, a->device));
-    TRY(configured(a->device));
+    TRY(ops_configured(a->device));
     SampleArgs k{};
     k.logits = a->logits;
     k.stride = a->n > 1 ? a->row_stride : a->vocab;
@@ -176,7 +175,7 @@ extern "C" talos_status talos_attention_shared_dev(const talos_attention_shared_
         return set_err(TALOS_ERR_INVALID_ARG, "a pointer is not aligned to its element");
     OnDevice d(a->device);
     TRY(on_device(d, a->device));
-    TRY(configured(a->device));
+    TRY(ops_configured(a->device));
     k.q = a->q, k.kp = a->k_prefix, k.vp = a->v_prefix, k.k = a->k, k.v = a->v, k.out = a->out;
     k.n = (int)a->n, k.n_kv = (int)a->n_head_kv, k.group = (int)(a->n_head / a->n_head_kv), k.hd = (int)a->head_dim;
     k.prefix = (int)a->prefix_len, k.n_slots = (int)a->n_slots, k.slot_len = (int)a->slot_len;

@@ -30,6 +30,7 @@ struct SampleArgs {
     float top_p, min_p;
     int32_t* tokens;  // [n]
     float* probs;     // [n] or null
+    const int* n_dev;  // or null: rows in device memory (n is then their largest number)
 };
 constexpr int SAMPLE_MAX_VOCAB = 1 << 20;
 cudaError_t sample_configure();  // once per device, on the current one

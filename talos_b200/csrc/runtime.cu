@@ -30,6 +30,7 @@
 
 #include "../../include/talos_cuda.h"
 #include "kernels.cuh"
+#include "ops.cuh"
 #include "status.cuh"
 
 using namespace talos;
@@ -451,9 +452,19 @@ struct talos_ctx {
     size_t bseq_stride = 0;                // floats per sequence in bkc / bvc
     float* h_blog = nullptr;               // pinned [TALOS_MAX_BATCH][V]
     alignas(64) uint8_t bmaps[3][128];     // tensor maps of bplanes for 32 / 64 / 128-column tiles
-    cudaGraphExec_t bgraph[5][3] = {};     // [BatchMode][token-tile size]
+    cudaGraphExec_t bgraph[6][3][2] = {};  // [BatchMode][token-tile size][with a shared prefix]
     uint32_t* bgen = nullptr;              // batched greedy: [MB_SEQ][kv_ctx] chosen tokens
     int bgen_cap = 0;
+    // batched sampling: [MB_SEQ][bgen_cap] random numbers, and per column {temperature,
+    // top-k, top-p, min-p, the step's random number, its token}
+    float *bu_all = nullptr, *bset = nullptr;
+    // shared prefix (talos_batch_share): its length, rows ([n_layer][kv_ctx][kv_dim] of K,
+    // then of V) and the attention's workspace; one allocation, made at the first use
+    size_t bprefix = 0;
+    void* bpmem = nullptr;
+    float *bpk = nullptr, *bpv = nullptr;
+    void* bpwork = nullptr;
+    size_t bpbytes = 0;
     // tensor parallel: the batched steps' IPC-exported area {arrival counters
     // [2 n_layer + 1], abort word, receive slots [2][tp][MB_SEQ][E], gathered
     // logits [MB_SEQ][V]}, every rank's mapping of it, and the local count of
@@ -466,11 +477,12 @@ struct talos_ctx {
 
     void drop_batch_graphs() {
         for (auto& row : bgraph)
-            for (auto& g : row)
-                if (g) {
-                    cudaGraphExecDestroy(g);
-                    g = nullptr;
-                }
+            for (auto& pair : row)
+                for (auto& g : pair)
+                    if (g) {
+                        cudaGraphExecDestroy(g);
+                        g = nullptr;
+                    }
     }
     void drop_graphs() {
         for (auto& g : graph)
@@ -909,7 +921,7 @@ extern "C" talos_status talos_weight_upload(talos_ctx* c, const char* name, cons
 
 extern "C" talos_status talos_ctx_device_bytes(talos_ctx* c, size_t* out) {
     if (!c || !out) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
-    size_t n = c->arena_bytes + c->kv_bytes + c->staging.cap + c->sync_bytes + c->weights.total + c->bbytes;
+    size_t n = c->arena_bytes + c->kv_bytes + c->staging.cap + c->sync_bytes + c->weights.total + c->bbytes + c->bpbytes;
     for (auto& kv : c->resident) n += kv.second.bytes;
     *out = n;
     return TALOS_OK;
@@ -1657,15 +1669,20 @@ static talos_status profile_fused(talos_ctx* c, double* kernel_ms, uint32_t* lau
 //  * BM_FILL (talos_prefill_slot): consecutive prompt positions of one
 //    sequence of the batch, into its cache slot, no logits;
 //  * BM_GREEDY (talos_generate_batch_greedy): BM_DECODE, then each column's
-//    argmax becomes its next token on the device (replayed step after step).
+//    argmax becomes its next token on the device (replayed step after step);
+//  * BM_SAMPLE (talos_generate_batch_sample): the same with a token drawn by each
+//    column's settings.
+// With a shared prefix (talos_batch_share) the steps on the sequences' slots read
+// positions 0 .. prefix-1 from its rows, once for all columns.
 // The step is the layered sequence of src/model/llama.rs:96-183 per column:
 // embedding row; per layer GEMM q/k/v (RoPE, cache append), attention, GEMM
 // o-proj (+ residual), GEMM gate/up (SwiGLU), GEMM down (+ residual); then the
 // final norm and the output GEMM. A column at position p attends to positions
 // 0 .. p of its cache, so prompt positions of one step see each other's rows.
 
-enum BatchMode { BM_DECODE = 0, BM_PREFILL = 1, BM_SCORE = 2, BM_FILL = 3, BM_GREEDY = 4 };
-static bool mode_slots(int mode) { return mode == BM_DECODE || mode == BM_FILL || mode == BM_GREEDY; }
+enum BatchMode { BM_DECODE = 0, BM_PREFILL = 1, BM_SCORE = 2, BM_FILL = 3, BM_GREEDY = 4,
+                 BM_SAMPLE = 5 };
+static bool mode_slots(int mode) { return mode != BM_PREFILL && mode != BM_SCORE; }
 static bool mode_logits(int mode) { return mode != BM_PREFILL && mode != BM_FILL; }
 static int nt_of(int ntc) { return 32 << ntc; }
 static int ntc_for(int n) { return n <= 32 ? 0 : (n <= 64 ? 1 : 2); }
@@ -1676,6 +1693,9 @@ static talos_status batch_free(talos_ctx* c) {
     CK(cudaStreamSynchronize(c->stream));
     c->drop_batch_graphs();
     if (c->bmem) cudaFree(c->bmem);
+    if (c->bpmem) cudaFree(c->bpmem);
+    c->bpmem = nullptr;
+    c->bprefix = c->bpbytes = 0;
     c->bmem = nullptr;
     c->bbytes = 0;
     c->bmax = 0;
@@ -1737,7 +1757,8 @@ static talos_status batch_alloc_body(talos_ctx* c, int max_seqs) {
     const size_t seq_stride = L * c->kv_ctx * (size_t)c->kv_l;
     const size_t o_kc = take((size_t)max_seqs * seq_stride * 4 + 4), o_vc = take((size_t)max_seqs * seq_stride * 4 + 4);
     const int gen_cap = max_seqs ? (int)c->kv_ctx : 0;
-    const size_t o_gen = take((size_t)MB_SEQ * gen_cap * 4 + 4);
+    const size_t o_gen = take((size_t)MB_SEQ * gen_cap * 4 + 4), o_ua = take((size_t)MB_SEQ * gen_cap * 4 + 4),
+                 o_set = take(6 * MB_SEQ * 4);
     void* mem = nullptr;
     CK(cudaMalloc(&mem, off));
     CK(cudaMemsetAsync(mem, 0, off, c->stream));
@@ -1754,6 +1775,7 @@ static talos_status batch_alloc_body(talos_ctx* c, int max_seqs) {
     c->bws = (float*)(b + o_ws), c->bcnt = (unsigned*)(b + o_cnt);
     c->bkc = (float*)(b + o_kc), c->bvc = (float*)(b + o_vc);
     c->bgen = (uint32_t*)(b + o_gen), c->bgen_cap = gen_cap;
+    c->bu_all = (float*)(b + o_ua), c->bset = (float*)(b + o_set);
     c->bseq_stride = seq_stride;
     if (gemm_map_bytes() > sizeof c->bmaps[0]) return set_err(TALOS_ERR_CUDA, "tensor map larger than its slot");
     for (int i = 0; i < 3; ++i) {
@@ -1894,7 +1916,7 @@ static talos_status tp_join(talos_ctx* c, int inst, int grid, bool sum, int buf)
     return TALOS_OK;
 }
 
-static talos_status enqueue_batch(talos_ctx* c, int mode, int ntc) {
+static talos_status enqueue_batch(talos_ctx* c, int mode, int ntc, bool shared) {
     const talos_cfg& cfg = c->cfg;
     const int E = (int)cfg.n_embd, Fl = c->ff_l, V = (int)cfg.vocab_size, Q = c->q_rows;
     const bool tp = c->tp > 1;
@@ -1937,8 +1959,24 @@ static talos_status enqueue_batch(talos_ctx* c, int mode, int ntc) {
         // attention (llama.rs:135-155), o-proj + residual (:157-161); under
         // tensor parallelism the o-proj is row-parallel: partial rows to every
         // rank, summed into the residual by the join
-        e = launch_attention_b(c->bq, Q, kc, vc, seq_stride, c->kv_l, c->nh_l, c->nkv_l, c->hd, c->batt, Q, c->bp,
-                               c->stream);
+        if (shared) {
+            AttnSharedArgs a{};
+            a.q = c->bq, a.q_sn = Q, a.q_sh = c->hd;
+            a.kp = c->bpk + l * kv_layer, a.vp = c->bpv + l * kv_layer, a.pre_st = c->kv_l, a.pre_sh = c->hd;
+            a.k = kc, a.v = vc, a.slot_ss = seq_stride, a.slot_st = c->kv_l, a.slot_sh = c->hd;
+            a.out = c->batt, a.out_sn = Q, a.out_sh = c->hd;
+            a.n = nt_of(ntc), a.n_kv = c->nkv_l, a.group = c->nh_l / c->nkv_l, a.hd = c->hd;
+            a.prefix = a.slot_len = (int)c->kv_ctx;
+            a.n_slots = c->bmax;
+            a.slots = (const int32_t*)c->bp->slot;
+            a.scale = 1.0f / sqrtf((float)c->hd);
+            a.n_dev = &c->bp->n, a.prefix_dev = &c->bp->prefix, a.pos = c->bp->pos, a.slot_row0 = 1;
+            a.error = &c->bp->error;
+            e = launch_attn_shared(a, DT_F32, DT_F32, c->bpwork, sm_count_dev(c->device), c->stream);
+        } else {
+            e = launch_attention_b(c->bq, Q, kc, vc, seq_stride, c->kv_l, c->nh_l, c->nkv_l, c->hd, c->batt, Q, c->bp,
+                                   c->stream);
+        }
         if (e != cudaSuccess) return set_err(TALOS_ERR_CUDA, "batched attention: %s", cudaGetErrorString(e));
         {
             GemmArgs a{};
@@ -1991,6 +2029,21 @@ static talos_status enqueue_batch(talos_ctx* c, int mode, int ntc) {
         e = launch_greedy_advance_b(c->blog, V, c->bp, c->bgen, c->bgen_cap, c->stream);
         if (e != cudaSuccess) return set_err(TALOS_ERR_CUDA, "batched greedy: %s", cudaGetErrorString(e));
     }
+    if (mode == BM_SAMPLE) {
+        SampleArgs a{};
+        a.logits = c->blog, a.stride = V;
+        a.n = nt_of(ntc), a.vocab = V;
+        a.n_dev = &c->bp->n;
+        a.temperature_dev = c->bset, a.top_k_dev = (const int32_t*)c->bset + MB_SEQ;
+        a.top_p_dev = c->bset + 2 * MB_SEQ, a.min_p_dev = c->bset + 3 * MB_SEQ;
+        float* u = c->bset + 4 * MB_SEQ;
+        a.u = u;
+        a.tokens = (int32_t*)c->bset + 5 * MB_SEQ;
+        e = launch_sample(a, DT_F32, sm_count_dev(c->device), c->stream);
+        if (e == cudaSuccess)
+            e = launch_sample_advance_b(a.tokens, c->bu_all, u, c->bp, c->bgen, c->bgen_cap, c->stream);
+        if (e != cudaSuccess) return set_err(TALOS_ERR_CUDA, "batched sampling: %s", cudaGetErrorString(e));
+    }
     return TALOS_OK;
 }
 
@@ -2011,12 +2064,13 @@ __global__ void k_set_batch(BatchParams* d, BatchParams v, bool keep_err) {
     *d = v;
 }
 
+static bool with_prefix(const talos_ctx* c, int mode) { return mode_slots(mode) && c->bprefix; }
 static talos_status batch_graph(talos_ctx* c, int mode, int ntc) {
-    cudaGraphExec_t* out = &c->bgraph[mode][ntc];
+    cudaGraphExec_t* out = &c->bgraph[mode][ntc][with_prefix(c, mode)];
     if (*out) return TALOS_OK;
     cudaGraph_t g = nullptr;
     CK(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
-    talos_status st = enqueue_batch(c, mode, ntc);
+    talos_status st = enqueue_batch(c, mode, ntc, with_prefix(c, mode));
     cudaError_t e = cudaStreamEndCapture(c->stream, &g);
     if (st != TALOS_OK) {
         if (g) cudaGraphDestroy(g);
@@ -2043,6 +2097,7 @@ static talos_status set_batch_params(talos_ctx* c, const uint32_t* tokens, const
         v.slot[i] = slots ? (uint32_t)slots[i] : (uint32_t)i;
     }
     v.tpstep = c->btpstep;
+    v.prefix = (uint32_t)c->bprefix;
     k_set_batch<<<1, 1, 0, c->stream>>>(c->bp, v, !first);
     CK(cudaGetLastError());
     return TALOS_OK;
@@ -2056,7 +2111,7 @@ static talos_status batch_step(talos_ctx* c, int mode, const uint32_t* tokens, c
     const int ntc = ntc_for(n);
     TRY(batch_graph(c, mode, ntc));
     TRY(set_batch_params(c, tokens, pos, slots, n, first));
-    CK(cudaGraphLaunch(c->bgraph[mode][ntc], c->stream));
+    CK(cudaGraphLaunch(c->bgraph[mode][ntc][with_prefix(c, mode)], c->stream));
     if (c->tp > 1) ++c->btpstep;
     return TALOS_OK;
 }
@@ -2074,13 +2129,21 @@ static talos_status batch_finish(talos_ctx* c, int n, float* logits_out) {
     return TALOS_OK;
 }
 
+// A column's token and position in a step on the sequences' slots.
+static talos_status check_slot_pos(talos_ctx* c, uint32_t token, size_t pos) {
+    TRY(check_tok_pos(c, token, pos));
+    if (pos < c->bprefix)
+        return set_err(TALOS_ERR_INVALID_ARG, "position %zu lies in the shared prefix (%zu rows)", pos, c->bprefix);
+    return TALOS_OK;
+}
+
 extern "C" talos_status talos_forward_batch(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
                                             float* logits_out) {
     if (!c || !tokens || !pos || !logits_out) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
     if (n < 1 || n > c->bmax)
         return set_err(TALOS_ERR_INVALID_ARG, "%d sequences (the context holds %d; talos_ctx_set_batch)", n, c->bmax);
     CK(cudaSetDevice(c->device));
-    for (int i = 0; i < n; ++i) TRY(check_tok_pos(c, tokens[i], pos[i]));
+    for (int i = 0; i < n; ++i) TRY(check_slot_pos(c, tokens[i], pos[i]));
     TRY(bind_if_dirty(c));
     TRY(batch_check(c));
     TRY(batch_step(c, BM_DECODE, tokens, pos, nullptr, n, true));
@@ -2094,7 +2157,7 @@ extern "C" talos_status talos_prefill_slot(talos_ctx* c, int slot, const uint32_
         return set_err(TALOS_ERR_INVALID_ARG, "slot %d (the context holds %d; talos_ctx_set_batch)", slot, c->bmax);
     if (n == 0) return TALOS_OK;
     CK(cudaSetDevice(c->device));
-    for (size_t i = 0; i < n; ++i) TRY(check_tok_pos(c, tokens[i], pos0 + i));
+    for (size_t i = 0; i < n; ++i) TRY(check_slot_pos(c, tokens[i], pos0 + i));
     TRY(bind_if_dirty(c));
     TRY(batch_check(c));
     std::vector<size_t> pos(MB_SEQ);
@@ -2116,33 +2179,128 @@ extern "C" talos_status talos_prefill_slot(talos_ctx* c, int slot, const uint32_
     return TALOS_OK;
 }
 
-extern "C" talos_status talos_generate_batch_greedy(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
-                                                    size_t steps, uint32_t* tokens_out) {
+// The device-driven decode loop: `steps` replays of the mode's graph, which advances every
+// column's token and position itself (and the tensor-parallel step count).
+static talos_status batch_generate(talos_ctx* c, int mode, const uint32_t* tokens, const size_t* pos, int n,
+                                   size_t steps, const talos_sampling* set, const float* u, uint32_t* tokens_out) {
     if (!c || !tokens || !pos || (!tokens_out && steps)) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
+    if (mode == BM_SAMPLE && (!set || (!u && steps))) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
     if (n < 1 || n > c->bmax)
         return set_err(TALOS_ERR_INVALID_ARG, "%d sequences (the context holds %d; talos_ctx_set_batch)", n, c->bmax);
     if (steps == 0) return TALOS_OK;
     CK(cudaSetDevice(c->device));
     for (int i = 0; i < n; ++i) {
-        TRY(check_tok_pos(c, tokens[i], pos[i]));
-        if (pos[i] + steps > c->kv_ctx)
+        TRY(check_slot_pos(c, tokens[i], pos[i]));
+        if (steps > c->kv_ctx || pos[i] + steps > c->kv_ctx)
             return set_err(TALOS_ERR_INVALID_ARG, "sequence %d: positions %zu .. %zu beyond the context (%zu)", i,
                            pos[i], pos[i] + steps - 1, c->kv_ctx);
+        if (set && set[i].top_k < 0) return set_err(TALOS_ERR_INVALID_ARG, "sequence %d: top_k %d", i, set[i].top_k);
     }
     TRY(bind_if_dirty(c));
     TRY(batch_check(c));
+    if (mode == BM_SAMPLE) {
+        if (c->cfg.vocab_size > (uint32_t)SAMPLE_MAX_VOCAB)
+            return set_err(TALOS_ERR_UNSUPPORTED, "%u logits per row (at most %d)", c->cfg.vocab_size, SAMPLE_MAX_VOCAB);
+        TRY(ops_configured(c->device));
+        float rows[5 * MB_SEQ] = {};  // as in bset
+        for (int i = 0; i < n; ++i) {
+            rows[i] = set[i].temperature;
+            memcpy(&rows[MB_SEQ + i], &set[i].top_k, 4);
+            rows[2 * MB_SEQ + i] = set[i].top_p, rows[3 * MB_SEQ + i] = set[i].min_p;
+            rows[4 * MB_SEQ + i] = u[i];
+        }
+        std::vector<float> ut((size_t)n * steps);  // a sequence's numbers in a row
+        for (size_t k = 0; k < steps; ++k)
+            for (int i = 0; i < n; ++i) ut[i * steps + k] = u[k * n + i];
+        // pageable memory: the copies have read it when the calls return
+        CK(cudaMemcpyAsync(c->bset, rows, sizeof rows, cudaMemcpyHostToDevice, c->stream));
+        CK(cudaMemcpy2DAsync(c->bu_all, (size_t)c->bgen_cap * 4, ut.data(), steps * 4, steps * 4, n,
+                             cudaMemcpyHostToDevice, c->stream));
+    }
     const int ntc = ntc_for(n);
-    TRY(batch_graph(c, BM_GREEDY, ntc));
+    TRY(batch_graph(c, mode, ntc));
     TRY(set_batch_params(c, tokens, pos, nullptr, n, true));
-    // the graph advances every column's token and position itself (and the
-    // tensor-parallel step count), so the replays need no host work
-    for (size_t k = 0; k < steps; ++k) CK(cudaGraphLaunch(c->bgraph[BM_GREEDY][ntc], c->stream));
+    for (size_t k = 0; k < steps; ++k) CK(cudaGraphLaunch(c->bgraph[mode][ntc][with_prefix(c, mode)], c->stream));
     if (c->tp > 1) c->btpstep += (uint32_t)steps;
     TRY(batch_finish(c, 0, nullptr));
     std::vector<uint32_t> g((size_t)n * c->bgen_cap);
     CK(cudaMemcpy(g.data(), c->bgen, g.size() * 4, cudaMemcpyDeviceToHost));
     for (size_t k = 0; k < steps; ++k)
         for (int i = 0; i < n; ++i) tokens_out[k * n + i] = g[(size_t)i * c->bgen_cap + k];
+    return TALOS_OK;
+}
+
+extern "C" talos_status talos_generate_batch_greedy(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
+                                                    size_t steps, uint32_t* tokens_out) {
+    return batch_generate(c, BM_GREEDY, tokens, pos, n, steps, nullptr, nullptr, tokens_out);
+}
+
+extern "C" talos_status talos_generate_batch_sample(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
+                                                    size_t steps, const talos_sampling* set, const float* u,
+                                                    uint32_t* tokens_out) {
+    try {
+        return batch_generate(c, BM_SAMPLE, tokens, pos, n, steps, set, u, tokens_out);
+    } catch (const std::bad_alloc&) {
+        return set_err(TALOS_ERR_OOM, "host memory for %zu steps", steps);
+    }
+}
+
+extern "C" talos_status talos_batch_share(talos_ctx* c, int slot, size_t n) {
+    if (!c) return set_err(TALOS_ERR_INVALID_ARG, "NULL ctx");
+    if (slot < 0 || slot >= c->bmax)
+        return set_err(TALOS_ERR_INVALID_ARG, "slot %d (the context holds %d; talos_ctx_set_batch)", slot, c->bmax);
+    if (n > c->kv_ctx)
+        return set_err(TALOS_ERR_INVALID_ARG, "a prefix of %zu rows (the context has %zu)", n, c->kv_ctx);
+    CK(cudaSetDevice(c->device));
+    if (n && !c->bpmem) {
+        const int group = c->nkv_l ? c->nh_l / c->nkv_l : 0;
+        if (c->hd > 128 || c->hd % 4 || group < 1 || group > 128)
+            return set_err(TALOS_ERR_UNSUPPORTED, "a shared prefix needs head_dim <= 128 and 1 .. 128 heads per kv head");
+        TRY(ops_configured(c->device));
+        const size_t rows = align256((size_t)c->cfg.n_layer * c->kv_ctx * c->kv_l * 4);
+        const size_t bytes = 2 * rows + attn_shared_work_bytes(MB_SEQ, group, sm_count_dev(c->device));
+        void* mem = nullptr;
+        CK(cudaMalloc(&mem, bytes));
+        const cudaError_t e = cudaMemsetAsync(mem, 0, bytes, c->stream);
+        if (e != cudaSuccess) {
+            cudaFree(mem);
+            CK(e);
+        }
+        c->bpmem = mem;
+        c->bpbytes = bytes;
+        c->bpk = (float*)mem, c->bpv = (float*)((uint8_t*)mem + rows);
+        c->bpwork = (uint8_t*)mem + 2 * rows;
+    }
+    if (n > c->bprefix) {  // the rows behind the present prefix (a plane per layer)
+        const size_t from = c->bprefix * c->kv_l, pitch = c->kv_ctx * (size_t)c->kv_l * 4;
+        const size_t src = (size_t)slot * c->bseq_stride + from, width = (n - c->bprefix) * c->kv_l * 4;
+        CK(cudaMemcpy2DAsync(c->bpk + from, pitch, c->bkc + src, pitch, width, c->cfg.n_layer,
+                             cudaMemcpyDeviceToDevice, c->stream));
+        CK(cudaMemcpy2DAsync(c->bpv + from, pitch, c->bvc + src, pitch, width, c->cfg.n_layer,
+                             cudaMemcpyDeviceToDevice, c->stream));
+    }
+    c->bprefix = n;
+    CK(cudaStreamSynchronize(c->stream));
+    return TALOS_OK;
+}
+
+extern "C" talos_status talos_batch_move(talos_ctx* c, const talos_kv_copy* moves, size_t n) {
+    if (!c || (!moves && n)) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
+    if (!c->bmax) return set_err(TALOS_ERR_STATE, "no cache slots (talos_ctx_set_batch)");
+    CK(cudaSetDevice(c->device));
+    void* base[2] = {c->bkc, c->bvc};
+    talos_kv_slots g{};
+    g.device = c->device;
+    g.n_base = 2;
+    g.base = base;
+    g.n_slots = (uint32_t)c->bmax;
+    g.n_outer = c->cfg.n_layer;
+    g.n_rows = (uint32_t)c->kv_ctx;
+    g.slot_stride = c->bseq_stride * 4;
+    g.row_stride = g.row_bytes = (size_t)c->kv_l * 4;
+    g.outer_stride = c->kv_ctx * g.row_stride;
+    TRY(talos_kv_move_dev(&g, moves, n, c->stream));
+    CK(cudaStreamSynchronize(c->stream));
     return TALOS_OK;
 }
 

@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int row = blockIdx.x / C;
+    if (a.n_dev && row >= *a.n_dev) return;  // (the whole cluster)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int VW = 16 / (int)sizeof(T);
     SpSmem* lead = cluster.map_shared_rank(&s, 0);

@@ -12,6 +12,8 @@ namespace talos {
 talos_status set_err(talos_status st, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // The streaming multiprocessors of a device (148 if it cannot be asked).
 int sm_count_dev(int device);
+// Set the attributes of the operators' kernels on a device (once each; it must be current).
+talos_status ops_configured(int device);
 
 }  // namespace talos
 

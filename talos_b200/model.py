@@ -214,6 +214,47 @@ class Context:
                                                            out.ctypes.data_as(C.POINTER(C.c_uint32))))
         return out[: int(steps)]
 
+    def generate_batch_sample(self, tokens, positions, u, temperature=1.0, top_k=0, top_p=1.0,
+                              min_p=0.0) -> np.ndarray:
+        """talos_generate_batch_sample: as ``generate_batch_greedy`` with tokens drawn by
+        the random numbers u [steps, n] (in [0, 1)); each setting is one value or one per
+        sequence. Returns the chosen tokens as [steps, n]."""
+        t = np.ascontiguousarray(tokens, np.uint32)
+        p = np.ascontiguousarray(positions, np.uint64)
+        u = np.ascontiguousarray(u, np.float32)
+        n = len(t)
+        if len(p) != n:
+            raise ValueError("tokens and positions differ in length")
+        if u.ndim != 2 or u.shape[1] != n:
+            raise ValueError(f"u: random numbers of shape [steps, {n}] expected, got {list(u.shape)}")
+        steps = u.shape[0]
+        set_ = (_lib.Sampling * max(n, 1))()
+        for name, v, kind in (("temperature", temperature, float), ("top_k", top_k, int), ("top_p", top_p, float),
+                              ("min_p", min_p, float)):
+            v = np.broadcast_to(np.asarray(v), (n,))
+            for i in range(n):
+                setattr(set_[i], name, kind(v[i]))
+        out = np.empty((max(steps, 1), n), np.uint32)
+        _lib.check(_lib.load().talos_generate_batch_sample(
+            self.h, t.ctypes.data_as(C.POINTER(C.c_uint32)), p.ctypes.data_as(C.POINTER(C.c_size_t)), n, steps, set_,
+            u.ctypes.data_as(C.POINTER(C.c_float)), out.ctypes.data_as(C.POINTER(C.c_uint32))))
+        return out[:steps]
+
+    def batch_share(self, slot: int, n: int):
+        """talos_batch_share: positions 0 .. n-1 of ``slot`` become the prefix of every
+        sequence of the batch (kept and read once); 0 ends the sharing."""
+        if n < 0:
+            raise ValueError("a prefix of less than no rows")
+        _lib.check(_lib.load().talos_batch_share(self.h, int(slot), int(n)))
+
+    def batch_move(self, moves):
+        """talos_batch_move: copies between cache slots, all at once; each of ``moves`` is
+        (source slot, destination slot, first position, positions)."""
+        m = [tuple(int(x) for x in v) for v in moves]
+        if any(len(v) != 4 or min(v) < 0 or max(v) > 0xFFFFFFFF for v in m):
+            raise ValueError("a move is (source slot, destination slot, first position, positions)")
+        _lib.check(_lib.load().talos_batch_move(self.h, (_lib.KvCopy * max(len(m), 1))(*m), len(m)))
+
     def device_bytes(self) -> int:
         n = C.c_size_t()
         _lib.check(_lib.load().talos_ctx_device_bytes(self.h, C.byref(n)))
@@ -384,6 +425,20 @@ class Model:
     def generate_batch_greedy(self, tokens, positions, steps: int) -> np.ndarray:
         """Greedy tokens of sequences 0 .. n-1 decoded together on the GPU: [steps, n]."""
         return self.ctx.generate_batch_greedy(tokens, positions, steps)
+
+    def generate_batch_sample(self, tokens, positions, u, **settings) -> np.ndarray:
+        """Drawn tokens of sequences 0 .. n-1 decoded together on the GPU: [steps, n] for
+        random numbers u [steps, n] (temperature, top_k, top_p, min_p: one value or one
+        per sequence)."""
+        return self.ctx.generate_batch_sample(tokens, positions, u, **settings)
+
+    def batch_share(self, slot: int, n: int):
+        """Make positions 0 .. n-1 of ``slot`` the prefix of every sequence (0: no more)."""
+        self.ctx.batch_share(slot, n)
+
+    def batch_move(self, moves):
+        """Copy cache rows between slots: (source, destination, first position, positions)."""
+        self.ctx.batch_move(moves)
 
     def forward_batch(self, tokens, positions) -> np.ndarray:
         """One step for sequences 0 .. n-1: token i at positions[i] in slot i;
