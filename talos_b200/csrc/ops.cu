@@ -169,6 +169,14 @@ extern "C" talos_status talos_attention_shared_dev(const talos_attention_shared_
     for (size_t x : {k.q_sn * qs, k.q_sh * qs, k.out_sn * qs, k.out_sh * qs, k.pre_st * ks, k.pre_sh * ks,
                      k.slot_ss * ks, k.slot_st * ks, k.slot_sh * ks})
         if (x % 16) return set_err(TALOS_ERR_INVALID_ARG, "a stride of %zu bytes (multiples of 16)", x);
+    {  // the output's rows must not overlap
+        const uint64_t cn = k.out_sn ? a->n : 1, ch = k.out_sh ? a->n_head : 1;
+        const bool n_outer = k.out_sn >= k.out_sh;
+        const uint64_t s0 = n_outer ? k.out_sh : k.out_sn, c0 = n_outer ? ch : cn, s1 = n_outer ? k.out_sn : k.out_sh;
+        const bool apart = (a->n == 1 || k.out_sn) && (a->n_head == 1 || k.out_sh) && (c0 == 1 || s0 >= a->head_dim) &&
+                           ((cn == 1 && ch == 1) || cn * ch == c0 || s1 >= s0 * (c0 - 1) + a->head_dim);
+        if (!apart) return set_err(TALOS_ERR_INVALID_ARG, "the output's strides make its rows overlap");
+    }
     for (const void* p : {a->q, (const void*)a->out, a->k_prefix, a->v_prefix, a->k, a->v, (const void*)work})
         if (!aligned(p, 16)) return set_err(TALOS_ERR_INVALID_ARG, "a pointer is not 16-byte aligned");
     if (!aligned(a->lens, 4) || !aligned(a->slots, 4))

@@ -38,6 +38,39 @@ def test_sample_refusals(lib):
     assert lib.talos_sample(v.ctypes.data, 4, 0.5, 1.0, 0, 1.0, 0.0, None, None) == _lib.INVALID_ARG
 
 
+def attention(lib, work=4096, work_bytes=1 << 30, **kw):
+    """A call of 3 sequences, 4 heads over 2 of 64, a prefix of 8, 5 slots of 16 rows."""
+    a = _lib.AttentionSharedArgs(
+        0, 0, 0, 3, 4, 2, 64, 8, 5, 16, 4096, 256, 64, 4096, 4096, 128, 64, 4096, 4096, 2048, 128, 64, None, 4096, 4096,
+        256, 64, 0.125)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return lib.talos_attention_shared_dev(C.byref(a), work, work_bytes, None)
+
+
+def test_attention_refusals(lib):
+    n = C.c_size_t()
+    assert lib.talos_attention_shared_work(0, 3, 4, 2, None) == _lib.INVALID_ARG
+    for args in ((0, 4, 2), (1025, 4, 2), (3, 4, 0), (3, 0, 2), (3, 5, 2), (3, 258, 2)):
+        assert lib.talos_attention_shared_work(0, *args, C.byref(n)) == _lib.INVALID_ARG, args
+    assert lib.talos_attention_shared_work(0, 3, 4, 2, C.byref(n)) == _lib.OK and n.value > 0
+    assert attention(lib, work_bytes=n.value - 1) == _lib.INVALID_ARG
+    assert lib.talos_attention_shared_dev(None, 4096, 1 << 30, None) == _lib.INVALID_ARG
+    assert attention(lib, n=0) == _lib.OK
+    for kw in (dict(q_type=30), dict(q_type=1), dict(kv_type=30), dict(kv_type=2), dict(q_type=1, kv_type=30),
+               dict(head_dim=0), dict(head_dim=132), dict(head_dim=62), dict(head_dim=60, kv_type=1),
+               dict(prefix_len=0x40000000), dict(slot_len=0x40000000)):
+        assert attention(lib, **kw) == _lib.UNSUPPORTED, kw
+    for kw in (dict(work=None), dict(work=4100), dict(q=None), dict(out=None), dict(lens=None), dict(k_prefix=None),
+               dict(v_prefix=None), dict(k=None), dict(v=None), dict(n_slots=0), dict(scale=0.0), dict(scale=float("nan")),
+               dict(scale=1e31), dict(scale=-1.0), dict(q=4100), dict(k=4104), dict(v_prefix=4100), dict(out=4100),
+               dict(lens=4097), dict(slots=4098), dict(q_stride_h=65), dict(prefix_stride_t=126), dict(slot_stride=2046),
+               dict(out_stride_n=257), dict(n_head=5), dict(n_head_kv=0), dict(n=1025),
+               dict(out_stride_h=0), dict(out_stride_n=0), dict(out_stride_h=32), dict(out_stride_n=128),
+               dict(out_stride_n=64, out_stride_h=128), dict(out_stride_n=64, out_stride_h=64)):
+        assert attention(lib, **kw) == _lib.INVALID_ARG, kw
+
+
 def move(lib, moves, n_slots=4, n_rows=8, bases=(256, 4096), **kw):
     base = (C.c_void_p * max(len(bases), 1))(*bases)
     g = _lib.KvSlots(0, len(bases), C.addressof(base), n_slots, 1, n_rows, 64 * n_rows, 64 * n_rows * n_slots, 64, 64)
@@ -73,3 +106,6 @@ def test_python_checks_without_a_gpu():
         talos_b200.sample_dev(x, torch.zeros(2))
     with pytest.raises(ValueError, match="CUDA"):
         talos_b200.kv_move_dev([torch.zeros(2, 1, 4, 4)], [0], [1], [1])
+    with pytest.raises(ValueError, match="CUDA"):
+        talos_b200.attention_shared_dev(torch.zeros(2, 2, 8), *[torch.zeros(4, 1, 8)] * 2, *[torch.zeros(2, 4, 1, 8)] * 2,
+                                        None, torch.zeros(2, dtype=torch.int32))
