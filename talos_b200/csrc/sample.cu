@@ -14,10 +14,10 @@
 // Exactness. An answer is a border between cumulative sums, so weights are
 // computed in f64 and summed as 64-bit integers in units of 2^-42: sums do not
 // depend on their order, and a weight is off by at most 2^-42 (a million weights
-// add up to less than 2^63). w = 2^-(k / 64) 2^(r / 64) with k the nearest integer
-// to 64 log2(e) (max - l) / T: a table of 64 powers and the exponential's series to
-// the fourth power (|r| <= 1/2: the fifth is below 4e-14), eleven f64 operations
-// where exp() took about a hundred instructions (64 rows of 128256: 117 -> 99 us).
+// add up to less than 2^63). w = 2^-(k / 512) 2^(r / 512) with k the nearest integer
+// to 512 log2(e) (max - l) / T: a table of 512 powers and the exponential's series to
+// the third power (|r| <= 1/2: the fourth is below 9e-15), nine f64 operations where
+// exp() took about a hundred instructions (64 rows of 128256: 117 -> 99 us).
 //
 // Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
 // shared memory, so the row is read from HBM once. No sort of the row: a
@@ -48,6 +48,7 @@ constexpr int SP_CAP = 1024;      // elements of a ranked list; two per thread
 constexpr double SP_ONE = 4398046511104.0;  // 2^42
 constexpr int SP_SLICE = 16384;  // logits of a row that one CTA keeps
 constexpr int SP_IDX_BITS = 20;
+static_assert(SP_THREADS == 512, "sp_pow's entries, one a thread");
 static_assert((1 << SP_IDX_BITS) == SAMPLE_MAX_VOCAB, "index bits");
 
 enum SpOp : int { SP_COUNT = 0, SP_WEIGH = 1, SP_GATHER_BINS = 2, SP_GATHER_KEYS = 3, SP_RANGE = 4, SP_SPLIT = 5,
@@ -73,7 +74,7 @@ struct SpSmem {
     uint32_t f_cnt, f_bin, f_at;
     u64 f_bc, f_bw;
     uint32_t keep;     // elements of the list with w >= min_p
-    double pow[64];    // sp_pow
+    double pow[512];   // sp_pow
 };
 
 __device__ __forceinline__ float sp_load(float v) { return isnan(v) ? -INFINITY : v + 0.0f; }  // -0 -> +0
@@ -87,20 +88,20 @@ __device__ __forceinline__ float sp_key_value(u64 k) {
     return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
 
-// 2^42 2^(-i / 64), i < 64: the product of 2^(-1 / 2) to 2^(-1 / 64) over i's bits.
+// 2^42 2^(-i / 512), i < 512: the product of 2^(-1 / 2) to 2^(-1 / 512) over i's bits.
 __device__ __forceinline__ double sp_pow(int i) {
-    constexpr double root[6] = {0.98922801319397548, 0.97857206208770013, 0.95760328069857365,
+    constexpr double root[9] = {0.99864711289097017, 0.99729605608547012, 0.99459942348363317,
+                                0.98922801319397548, 0.97857206208770013, 0.95760328069857365,
                                 0.91700404320467123, 0.84089641525371454, 0.70710678118654752};
     double w = SP_ONE;
 #pragma unroll
-    for (int b = 0; b < 6; ++b)
+    for (int b = 0; b < 9; ++b)
         if (i >> b & 1) w *= root[b];
     return w;
 }
 
 struct SpScale {
-    float vmax;
-    double vmax_d, c;  // c: 64 log2(e) / T
+    double vmax, c;  // c: 512 log2(e) / T
 };
 // f32 -> f64 by its bits (two integer operations where the conversion runs at a quarter
 // of their rate). Zeros and denormals become 2^-126 to 2^-125, which matters below a
@@ -109,23 +110,22 @@ __device__ __forceinline__ double sp_f64(float v) {
     const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
     return __hiloint2double((int)((b & 0x80000000u) | ((m >> 3) + (896u << 20))), (int)(m << 29));
 }
-// 2^42 w of a finite value v whose bin is below SP_NB (2^42 at the maximum, +inf included).
-__device__ __forceinline__ double sp_weight(float v, const SpScale& q, const double* pow) {
-    if (v == q.vmax) return SP_ONE;
-    const double t = (q.vmax_d - sp_f64(v)) * q.c;
+// 2^42 w of a value v whose bin is below SP_NB, plus `base` (a power of two, or 0). At the
+// maximum, +inf included, the difference is 0 and w is 2^42 exactly.
+__device__ __forceinline__ double sp_weight(float v, const SpScale& q, const double* pow, double base) {
+    const double t = (q.vmax - sp_f64(v)) * q.c;
     const double round = 6755399441055744.0;  // 1.5 2^52: the sum's low word is the nearest integer
     const double tm = t + round;
     const int k = __double2loint(tm);
-    const double r = (tm - round) - t, h = 0.010830424696249145;  // ln 2 / 64
-    const double z = r * h;
-    const double e = fma(z, fma(z, fma(z, fma(z, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
-    const double w = pow[k & 63] * e;
-    return __hiloint2double(__double2hiint(w) - ((k >> 6) << 20), __double2loint(w));  // times 2^-(k / 64)
+    const double r = (tm - round) - t;
+    constexpr double h = 0.0013538030870311431;  // ln 2 / 512
+    const double e = fma(r, fma(r, fma(r, h * h * h / 6, h * h / 2), h), 1.0);
+    const double p = pow[k & 511];
+    return fma(__hiloint2double(__double2hiint(p) - ((k >> 9) << 20), __double2loint(p)), e, base);  // 2^-(k / 512)
 }
 // To the nearest integer (w <= 2^42).
-__device__ __forceinline__ u64 sp_fixed(double w) {
-    const double x = w + 4503599627370496.0;  // 2^52
-    return (u64)__double_as_longlong(x) & 0xfffffffffffffull;
+__device__ __forceinline__ u64 sp_fixed(float v, const SpScale& q, const double* pow) {
+    return (u64)__double_as_longlong(sp_weight(v, q, pow, 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52
 }
 // Bin of value v, SP_NB for weight 0. Non-decreasing as v falls: every rounding here is monotone.
 __device__ __forceinline__ float sp_z(float v, float vmax, float scale) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     minp = minp > 0.f ? fminf(minp, 1.0f) : 0.f;  // NaN: off
     if (!(temp > 0.f)) temp = 1.f, topk = 1;
     const double inv_t = fmin(1.0 / (double)temp, 1e30);
-    if (tid < 64) s.pow[tid] = sp_pow(tid);
+    s.pow[tid] = sp_pow(tid);
 
     // the row's largest and smallest finite logit
     mx = warp_max(mx);
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         return;
     }
 
-    const SpScale q{vmax, sp_f64(vmax), inv_t * 92.332482616893656};  // 64 log2(e)
+    const SpScale q{sp_f64(vmax), inv_t * 738.65986093514925};  // 512 log2(e)
     // Bins per logit: the row's range over all bins, at most 32 nats (the smallest logit's
     // bin is below SP_NB for every rounding; an infinite or empty range leaves the 32 nats).
     // With 32 nats always, rows of 128256 with a deviation of 1.5 nats had bins of more than
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                     const int b = sp_bin(v, vmax, scale);
                     if (b < SP_NB) {
                         atomicAdd(&s.cnt[b], 1u);
-                        if (c.op == SP_WEIGH) add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
+                        if (c.op == SP_WEIGH) add_hist(b, sp_fixed(v, q, s.pow));
                     }
                 });
                 sum_hist();
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                     if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, scale) < SP_NB) {
                         const int b = (int)((k - c.k0) >> c.shift);
                         atomicAdd(&s.cnt[b], 1u);
-                        add_hist(b, sp_fixed(sp_weight(v, q, s.pow)));
+                        add_hist(b, sp_fixed(v, q, s.pow));
                     }
                 });
                 sum_hist();
@@ -397,8 +397,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                 u64 sum = 0;
                 each([&](float v, uint32_t) {
                     if (sp_bin(v, vmax, scale) < SP_NB) {
-                        const double w = sp_weight(v, q, s.pow);
-                        if (w >= min_w) sum += sp_fixed(w);
+                        if (sp_weight(v, q, s.pow, 0.0) >= min_w) sum += sp_fixed(v, q, s.pow);
                     }
                 });
 #pragma unroll
@@ -519,9 +518,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
         for (int j = 0; j < 2; ++j) {
             const int i = 2 * tid + j;
             if (i < n) {
-                const double w = sp_weight(sp_key_value(s.list[i]), q, s.pow);
-                x[j] = sp_fixed(w);
-                keep += w >= min_w ? 1u : 0u;
+                const float v = sp_key_value(s.list[i]);
+                x[j] = sp_fixed(v, q, s.pow);
+                keep += sp_weight(v, q, s.pow, 0.0) >= min_w ? 1u : 0u;
             }
         }
         l0 = x[0], l1 = x[1];
@@ -659,7 +658,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     if (tid == 0) {
         a.tokens[row] = (int32_t)(chosen & (SAMPLE_MAX_VOCAB - 1));
         if (a.probs)
-            a.probs[row] = (float)(sp_weight(sp_key_value(chosen), q, s.pow) / (double)W);
+            a.probs[row] = (float)(sp_weight(sp_key_value(chosen), q, s.pow, 0.0) / (double)W);
     }
     __syncthreads();
     if (tid < C) cluster.map_shared_rank(&s, tid)->cmd.op = SP_DONE;
