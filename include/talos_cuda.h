@@ -473,7 +473,7 @@ talos_status talos_matvec_bench(const talos_weight* const* ws, int n, const floa
  * this the first. NaN logits count as -inf; -inf is never chosen, and +inf
  * shares the whole weight with the other +inf. A row with nothing above -inf
  * gives token -1 and probability 0. u outside [0, 1) is clamped (NaN: 0).
- * Sums are exact to 2^-43 of the largest weight and do not depend on any order,
+ * Weights are exact to 2^-42 of the largest one and their sums do not depend on any order,
  * so a call gives the same tokens every time. probs (optional): the weight of
  * the token over the kept weight.
  */
@@ -527,7 +527,11 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * work: talos_attention_shared_work bytes of device memory, 16-byte aligned,
  * used by this call alone until it has run (two calls in flight, or two graphs
  * that may run at once, need one each); its contents need not be kept or set.
- * Every wait inside is bounded (2 s): rows of a CTA whose wait ran out are NaN.
+ * Every wait inside is bounded (a number of polls, seconds at most): rows of a CTA whose
+ * wait ran out are NaN. f32 accuracy: q keeps 22 bits per element (of its row's largest
+ * element), the weights 22 bits, an element of an f32 cache 22 bits or 2^-39 of the
+ * largest element among the 64 rows of its tile. 16-bit types: the weights are rounded
+ * to the type (half a step of 2^-11 or 2^-8 each) and summed as rounded, the rest is f32.
  * No reference counterpart (the reference decodes one sequence at a time).
  */
 typedef struct talos_attention_shared_args {

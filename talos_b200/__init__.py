@@ -5,6 +5,7 @@ Public API (mirrors Tsuskov/talos ``src/model`` for the CUDA backend):
     Model.forward_gpu / forward_hidden_gpu / step / step_hidden / reset / cap_context
     Model.generate_greedy / prefill
     Model.set_batch / forward_batch / prefill_slot / generate_batch_greedy  (batches)
+    Model.batch_share / batch_move / generate_batch_sample   (batches that continue one prompt, drawn tokens)
     argmax, dequant, matvec, Weight   (single-kernel entry points)
     attention_shared_dev, sample, sample_dev, kv_move_dev   (batch operators; the *_dev ones on torch tensors)
 The compute runs in libtalos_cuda.so through the C ABI of include/talos_cuda.h.

@@ -2,7 +2,7 @@
 definition in 64 bits with numpy, row by row: temperature, top-k, top-p, min-p
 and one random number per row (src/sample.rs:19-76 with min-p besides).
 
-Tokens must be equal: the kernel sums weights to 2^-43 of the largest one, the
+Tokens must be equal: the kernel sums weights to 2^-42 of the largest one, the
 oracle to f64 rounding, so both sides of a border agree unless a random number
 lies within about 1e-11 of it. Probabilities are within 4 half-steps of f32
 (the rounding of the result and of the sums behind it: 4 * 2^-24)."""
