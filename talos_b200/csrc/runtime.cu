@@ -2232,7 +2232,11 @@ static talos_status batch_generate(talos_ctx* c, int mode, const uint32_t* token
 
 extern "C" talos_status talos_generate_batch_greedy(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
                                                     size_t steps, uint32_t* tokens_out) {
-    return batch_generate(c, BM_GREEDY, tokens, pos, n, steps, nullptr, nullptr, tokens_out);
+    try {
+        return batch_generate(c, BM_GREEDY, tokens, pos, n, steps, nullptr, nullptr, tokens_out);
+    } catch (const std::bad_alloc&) {
+        return set_err(TALOS_ERR_OOM, "host memory for %zu steps", steps);
+    }
 }
 
 extern "C" talos_status talos_generate_batch_sample(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,

@@ -275,7 +275,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     // bin is below SP_NB for every rounding; an infinite or empty range leaves the 32 nats).
     // With 32 nats always, rows of 128256 with a deviation of 1.5 nats had bins of more than
     // SP_CAP and took 193,000 clocks instead of 85,000 (64 rows with top-p: 105 -> 63 us).
-    const float scale = fmaxf((float)inv_t * SP_PER_NAT, (float)(SP_NB - 1) / (vmax - vmin));
+    // (1e30: logits closer than 1e-27 to each other all lie in bin 0, where an infinite
+    // scale would leave the maximum alone.)
+    const float scale = fmaxf((float)inv_t * SP_PER_NAT, fminf((float)(SP_NB - 1) / (vmax - vmin), 1e30f));
     const double min_w = (double)minp * SP_ONE;
 
     auto zero_hist = [&]() {

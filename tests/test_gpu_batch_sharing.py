@@ -245,3 +245,16 @@ def test_refusals_leave_the_batch_as_it_was():
     first = oracle_logits(data, [77])[-1]
     assert np.max(np.abs(m.forward_batch([77, 77], [0, 0]) - first)) <= 1e-3
     m.close()
+
+
+def test_a_row_without_a_choice_ends_the_call():
+    """NaN scales in the output matrix make every logit NaN."""
+    data = tiny_model(gguf.Q8_0)
+    m = load(data, 2)
+    rows, cols = 4096, m.cfg.n_embd
+    raw = np.zeros((rows * cols // 32, 34), np.uint8)
+    raw[:, 1] = 0x7E  # f16 NaN
+    m.ctx.upload("output.weight", raw.tobytes(), gguf.Q8_0, rows, cols)
+    with pytest.raises(TalosError, match="device check"):
+        m.generate_batch_sample([1, 2], [0, 0], np.full((3, 2), 0.5))
+    m.close()

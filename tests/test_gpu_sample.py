@@ -272,3 +272,34 @@ def test_refusals():
     with pytest.raises(TalosError, match="INVALID_ARG"):
         talos_b200.sample_dev(torch.zeros(1, 50, device="cuda").expand(3, 50), u)  # rows that overlap
     assert _lib.load().talos_sample_dev(None, None) == _lib.INVALID_ARG
+
+
+@pytest.mark.parametrize("spread", [1e-45, 1e-40, 3e-37, 1e-30, 1e-20])
+@pytest.mark.parametrize("vocab", [2, 5, 1500, 40000])
+def test_logits_closer_than_any_bin(spread, vocab):
+    """Logits that differ by (almost) nothing share the weight evenly, whatever the bins.
+    (At a temperature of 1 every weight is 1 to 1e-20: the oracle's choice is exact.)"""
+    import torch
+
+    rng = np.random.default_rng(3)
+    x = (rng.integers(0, 9, (3, vocab)) * np.float64(spread)).astype(np.float32)
+    x[:, -1] = -np.inf
+    u = rng.random(3).astype(np.float32)
+    check(torch.from_numpy(x).cuda(), u)
+    check(torch.from_numpy(x).cuda(), u, p=0.4, m=0.5)
+    check(torch.from_numpy(x).cuda(), u, t=float("inf"))
+
+
+@pytest.mark.parametrize("t", [1e-3, 1e4, 1e30])
+def test_extreme_temperatures_and_ranges(t):
+    import torch
+
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((4, 3000)).astype(np.float32)
+    x[1] *= 1e30
+    x[2, ::3] = -3.4028234663852886e38
+    x[3] = np.linspace(-3e38, 3e38, 3000)
+    u = rng.random(4).astype(np.float32)
+    check(torch.from_numpy(x).cuda(), u, t=t)
+    check(torch.from_numpy(x).cuda(), u, t=t, k=700, p=0.7)
+    check(torch.from_numpy(x).cuda(), u, t=t, m=0.2)
