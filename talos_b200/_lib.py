@@ -113,10 +113,10 @@ SIGNATURES = {
     "talos_argmax": (_i, [_vp, _sz, C.POINTER(C.c_uint32)]),
     "talos_sample": (_i, [_vp, _sz, C.c_float, C.c_float, C.c_int32, C.c_float, C.c_float, C.POINTER(C.c_uint32),
                           C.POINTER(C.c_float)]),
-    "talos_sample_dev": (_i, [C.POINTER(SampleArgs), _vp]),
+    "talos_sample_dev": (_i, [_vp, _vp]),
     "talos_attention_shared_work": (_i, [_i, _u32, _u32, _u32, C.POINTER(_sz)]),
-    "talos_attention_shared_dev": (_i, [C.POINTER(AttentionSharedArgs), _vp, _sz, _vp]),
-    "talos_kv_move_dev": (_i, [C.POINTER(KvSlots), _vp, _sz, _vp]),
+    "talos_attention_shared_dev": (_i, [_vp, _vp, _sz, _vp]),
+    "talos_kv_move_dev": (_i, [_vp, _vp, _sz, _vp]),
     "talos_matvec": (_i, [_i, _i, _vp, _sz, _sz, _sz, _vp, _vp]),
     "talos_matvec_resident": (_i, [_vp, C.c_char_p, _i, _vp, _sz, _sz, _sz, _vp, _vp]),
     "talos_weight_create": (_i, [_i, _i, _vp, _sz, _sz, _sz, C.POINTER(_vp)]),

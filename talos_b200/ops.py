@@ -12,12 +12,21 @@ call, not by the package.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+from array import array
 
 import numpy as np
 
 from . import _lib
 
 _state = None
+
+# The argument structs of the C ABI (native layout), packed at once: a ctypes Structure of
+# 27 fields takes 3 us to fill, a tenth of the smallest call.
+_ATTENTION = struct.Struct("@3i7IP2N2P2N2P3N2PP2Nf0P")
+_SLOTS = struct.Struct("@2iP3I4N0P")
+_SAMPLE = struct.Struct("@2i2IPN5Pfiff2P")
+assert _ATTENTION.size == C.sizeof(_lib.AttentionSharedArgs) and _SAMPLE.size == C.sizeof(_lib.SampleArgs)
 
 
 class _Torch:
@@ -30,6 +39,9 @@ class _Torch:
         self.tag = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
         self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
         self.lib = _lib.load()
+        # the handle of the current stream; through the Stream object it takes 2 us
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.stream = raw or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _torch() -> _Torch:
@@ -40,18 +52,26 @@ def _torch() -> _Torch:
 
 
 def _device(t, name: str) -> int:
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} is on {t.device}, not on a CUDA device")
-    return t.device.index
+    return dev
 
 
 def _stream(T: _Torch, dev: int, stream) -> int:
-    return T.torch.cuda.current_stream(dev).cuda_stream if stream is None else int(stream)
+    return T.stream(dev) if stream is None else int(stream)
+
+
+def _pack(s: struct.Struct, *values) -> bytes:
+    try:
+        return s.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"a number that its argument cannot hold: {e}") from None
 
 
 def _vector(T: _Torch, t, name: str, n: int, dtype, dev: int) -> int:
     """The pointer of a contiguous [n] tensor of dtype on device dev."""
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device.index != dev or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [{n}] {dtype} tensor on cuda:{dev}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
@@ -81,16 +101,20 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
     if k.shape[3] != hd or k_prefix.shape[1] != n_kv or k_prefix.shape[2] != hd:
         raise ValueError(f"q {tuple(q.shape)}, prefix {tuple(k_prefix.shape)} and cache {tuple(k.shape)} do not match")
     kt, qs, ps, cs = k.dtype, q.stride(), k_prefix.stride(), k.stride()
-    for name, t, like, st in (("v_prefix", v_prefix, k_prefix, ps), ("v", v, k, cs), ("k_prefix", k_prefix, k_prefix, ps)):
-        if t.shape != like.shape or t.dtype != kt or t.device.index != dev or (t.stride() != st and t.numel()):
-            raise ValueError(f"{name} must be {kt} on cuda:{dev} with the shape and strides of its keys, got "
-                             f"{tuple(t.shape)} {t.dtype} {t.stride()} on {t.device}")
-    if k.device.index != dev or (hd > 1 and (qs[2] != 1 or cs[3] != 1 or (prefix and ps[2] != 1))):
+    if not (v.shape == k.shape and v_prefix.shape == k_prefix.shape and v.dtype is kt and k_prefix.dtype is kt
+            and v_prefix.dtype is kt and v.get_device() == dev == k_prefix.get_device() == v_prefix.get_device()
+            and (v.stride() == cs or not v.numel()) and (v_prefix.stride() == ps or not prefix)):
+        for name, t, like in (("v_prefix", v_prefix, k_prefix), ("v", v, k), ("k_prefix", k_prefix, k_prefix)):
+            if (t.shape != like.shape or t.dtype != kt or t.get_device() != dev
+                    or (t.stride() != like.stride() and t.numel())):
+                raise ValueError(f"{name} must be {kt} on cuda:{dev} with the shape and strides of its keys, got "
+                                 f"{tuple(t.shape)} {t.dtype} {t.stride()} on {t.device}")
+    if k.get_device() != dev or (hd > 1 and (qs[2] != 1 or cs[3] != 1 or (prefix and ps[2] != 1))):
         raise ValueError("q and the caches must be on one device with a contiguous last dimension")
     if q.dtype not in T.tag or kt not in T.tag:
         raise ValueError(f"queries of {q.dtype} with a cache of {kt}")
     if out is None:
-        out = T.torch.empty((n, n_head, hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, n_head, hd))
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (hd > 1 and out.stride(2) != 1):
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device} with a contiguous last dimension")
     if n == 0:
@@ -101,14 +125,14 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
         need = C.c_size_t()
         _lib.check(T.lib.talos_attention_shared_work(dev, n, n_head, n_kv, C.byref(need)))
         size = _work_bytes[key] = need.value
-    work = T.torch.empty(size, dtype=T.u8, device=q.device)
+    work = q.new_empty(size, dtype=T.u8)
     os_ = out.stride()
-    a = _lib.AttentionSharedArgs(
-        dev, T.tag[q.dtype], T.tag[kt], n, n_head, n_kv, hd, prefix, n_slots, rows, q.data_ptr(), qs[0], qs[1],
+    a = _pack(
+        _ATTENTION, dev, T.tag[q.dtype], T.tag[kt], n, n_head, n_kv, hd, prefix, n_slots, rows, q.data_ptr(), qs[0], qs[1],
         k_prefix.data_ptr(), v_prefix.data_ptr(), ps[0], ps[1], k.data_ptr(), v.data_ptr(), cs[0], cs[1], cs[2],
-        None if slots is None else _vector(T, slots, "slots", n, T.i32, dev), _vector(T, lens, "lens", n, T.i32, dev),
+        0 if slots is None else _vector(T, slots, "slots", n, T.i32, dev), _vector(T, lens, "lens", n, T.i32, dev),
         out.data_ptr(), os_[0], os_[1], hd ** -0.5 if scale is None else scale)
-    _lib.check(T.lib.talos_attention_shared_dev(C.byref(a), work.data_ptr(), size, _stream(T, dev, stream)))
+    _lib.check(T.lib.talos_attention_shared_dev(a, work.data_ptr(), size, _stream(T, dev, stream)))
     return out
 
 
@@ -131,30 +155,23 @@ def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
         raise ValueError(f"logits must be [n, vocab] with neighbouring logits of a row adjacent, got "
                          f"{tuple(logits.shape)} with strides {logits.stride()}")
     n, vocab = logits.shape
-    a = _lib.SampleArgs(dev, tag, n, vocab, logits.data_ptr(), logits.stride(0), _vector(T, u, "u", n, T.f32, dev))
-    if isinstance(temperature, (int, float)):
-        a.temperature = temperature
-    else:
-        a.temperature_dev = _vector(T, temperature, "temperature", n, T.f32, dev)
-    if isinstance(top_k, int):
-        a.top_k = top_k
-    else:
-        a.top_k_dev = _vector(T, top_k, "top_k", n, T.i32, dev)
-    if isinstance(top_p, (int, float)):
-        a.top_p = top_p
-    else:
-        a.top_p_dev = _vector(T, top_p, "top_p", n, T.f32, dev)
-    if isinstance(min_p, (int, float)):
-        a.min_p = min_p
-    else:
-        a.min_p_dev = _vector(T, min_p, "min_p", n, T.f32, dev)
     if tokens is None:
-        tokens = T.torch.empty(n, dtype=T.i32, device=logits.device)
+        tokens = logits.new_empty(n, dtype=T.i32)
     if probs is None:
-        probs = T.torch.empty(n, dtype=T.f32, device=logits.device)
-    a.tokens = _vector(T, tokens, "tokens", n, T.i32, dev)
-    a.probs = _vector(T, probs, "probs", n, T.f32, dev)
-    _lib.check(T.lib.talos_sample_dev(C.byref(a), _stream(T, dev, stream)))
+        probs = logits.new_empty(n, dtype=T.f32)
+    td = kd = pd = md = 0
+    if not isinstance(temperature, (int, float)):
+        td, temperature = _vector(T, temperature, "temperature", n, T.f32, dev), 0.0
+    if not isinstance(top_k, int):
+        kd, top_k = _vector(T, top_k, "top_k", n, T.i32, dev), 0
+    if not isinstance(top_p, (int, float)):
+        pd, top_p = _vector(T, top_p, "top_p", n, T.f32, dev), 0.0
+    if not isinstance(min_p, (int, float)):
+        md, min_p = _vector(T, min_p, "min_p", n, T.f32, dev), 0.0
+    a = _pack(_SAMPLE, dev, tag, n, vocab, logits.data_ptr(), logits.stride(0), _vector(T, u, "u", n, T.f32, dev), td,
+              kd, pd, md, temperature, top_k, top_p, min_p, _vector(T, tokens, "tokens", n, T.i32, dev),
+              _vector(T, probs, "probs", n, T.f32, dev))
+    _lib.check(T.lib.talos_sample_dev(a, _stream(T, dev, stream)))
     return tokens, probs
 
 
@@ -186,21 +203,21 @@ def kv_move_dev(caches, src, dst, lens, starts=None, stream=None) -> None:
         if size > 1 and step != width:
             raise ValueError(f"the dimensions of a row must be contiguous, got {tuple(shape)} with strides {strides}")
         width *= size
-    base = (C.c_void_p * len(caches))()
-    for i, c in enumerate(caches):
-        if c.shape != shape or c.stride() != strides or c.dtype != dtype or not c.is_cuda or c.device.index != dev:
+    base = array("Q")
+    i = 0
+    for c in caches:
+        if c.shape != shape or c.stride() != strides or c.dtype is not dtype or c.get_device() != dev:
             raise ValueError(f"caches[{i}] differs from caches[0] in shape, strides, dtype or device")
-        base[i] = c.data_ptr()
+        base.append(c.data_ptr())
+        i += 1
     n = len(src)
     if len(dst) != n or len(lens) != n or (starts is not None and len(starts) != n):
         raise ValueError("src, dst, lens and starts differ in length")
-    m = (C.c_uint32 * (4 * n))()
-    m[0::4], m[1::4], m[3::4] = src, dst, lens
-    if starts is not None:
-        m[2::4] = starts
-    if n and (min(src) < 0 or min(dst) < 0 or min(lens) < 0 or (starts is not None and min(starts) < 0)):
-        raise ValueError("negative slot, start or length")
+    try:
+        m = array("I", [x for move in zip(src, dst, (0,) * n if starts is None else starts, lens) for x in move])
+    except OverflowError:
+        raise ValueError("negative slot, start or length") from None
     es = first.element_size()
-    g = _lib.KvSlots(dev, len(caches), C.addressof(base), shape[0], shape[1], shape[2], strides[0] * es,
-                     strides[1] * es, strides[2] * es, width * es)
-    _lib.check(T.lib.talos_kv_move_dev(C.byref(g), m, n, _stream(T, dev, stream)))
+    g = _pack(_SLOTS, dev, len(base), base.buffer_info()[0], shape[0], shape[1], shape[2], strides[0] * es,
+              strides[1] * es, strides[2] * es, width * es)
+    _lib.check(T.lib.talos_kv_move_dev(g, m.buffer_info()[0], n, _stream(T, dev, stream)))

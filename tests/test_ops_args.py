@@ -109,3 +109,13 @@ def test_python_checks_without_a_gpu():
     with pytest.raises(ValueError, match="CUDA"):
         talos_b200.attention_shared_dev(torch.zeros(2, 2, 8), *[torch.zeros(4, 1, 8)] * 2, *[torch.zeros(2, 4, 1, 8)] * 2,
                                         None, torch.zeros(2, dtype=torch.int32))
+
+
+def test_packed_arguments_have_the_structs_layout():
+    from talos_b200 import ops
+
+    for packed, struct_ in ((ops._ATTENTION, _lib.AttentionSharedArgs), (ops._SAMPLE, _lib.SampleArgs),
+                            (ops._SLOTS, _lib.KvSlots)):
+        fields = [name for name, _ in struct_._fields_]
+        got = struct_.from_buffer_copy(packed.pack(*range(1, len(fields) + 1)))
+        assert [int(getattr(got, name)) for name in fields] == list(range(1, len(fields) + 1))
