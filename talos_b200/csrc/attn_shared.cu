@@ -364,17 +364,19 @@ struct AsConv {
     static constexpr int QC = DP / 4, QR = 32 / QC;  // float4 chunks of a row, rows per warp step
     static constexpr int NI = (KT / QR + NW - 1) / NW, HALF = AS_SLOT / (DP * 4);
     float4 v[NI];
-    // the warp's largest |element| as bits; rows behind the last key (the next ones of
-    // the slot, or stale) become zeros
-    __device__ __forceinline__ uint32_t load(const uint8_t* raw0, const uint8_t* raw1, int w, int lane, int valid) {
+    // rows behind the last key (the next ones of the slot, or stale) become zeros
+    __device__ __forceinline__ void load(const uint8_t* raw0, const uint8_t* raw1, int w, int lane, int valid) {
         const int ch = lane % QC, sub = lane / QC;
-        float mx = 0.f;
 #pragma unroll
         for (int q = 0; q < NI; ++q) {
             const int r = (w + NW * q) * QR + sub;
             v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < valid) v[q] = *(const float4*)((r < HALF ? raw0 : raw1) + r % HALF * (QC * 16) + ch * 16);
         }
+    }
+    // the warp's largest |element| as bits
+    __device__ __forceinline__ uint32_t largest() {
+        float mx = 0.f;
 #pragma unroll
         for (int q = 0; q < NI; ++q) {
             mx = as_max3(mx, fabsf(v[q].x), fabsf(v[q].y));
@@ -767,17 +769,21 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 }
                 w.tile(m, ntp, prefix, KT);
 #pragma unroll 1
-                for (int h = 0; h < 4; ++h) {  // K, then V
-                    if ((h & 1) * C::HALF >= w.valid) continue;
+                for (int h = 0; h < 4; ++h) {  // K, then V: one or two slots each, both on the first one's barrier
+                    const bool two = C::HALF < w.valid;
+                    if ((h & 1) && !two) continue;
+                    const uint32_t bar_st = (h & 1) ? (st == 0 ? C::NR : st) - 1 : st;
                     slot_free();
                     if (ok) {
-                        mbar_expect_tx(&m->r_full[st], AS_SLOT);
+                        if (h & 1) mbar_arrive(&m->r_full[st]);  // (its phases count the laps)
+                        else mbar_expect_tx(&m->r_full[st], two ? 2 * AS_SLOT : AS_SLOT);
+                        uint64_t* bar = &m->r_full[bar_st];
                         const uint32_t dst = smem_u32(sR) + st * AS_SLOT;
                         const int row = w.key + (h & 1) * C::HALF;
-                        if (w.off < ntp) as_tma3(dst, h < 2 ? &maps.kp : &maps.vp, 0, w.kvh, row, &m->r_full[st]);
+                        if (w.off < ntp) as_tma3(dst, h < 2 ? &maps.kp : &maps.vp, 0, w.kvh, row, bar);
                         else
                             as_tma4(dst, h < 2 ? &maps.k : &maps.v, 0, w.kvh, row + a.slot_row0 * prefix, m->slot[w.i],
-                                    &m->r_full[st]);
+                                    bar);
                     }
                     next();
                 }
@@ -805,11 +811,12 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_wait(m, &m->r_full[st], par, ok);
                 ring_step(st, par, 1);
                 const uint32_t s1 = st;
-                if (two) {
-                    as_wait(m, &m->r_full[st], par, ok);
-                    ring_step(st, par, 1);
-                }
-                const uint32_t own = cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
+                if (two) ring_step(st, par, 1);
+                cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
+                // (a wait takes 200 clocks also when nothing is to be waited for: beside the loads)
+                if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
+                if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+                const uint32_t own = cv.largest();
                 if (lane == 0) m->cmax[is_v][w] = own;
                 // (the slots are free once every warp's values have arrived, which the reductions
                 // waited for: an arrival may overtake loads that are still under way)
@@ -821,8 +828,6 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                     if (two) as_arrive(&m->r_empty[s1], ok);
                     (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
                 }
-                if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
-                if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
                 cv.store(is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK, w, lane, e);
                 if (lane == 0) as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
             }
