@@ -67,7 +67,7 @@ namespace talos {
 
 constexpr int AS_ROWS = 128;   // rows per tile = TMEM lanes
 constexpr int AS_SOFT = 8;     // softmax warps
-constexpr int AS_CONV = 9;     // f32: converter warps
+constexpr int AS_CONV = 4;     // f32: converter warps of K, and of V
 constexpr int AS_SLOT = 16 * 1024;  // f32: one slot of the ring
 constexpr int AS_MISC = 12 * 1024;
 constexpr int AS_SMEM = 227 * 1024;
@@ -118,7 +118,7 @@ struct AsMisc {
     float mx[2][2][AS_ROWS];  // [tile parity][half] row maxima
     float lx[2][AS_ROWS];
     float ksc[4], vsc[4];     // f32 cache: 2^exponent of a tile's keys, values
-    uint32_t cmax[2][AS_CONV];  // f32 cache: largest |element| of each converter warp (K, V)
+    uint32_t cmax[2][2][AS_CONV];  // f32 cache: largest |element| of each converter warp (K, V; tile parity)
 };
 static_assert(sizeof(AsMisc) <= AS_MISC, "misc area");
 
@@ -356,45 +356,44 @@ __device__ __forceinline__ int as_suffix_tiles(const AttnSharedArgs& a, int seq0
     return t;
 }
 
-// f32 tiles: NW warps take the rows of a raw tile (two ring slots of HALF rows, or
-// one) into registers, find the largest element, and store the tile scaled by
-// 2^(14 - e) as f16 hi and lo operand tiles.
+// f32 tiles: NW warps read the rows of a raw tile (two ring slots of HALF rows, or
+// one) for the largest element, then again and store the tile scaled by 2^(14 - e) as
+// f16 hi and lo operand tiles. Rows behind the last key (the next ones of the slot, or
+// stale) become zeros.
 template <int DP, int KT, int NW>
 struct AsConv {
     static constexpr int QC = DP / 4, QR = 32 / QC;  // float4 chunks of a row, rows per warp step
-    static constexpr int NI = (KT / QR + NW - 1) / NW, HALF = AS_SLOT / (DP * 4);
-    float4 v[NI];
-    // rows behind the last key (the next ones of the slot, or stale) become zeros
-    __device__ __forceinline__ void load(const uint8_t* raw0, const uint8_t* raw1, int w, int lane, int valid) {
-        const int ch = lane % QC, sub = lane / QC;
-#pragma unroll
-        for (int q = 0; q < NI; ++q) {
-            const int r = (w + NW * q) * QR + sub;
-            v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < valid) v[q] = *(const float4*)((r < HALF ? raw0 : raw1) + r % HALF * (QC * 16) + ch * 16);
-        }
+    static constexpr int NI = KT / QR / NW, HALF = AS_SLOT / (DP * 4);
+    static_assert(NI * QR * NW == KT, "rows of a warp");
+    static __device__ __forceinline__ float4 chunk(const uint8_t* raw0, const uint8_t* raw1, int r, int ch, int valid) {
+        if (r >= valid) return make_float4(0.f, 0.f, 0.f, 0.f);
+        return *(const float4*)((r < HALF ? raw0 : raw1) + r % HALF * (QC * 16) + ch * 16);
     }
     // the warp's largest |element| as bits
-    __device__ __forceinline__ uint32_t largest() {
+    static __device__ __forceinline__ uint32_t largest(const uint8_t* raw0, const uint8_t* raw1, int w, int lane,
+                                                       int valid) {
+        const int ch = lane % QC, sub = lane / QC;
         float mx = 0.f;
-#pragma unroll
+#pragma unroll 8
         for (int q = 0; q < NI; ++q) {
-            mx = as_max3(mx, fabsf(v[q].x), fabsf(v[q].y));
-            mx = as_max3(mx, fabsf(v[q].z), fabsf(v[q].w));
+            const float4 v = chunk(raw0, raw1, (w + NW * q) * QR + sub, ch, valid);
+            mx = as_max3(mx, fabsf(v.x), fabsf(v.y));
+            mx = as_max3(mx, fabsf(v.z), fabsf(v.w));
         }
         return __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
     }
-    __device__ __forceinline__ void store(uint8_t* tile, int w, int lane, int e) {
+    static __device__ __forceinline__ void store(const uint8_t* raw0, const uint8_t* raw1, uint8_t* tile, int w, int lane,
+                                                 int valid, int e) {
         const int ch = lane % QC, sub = lane / QC;
         const float f = as_pow2(14 - e);
         const f2 ff = as_f2(f, f);
         uint8_t* dst0 = tile + (ch / 16) * (KT * 128) + (ch & 1) * 8;
-#pragma unroll
+#pragma unroll 4
         for (int q = 0; q < NI; ++q) {
             const int r = (w + NW * q) * QR + sub;
-            if (NI * NW * QR > KT && r >= KT) continue;
+            const float4 v = chunk(raw0, raw1, r, ch, valid);
             float x, y, z, u;
-            as_un2(as_mul2(as_f2(v[q].x, v[q].y), ff), x, y), as_un2(as_mul2(as_f2(v[q].z, v[q].w), ff), z, u);
+            as_un2(as_mul2(as_f2(v.x, v.y), ff), x, y), as_un2(as_mul2(as_f2(v.z, v.w), ff), z, u);
             uint2 hi, lo;
             as_split_cut(x, y, hi.x, lo.x);
             as_split_cut(z, u, hi.y, lo.y);
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
             mbar_init(&m->r_full[i], 1);
-            mbar_init(&m->r_empty[i], 1);
+            mbar_init(&m->r_empty[i], AS_CONV);
         }
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -725,7 +724,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_settle(ok);
         }
         __syncwarp();
-    } else if (C::KF32 && warp == 8 + AS_CONV) {
+    } else if (C::KF32 && warp == 17) {
         // ---------------------------------------------------- f32: the ring's copies
         if (as_elect()) {
             uint32_t st = 0, par = 0;            // the next slot, the parity of its data
@@ -793,11 +792,14 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         }
         __syncwarp();
     } else if constexpr (C::KF32) {
-        // ---------------------------------------------------- ring -> operand tiles
-        const int w = warp - 8;
+        // ---------------------------------------------------- ring -> operand tiles: K by the first
+        // four warps, V by the next (warp 16 only fills up the warpgroup)
+        if (warp < 8 + 2 * AS_CONV) {
+        const int w = warp & 3;
+        const bool is_v = warp >= 8 + AS_CONV;
         int cur = -1, j = 0;
         uint32_t st = 0, par = 0;
-        AsConv<DP, KT, AS_CONV> cv;
+        using cv = AsConv<DP, KT, AS_CONV>;
         AsWalk wk;
         wk.start(t0, tpg);
         for (int t = t0; t < t1; ++t, ++j) {
@@ -805,33 +807,32 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             const int valid = wk.valid;
             const bool two = C::HALF < valid;
             if (wk.kvh != cur) cur = wk.kvh, ring_step(st, par, C::QB);  // the queries' slots: the softmax warps'
-#pragma unroll 1
-            for (int is_v = 0; is_v < 2; ++is_v) {
-                const uint32_t s0 = st;
-                as_wait(m, &m->r_full[st], par, ok);
-                ring_step(st, par, 1);
-                const uint32_t s1 = st;
-                if (two) ring_step(st, par, 1);
-                cv.load(sR + s0 * AS_SLOT, sR + s1 * AS_SLOT, w, lane, valid);
-                // (a wait takes 200 clocks also when nothing is to be waited for: beside the loads)
-                if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
-                if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
-                const uint32_t own = cv.largest();
-                if (lane == 0) m->cmax[is_v][w] = own;
-                // (the slots are free once every warp's values have arrived, which the reductions
-                // waited for: an arrival may overtake loads that are still under way)
-                asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
-                const uint32_t all = __reduce_max_sync(0xffffffffu, m->cmax[is_v][lane < AS_CONV ? lane : 0]);
-                const int e = as_exponent(all);
-                if (w == 0 && lane == 0) {
-                    as_arrive(&m->r_empty[s0], ok);
-                    if (two) as_arrive(&m->r_empty[s1], ok);
-                    (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
-                }
-                cv.store(is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK, w, lane, e);
-                if (lane == 0) as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
+            if (is_v) ring_step(st, par, two ? 2 : 1);                   // the keys'
+            const uint32_t s0 = st;
+            as_wait(m, &m->r_full[st], par, ok);
+            ring_step(st, par, 1);
+            const uint32_t s1 = st;
+            if (two) ring_step(st, par, 1);
+            if (!is_v) ring_step(st, par, two ? 2 : 1);  // the values'
+            const uint8_t *raw0 = sR + s0 * AS_SLOT, *raw1 = sR + s1 * AS_SLOT;
+            const uint32_t own = cv::largest(raw0, raw1, w, lane, valid);
+            if (lane == 0) m->cmax[is_v][j & 1][w] = own;
+            if (is_v) asm volatile("bar.sync 6, %0;" ::"n"(AS_CONV * 32) : "memory");
+            else asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
+            const uint32_t all = __reduce_max_sync(0xffffffffu, m->cmax[is_v][j & 1][lane & 3]);
+            const int e = as_exponent(all);
+            if (w == 0 && lane == 0) (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
+            if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
+            if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+            cv::store(raw0, raw1, is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK, w, lane, valid, e);
+            // (every value read has been stored: nothing of the slots is under way)
+            if (lane == 0) {
+                as_arrive(is_v ? &m->v_full[j & 1] : &m->k_full[0], ok);
+                as_arrive(&m->r_empty[s0], ok);
+                if (two) as_arrive(&m->r_empty[s1], ok);
             }
             wk.next(tpg);
+        }
         }
     }
     } else {
