@@ -43,15 +43,21 @@
 //    queries, warp 9 those of the V tiles, straight into the swizzled operand tiles
 //    (separate, so that K runs ahead of V).
 //  * f32 cache, 20 warps: warp 17 fills a ring of 16 KB slots by TMA (the queries of a
-//    kv head, then half tiles, or whole ones of heads up to 64); warps 8-16 scale and
-//    split the tiles into the operand tiles.
+//    kv head, then half tiles, or whole ones of heads up to 64); warps 8-11 scale and
+//    split the K tiles into the operand tiles, warps 12-15 the V tiles (side by side:
+//    a tile takes either about 4,500 clocks, most of them latencies).
 //  * the last two warps issue the MMAs: the last one (which allocates TMEM) S = Q K^T,
 //    a tile ahead of the other's O = P V, so that the softmax of one tile runs beside
 //    the products of its neighbours. Tiles that end early take fewer of both. The
 //    copies bring along the rows behind a suffix's last key, which may hold anything:
 //    the PV warp clears those V rows that its product reads.
 // Bound: HBM (the keys once) up to one row tile; above, the exponentials and the
-// tensor cores.
+// tensor cores. Measured: 64 sequences, 64 / 8 heads of 128, bf16, 32768 shared and up to
+// 1024 own positions 148-153 us, 0.47 PFLOP/s (2,300 clocks a dense tile,
+// where its products take 1,024); 32 sequences, f32 queries and f16 cache, 8192 and up
+// to 512, 46 us, 1.5 TB/s of keys once (suffix tiles: the latencies from S to O);
+// 32 sequences, 32 / 8 heads, f32, 1024 and up to 256, 34 us (the f32 tiles'
+// conversion).
 //
 // Every wait is bounded; on expiry a CTA flag makes all roles run on without
 // waiting or multiplying, and the rows come out as NaN.
@@ -388,7 +394,7 @@ struct AsConv {
         const float f = as_pow2(14 - e);
         const f2 ff = as_f2(f, f);
         uint8_t* dst0 = tile + (ch / 16) * (KT * 128) + (ch & 1) * 8;
-#pragma unroll 4
+#pragma unroll 8
         for (int q = 0; q < NI; ++q) {
             const int r = (w + NW * q) * QR + sub;
             const float4 v = chunk(raw0, raw1, r, ch, valid);
