@@ -233,7 +233,8 @@ class Context:
                               ("min_p", min_p, float)):
             v = np.broadcast_to(np.asarray(v), (n,))
             for i in range(n):
-                setattr(set_[i], name, kind(v[i]))
+                x = kind(v[i])
+                setattr(set_[i], name, min(max(x, -1), 0x7FFFFFFF) if kind is int else x)
         out = np.empty((max(steps, 1), n), np.uint32)
         _lib.check(_lib.load().talos_generate_batch_sample(
             self.h, t.ctypes.data_as(C.POINTER(C.c_uint32)), p.ctypes.data_as(C.POINTER(C.c_size_t)), n, steps, set_,

@@ -153,3 +153,12 @@ def test_no_moves():
     cs = caches((2, 1, 4, 4), "float32")
     talos_b200.kv_move_dev(cs, [], [], [])
     talos_b200.kv_move_dev(cs, [1], [1], [4])
+
+
+def test_long_runs_of_several_chains():
+    """Chains long enough that a thread takes several offsets, with rows that end inside a
+    block's run; then the same arrays with an exchange and a fork."""
+    cs = caches((9, 8, 1024, 1024), "float32")
+    run(cs, [1, 2, 3, 6, 7], [0, 1, 2, 5, 6], [1024, 1003, 700, 1021, 977])
+    run(cs, [3, 4, 8, 7], [2, 3, 6, 5], [1000, 1024, 1, 513], [24, 0, 1023, 11])
+    run(cs, [0, 1, 4, 4], [1, 0, 7, 8], [1024, 1024, 301, 1024])

@@ -303,3 +303,15 @@ def test_extreme_temperatures_and_ranges(t):
     check(torch.from_numpy(x).cuda(), u, t=t)
     check(torch.from_numpy(x).cuda(), u, t=t, k=700, p=0.7)
     check(torch.from_numpy(x).cuda(), u, t=t, m=0.2)
+
+
+@pytest.mark.parametrize("settings", [SETTINGS[0], SETTINGS[2], SETTINGS[3], SETTINGS[8], SETTINGS[11]])
+@pytest.mark.parametrize("dtype,vocab,pad", [("float32", 100003, 1), ("float32", 100000, 0), ("float16", 100003, 5),
+                                             ("bfloat16", 90005, 0)])
+def test_slices_that_are_read_again(settings, dtype, vocab, pad):
+    """Rows enough that each takes fewer CTAs than would keep it in shared memory, with and
+    without 16-byte loads, and slices that end inside a load."""
+    import torch
+
+    lg, rng = rows(44, vocab, 7, getattr(torch, dtype), pad)
+    check(lg, rng.random(44).astype(np.float32), *settings)
