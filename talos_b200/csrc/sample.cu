@@ -19,8 +19,8 @@
 // the third power (|r| <= 1/2: the fourth is below 9e-15), nine f64 operations where
 // exp() took about a hundred instructions (64 rows of 128256: 117 -> 99 us).
 //
-// Bound: instructions (about 50 a logit for the exact weight), then the chain of
-// phases. 64 rows of 128256 f32: plain temperature 48 us (0.69 TB/s), top-p 61, top-k
+// Bound: the weighing pass (about 50 instructions a logit for the exact weight), then
+// the chain of phases; over the kernel the issue slots are 42 % busy. 64 rows of 128256 f32: plain temperature 48 us (0.69 TB/s), top-p 61, top-k
 // 35; 32 rows of 32000 with top-p 27 us; one row of 32000 14 us.
 //
 // Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
