@@ -374,3 +374,30 @@ def test_refusals():
     with pytest.raises(TalosError, match="INVALID_ARG"):
         talos_b200.attention_shared_dev(odd, *a[1:])
     assert _lib.load().talos_attention_shared_dev(None, None, 0, None) == _lib.INVALID_ARG
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n,heads,kvh,hd,prefix,rows", [(1024, 32, 1, 64, 100, 5), (160, 128, 1, 16, 300, 3),
+                                                        (1024, 2, 2, 128, 65, 9), (152, 200, 2, 32, 0, 70)])
+def test_more_row_tiles_than_sms(types, n, heads, kvh, hd, prefix, rows):
+    check(make(n, heads, kvh, hd, prefix, rows, types, seed=n + hd))
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, each with its own workspace, give what each gives alone."""
+    import torch
+
+    a = make(32, 32, 8, 128, 1500, 200, ("float32", "float32"), seed=1)
+    b = make(48, 32, 8, 128, 900, 300, ("bfloat16", "bfloat16"), seed=2)
+    wa, wb = check(a), check(b)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        with torch.cuda.stream(sa):
+            outs.append((talos_b200.attention_shared_dev(*a), wa))
+        with torch.cuda.stream(sb):
+            outs.append((talos_b200.attention_shared_dev(*b), wb))
+    torch.cuda.synchronize()
+    for got, want in outs:
+        assert torch.equal(got, want)
