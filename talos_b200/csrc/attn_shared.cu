@@ -22,7 +22,10 @@
 // in 16 bits as the A operand. The softmax keeps a running maximum m, rounded up
 // to an integer (base 2), so every rescaling is by an exact power of two. For f32
 // outputs O is added up in registers (the tensor core only sums one tile: its
-// accumulation truncates); for 16-bit outputs it stays in tensor memory.
+// accumulation truncates); for 16-bit outputs it stays in tensor memory for runs of
+// AS_RUN prefix tiles. A step of 16 keys was seen to lose 2 to 3 units in the last
+// place of the sum, always towards zero: with one run over 2,048 tiles the output was
+// 1.5e-3 to 2e-3 too small; a run of 16 loses about 1.5e-5 (half a step of f16 is 2.4e-4).
 //
 // Precision. f16 / bf16 queries: one product each, P rounded to 16 bits (half a
 // step of 2^-11 / 2^-8 relative per weight, averaged by the sum; the row's sum is that
@@ -77,6 +80,7 @@ constexpr int AS_CONV = 4;     // f32: converter warps of K, and of V
 constexpr int AS_SLOT = 16 * 1024;  // f32: one slot of the ring
 constexpr int AS_MISC = 12 * 1024;
 constexpr int AS_SMEM = 227 * 1024;
+constexpr int AS_RUN = 16;  // 16-bit outputs: prefix tiles added up in tensor memory
 constexpr float AS_LOG2E = 1.4426950408889634f;
 
 // MODE: types of (q, cache): 0 (f32, f32), 1 (f32, f16), 2 (f16, f16), 3 (bf16, bf16)
@@ -96,8 +100,9 @@ struct AsCfg {
     static constexpr int NR = KF32 ? 7 : 0;
     static constexpr int QB = Q_BYTES / AS_SLOT;     // f32: slots of the queries
     // 16-bit outputs: the prefix's O is added up in tensor memory, in O buffer 0. The
-    // rows' warps take it from there before their suffix tiles, whose products go to
-    // buffers 1, 0, 1, ... and are added in registers: no other row meets their values
+    // rows' warps add it to their registers after every AS_RUN tiles and before their
+    // suffix tiles, whose products go to buffers 1, 0, 1, ... and are added in registers
+    // too: no other row meets their values
     static constexpr bool ACC = !QF32;
     static constexpr int Q_OWN = KF32 ? 0 : Q_BYTES;  // (f32: in the ring)
     static constexpr int FIT = (AS_SMEM - AS_MISC - Q_OWN) / KPLANE;  // 16-bit: operand tiles that fit
@@ -639,7 +644,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const bool lead = as_elect();
         const uint32_t idesc = as_idesc((a.hd + 15) / 16 * 16, C::BF, true);
         const uint64_t dv0 = as_desc(smem_u32(sV), KT * 128);
-        int j = 0, cur = -1, nsuf = 0, ntaken = 0;  // ACC: suffix tiles of the segment, hand-overs before it
+        int j = 0, cur = -1, seg_t0 = t0, nsuf = 0, ntaken = 0;  // ACC: suffix tiles of the segment, hand-overs before it
         uint32_t sv = 0, pv = 0;
         AsWalk w;
         w.start(t0, tpg);
@@ -647,6 +652,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             const uint32_t bf = j & 1, par = (j >> 1) & 1;
             const bool pre = w.off < ntp, pre0 = w.kvh != cur;
             cur = w.kvh;
+            if (pre0) seg_t0 = t;
             w.tile(m, ntp, prefix, KT);
             const int valid = w.valid, ksteps = (valid + 15) / 16;
             as_wait(m, &m->v_full[sv], pv, ok);
@@ -676,7 +682,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_tc_after();
             if (lead && ok) {
                 const uint32_t d = tmem + C::O_COL + (C::ACC ? (pre ? 0 : (nsuf & 1) ^ 1) : C::NOB == 2 ? bf : 0) * DP, p = tmem + bf * C::S_COLS;
-                const uint32_t keep = C::ACC && pre && !pre0 ? 1u : 0u;
+                const uint32_t keep = C::ACC && pre && (t - seg_t0) % AS_RUN ? 1u : 0u;
                 const uint64_t v = dv0 + (uint64_t)(sv * (C::NK * C::KPLANE >> 4));
                 // the small terms first
 #pragma unroll
@@ -904,9 +910,11 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_arrive(&m->q_empty, ok);
             }
         };
-        // ACC: the prefix's O (buffer 0) times c
+        // ACC: the prefix's O (registers and buffer 0) times c
         auto rescale = [&](float c) {
             const f2 c2 = as_f2(c, c);
+#pragma unroll
+            for (int k = 0; k < HD / 2; ++k) o[k] = as_mul2(o[k], c2);
 #pragma unroll 1
             for (int k = 0; k < HD; k += 32) {
                 float x[32];
@@ -919,7 +927,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             }
             as_wait_st();
         };
-        // ACC: the prefix's O into registers
+        // ACC: the run's O joins the prefix's in registers
         auto bring = [&]() {
 #pragma unroll
             for (int k = 0; k < HD; k += 32) {
@@ -927,7 +935,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_ld32(o_base + k, x);
                 as_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[k / 2 + i] = as_f2(x[2 * i], x[2 * i + 1]);
+                for (int i = 0; i < 16; ++i) o[k / 2 + i] = as_add2(o[k / 2 + i], as_f2(x[2 * i], x[2 * i + 1]));
             }
         };
         // scores of tile j -> weights of the rows that act, for the first h0 of this half's keys.
@@ -1064,6 +1072,12 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             if (any) {
                 const float kq = C::KF32 ? fmaxf(qs * m->ksc[j & 3], 1e-37f) : qs;  // (above 0: -inf stays -inf)
                 cnew = weigh(j, act, w.valid - half * HC, kq, of_prefix && !first);
+                // a new run starts: its first product waits for p_full, behind these reads
+                if (C::ACC && of_prefix && !first && (t - seg_t0) % AS_RUN == 0) {
+                    as_wait(m, &m->o_full[bf ^ 1], ((j - 1) >> 1) & 1, ok);
+                    as_tc_after();
+                    bring();
+                }
             }
             as_wait_st();
             as_tc_before();

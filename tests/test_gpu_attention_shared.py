@@ -401,3 +401,38 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for got, want in outs:
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("types", TYPES[2:])
+def test_long_prefix_of_one_cta(types):
+    """Row tiles enough that one CTA walks a head's whole prefix of 2,048 tiles. Every V is 1,
+    and so is the output: the weights are summed as rounded. Of the f32 sums behind it, the
+    row's adds one rounding a tile (2,048 of 2^-24); O's, with a run of 16 tiles that adds 16
+    keys 128 times, loses at most 17 / 4 of 2^-23 each time (17 terms cut two bits below the
+    sum's last place) and one rounding a run; the rest is below 2^-18. Together 2.0e-4, where
+    f16 has its half step below 1 at 2.4e-4 (bf16 further)."""
+    import torch
+
+    n, prefix = 1024, 2048 * 128
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    t = getattr(torch, types[0])
+    q = (torch.randn(n, 16, 64, device="cuda", generator=g) * 2).to(t)
+    kp = torch.randn(prefix, 1, 64, device="cuda", generator=g).to(t)
+    k = torch.randn(4, 3, 1, 64, device="cuda", generator=g).to(t)
+    lens = torch.arange(n, dtype=torch.int32, device="cuda") % 4
+    slots = torch.arange(n, dtype=torch.int32, device="cuda") % 5  # 4: no suffix
+    got = talos_b200.attention_shared_dev(q, kp, torch.ones_like(kp), k, torch.ones_like(k), slots, lens)
+    assert bool((got == 1).all()), f"off by up to {float((got.double() - 1).abs().max()):.3g}"
+
+
+@pytest.mark.parametrize("types", TYPES[2:])
+@pytest.mark.parametrize("prefix,rows", [(64 * 128, 130), (3 * 64 * 128 + 77, 5), (65 * 128, 0), (16 * 128, 40)])
+def test_prefix_runs_and_late_maxima(types, prefix, rows):
+    """Runs of 16 prefix tiles that end with the prefix or behind it, with maxima that grow
+    around a run's end."""
+    q, kp, vp, k, v, slots, lens = make(140, 128, 1, 64, prefix, rows, types, seed=prefix)
+    for at in (16 * 128 - 1, 16 * 128 + 1, 64 * 128, prefix - 3):
+        if at < prefix:
+            kp[at] *= 1 + at / prefix
+    check((q, kp, vp, k, v, slots, lens))
