@@ -833,9 +833,11 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             else asm volatile("bar.sync 5, %0;" ::"n"(AS_CONV * 32) : "memory");
             const uint32_t all = __reduce_max_sync(0xffffffffu, m->cmax[is_v][j & 1][lane & 3]);
             const int e = as_exponent(all);
-            if (w == 0 && lane == 0) (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
             if (!is_v && j > 0) as_wait(m, &m->k_empty[0], (j - 1) & 1, ok);
             if (is_v && j > 1) as_wait(m, &m->v_empty[j & 1], ((j >> 1) - 1) & 1, ok);
+            // behind these waits: P V of tile j - 2 followed the hand-over of O of tile j - 4,
+            // whose scale stood in this word
+            if (w == 0 && lane == 0) (is_v ? m->vsc : m->ksc)[j & 3] = as_pow2(e - 14);
             cv::store(raw0, raw1, is_v ? sV + (j & 1) * (C::NK * C::KPLANE) : sK, w, lane, valid, e);
             // (every value read has been stored: nothing of the slots is under way)
             if (lane == 0) {

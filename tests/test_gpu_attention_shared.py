@@ -436,3 +436,20 @@ def test_prefix_runs_and_late_maxima(types, prefix, rows):
         if at < prefix:
             kp[at] *= 1 + at / prefix
     check((q, kp, vp, k, v, slots, lens))
+
+
+@pytest.mark.parametrize("kvh,hd", [(1, 64), (2, 128)])
+def test_f32_tiles_of_changing_magnitude(kvh, hd):
+    """Every tile of 64 keys has values of its own magnitude (and so its own power of two),
+    over many prefix tiles and many suffix tiles, most of which end early."""
+    import torch
+
+    types = ("float32", "float32")
+    for n, prefix, rows in ((40, 5000, 300), (128, 0, 140), (16, 64 * 70, 64 * 9)):
+        q, kp, vp, k, v, slots, lens = make(n, 4 * kvh, kvh, hd, prefix, rows, types, seed=n)
+        f = 2.0 ** torch.randint(-8, 9, (prefix // 64 + 1,), device="cuda")
+        g = 2.0 ** torch.randint(-8, 9, (n, rows // 64 + 1), device="cuda")
+        vp *= f.repeat_interleave(64)[:prefix, None, None]
+        v *= g.repeat_interleave(64, 1)[:, :rows, None, None]
+        for _ in range(3):
+            check((q, kp, vp, k, v, slots, lens))
