@@ -118,7 +118,7 @@ struct AsCfg {
 };
 
 struct AsMisc {
-    uint64_t q_raw[2], q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], r_full[8], r_empty[8];
+    uint64_t q_raw[2], q_full, q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4], r_full[8], r_empty[8];
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], done;
     uint32_t tmem;
     int fail;
@@ -457,7 +457,10 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         mbar_init(&m->q_full, C::QF32 ? AS_SOFT : 1);
         mbar_init(&m->q_raw[0], 1);
         mbar_init(&m->q_raw[1], 1);
-        mbar_init(&m->q_empty, C::QF32 ? AS_SOFT : 1);
+        // (one for the even kv heads of a run and one for the odd: with heads up to 64 the softmax
+        // warps can be done with a kv head's queries before the copies wait for those before)
+        mbar_init(&m->q_empty[0], C::QF32 ? AS_SOFT : 1);
+        mbar_init(&m->q_empty[1], C::QF32 ? AS_SOFT : 1);
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             mbar_init(&m->k_full[i], C::KF32 ? AS_CONV : 1);
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
     auto copy_q = [&](int kvh, int seg) {
         constexpr int W = C::QF32 ? 32 : 64;
         uint64_t* bar = C::QF32 ? &m->q_raw[seg & 1] : &m->q_full;
-        if (seg > 0) as_wait(m, &m->q_empty, (seg - 1) & 1, ok);
+        if (seg > 0) as_wait(m, &m->q_empty[(seg - 1) & 1], ((seg - 1) >> 1) & 1, ok);
         if (!ok) return;
         mbar_expect_tx(bar, (uint32_t)(min(spt, a.n) * G) * 128 * (DP / W));
 #pragma unroll
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 }
                 as_commit(&m->k_empty[sk]);
                 as_commit(&m->s_full[bf]);
-                if (!C::QF32 && (t + 1 == t1 || w.off + 1 == tpg)) as_commit(&m->q_empty);  // the queries may be replaced
+                if (!C::QF32 && (t + 1 == t1 || w.off + 1 == tpg)) as_commit(&m->q_empty[seg & 1]);  // the queries may be replaced
             }
             __syncwarp();
             w.next(tpg);
@@ -746,7 +749,10 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             auto slot_free = [&]() {
                 const uint32_t b = 1u << st;
                 if (held_q & b) {
-                    if (first_q & b) as_wait(m, &m->q_empty, q_done++ & 1, ok);
+                    if (first_q & b) {
+                        as_wait(m, &m->q_empty[q_done & 1], q_done >> 1 & 1, ok);
+                        ++q_done;
+                    }
                     held_q &= ~b, first_q &= ~b;
                 } else if (used & b) {
                     as_wait(m, &m->r_empty[st], re_par >> st & 1, ok);
@@ -864,7 +870,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
         const uint32_t o_base = lane_base + C::O_COL + half * HD;
 
         // the row's f32 queries (this thread's half of the dims), scaled and split into TMEM
-        auto load_q = [&](int seg) {
+        auto load_q = [&](int seg) {  // seg: kv heads before this one in the run
             float4 v[HD / 4];
             float mx = 0.f;
             as_wait(m, &m->q_raw[seg & 1], (seg >> 1) & 1, ok);
@@ -909,7 +915,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             __syncwarp();
             if (lane == 0) {
                 as_arrive(&m->q_full, ok);
-                as_arrive(&m->q_empty, ok);
+                as_arrive(&m->q_empty[seg & 1], ok);
             }
         };
         // ACC: the prefix's O (registers and buffer 0) times c

@@ -453,3 +453,15 @@ def test_f32_tiles_of_changing_magnitude(kvh, hd):
         v *= g.repeat_interleave(64, 1)[:, :rows, None, None]
         for _ in range(3):
             check((q, kp, vp, k, v, slots, lens))
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("n,kvh,group,hd,prefix", [(256, 64, 1, 64, 40), (130, 40, 16, 48, 64), (1024, 6, 16, 64, 1),
+                                                   (64, 300, 2, 32, 20), (64, 64, 2, 128, 33)])
+def test_one_tile_per_kv_head(types, n, kvh, group, hd, prefix):
+    """CTAs that take one tile of one kv head after another: the queries change with every
+    tile (room for long suffixes, of which there are none or few)."""
+    lens = np.zeros(n, np.int64)
+    check(make(n, kvh * group, kvh, hd, prefix, 300, types, seed=n, lens=lens, n_slots=4))
+    lens[n // 2] = 3
+    check(make(n, kvh * group, kvh, hd, prefix, 300, types, seed=n, lens=lens, n_slots=4))
