@@ -1078,7 +1078,8 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
             as_tc_after();
             float cnew = 1.f;
             if (any) {
-                const float kq = C::KF32 ? fmaxf(qs * m->ksc[j & 3], 1e-37f) : qs;  // (above 0: -inf stays -inf)
+                // (f32 queries: above 0, or the -inf of the keys that do not count would become NaN)
+                const float kq = C::QF32 ? fmaxf(C::KF32 ? qs * m->ksc[j & 3] : qs, 1e-37f) : qs;
                 cnew = weigh(j, act, w.valid - half * HC, kq, of_prefix && !first);
                 // a new run starts: its first product waits for p_full, behind these reads
                 if (C::ACC && of_prefix && !first && (t - seg_t0) % AS_RUN == 0) {

@@ -465,3 +465,13 @@ def test_one_tile_per_kv_head(types, n, kvh, group, hd, prefix):
     check(make(n, kvh * group, kvh, hd, prefix, 300, types, seed=n, lens=lens, n_slots=4))
     lens[n // 2] = 3
     check(make(n, kvh * group, kvh, hd, prefix, 300, types, seed=n, lens=lens, n_slots=4))
+
+
+@pytest.mark.parametrize("scale", [1e-10, 1e-30])
+def test_zero_queries_with_small_scales(scale):
+    """A row of zeros has equal weights, whatever the scale: the mean of its values."""
+    for types in TYPES[:2]:
+        q, kp, vp, k, v, slots, lens = make(6, 8, 2, 64, 200, 70, types, seed=9)
+        q[2] = 0
+        q[4, 3] = 0
+        check((q, kp, vp, k, v, slots, lens), scale=scale)
