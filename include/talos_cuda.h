@@ -512,7 +512,8 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * kv head h / (n_head / n_head_kv), the keys are prefix rows 0 .. prefix_len-1
  * and rows 0 .. lens[i]-1 of cache slot slots[i];
  *   out[i][h] = softmax(scale * q . K) V        (src/model/llama.rs:135-155)
- * and zeros where there is no key at all. The prefix is read once for all
+ * and zeros where there is no key at all, or none whose score in f32 is above -inf
+ * (such a key has no weight beside others). The prefix is read once for all
  * sequences of a row tile (128 / (n_head / n_head_kv) of them) instead of once
  * per sequence. Rows behind lens[i], and slots that no sequence names, are not
  * read. Types (q and out, cache): F32 with F32 (the reference's cache) or F16,

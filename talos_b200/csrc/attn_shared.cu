@@ -975,7 +975,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 // only moves when it is passed by 2^8, as O in tensor memory then moves too
                 const float top = ceilf(fmaxf(mt, m->mx[bf][half ^ 1][row]));
                 const float mnew = top > mrun + (C::ACC ? 8.f : 0.f) ? top : mrun;
-                cnew = as_ex2(mrun - mnew);
+                if (mnew != mrun) cnew = as_ex2(mrun - mnew);  // (equal: also -inf, where no score was above it)
                 lsum *= cnew;
                 mrun = mnew;
             }
@@ -984,7 +984,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 as_tc_after();
                 rescale(cnew);
             }
-            const float sub = act ? OFF - mrun : 0.f;  // (no weight where -inf)
+            const float sub = act && mrun > -INFINITY ? OFF - mrun : 0.f;  // (no weight where -inf)
             const f2 q2 = as_f2(kq, kq), sub2 = as_f2(sub, sub);
             f2 l2[2] = {0ull, 0ull};
             // P over S: hi planes in the first half of the columns, lo in the second

@@ -475,3 +475,45 @@ def test_zero_queries_with_small_scales(scale):
         q[2] = 0
         q[4, 3] = 0
         check((q, kp, vp, k, v, slots, lens), scale=scale)
+
+
+def test_scores_that_overflow():
+    """Keys whose score is -inf in f32 have no weight: they fill the first tiles of the
+    prefix, all of some suffixes and some rows alone."""
+    import torch
+
+    types = ("bfloat16", "bfloat16")
+    q, kp, vp, k, v, slots, lens = make(6, 8, 2, 64, 400, 150, types, seed=12, lens=[150, 0, 1, 130, 64, 129])
+    q[:, :, 5] = 3e38
+    q[1, 2, 5] = 0.0
+    kp[:, :, 5], k[..., 5] = 0, 0
+    clean = oracle(q, torch.cat([kp[300:], kp[:0]]), torch.cat([vp[300:], vp[:0]]), k, v, slots, lens * 0)
+    kp[:300, :, 5] = -10
+    k[..., 5] = -10
+    got = talos_b200.attention_shared_dev(q, kp, vp, k, v, slots, lens)
+    ref, top, vmax, keys = clean
+    # the bound of check() over the keys that count (q's huge element meets zeros there)
+    bound = 2 * 2.0**-23 * ((64 / 16 + 5) * top + 64 + 6) * vmax + 2.0**-8 * (vmax + ref.abs())
+    rows = torch.ones(6, 8, dtype=torch.bool, device="cuda")
+    rows[1, 2] = False  # (this row attends to every key)
+    assert torch.isfinite(got).all()
+    assert bool(((got.double() - ref).abs() <= bound)[rows].all())
+    whole = oracle(q[1:2, 2:3], kp[:, :1], vp[:, :1], k[:, :, :1], v[:, :, :1], slots[1:2], lens[1:2])[0]
+    assert bool(((got[1, 2].double() - whole[0, 0]).abs() <= bound[1, 2]).all())
+
+
+def test_a_sequence_whose_scores_all_overflow():
+    """No key with a weight: zeros, in one CTA's tile and in partials."""
+    import torch
+
+    for prefix, rows in ((0, 40), (700, 600)):
+        q, kp, vp, k, v, slots, lens = make(5, 8, 2, 64, prefix, rows, ("bfloat16", "bfloat16"), seed=3,
+                                            lens=[rows] * 5)
+        q[:, :, 5] = 0
+        kp[:, :, 5], k[..., 5] = -10, -10
+        want = talos_b200.attention_shared_dev(q, kp, vp, k, v, slots, lens)
+        q[3, :, 5] = 3e38
+        got = talos_b200.attention_shared_dev(q, kp, vp, k, v, slots, lens)
+        assert not got[3].any()
+        keep = [0, 1, 2, 4]
+        assert torch.equal(got[keep], want[keep])
