@@ -523,7 +523,9 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * strides are in elements; pointers and strides are multiples of 16 bytes. K
  * and V share their strides. lens are clamped to 0 .. slot_len; a sequence
  * whose slot is out of range has no suffix. Keys that are attended to hold
- * finite values; one sequence's infinities or NaN do not reach another's output.
+ * finite values; an infinite or NaN value makes its own dimension of the outputs that
+ * attend to it infinite or NaN. What a sequence's own rows hold does not reach another's
+ * output.
  *
  * work: talos_attention_shared_work bytes of device memory, 16-byte aligned,
  * used by this call alone until it has run (two calls in flight, or two graphs

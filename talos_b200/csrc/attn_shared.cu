@@ -380,7 +380,7 @@ struct AsConv {
         if (r >= valid) return make_float4(0.f, 0.f, 0.f, 0.f);
         return *(const float4*)((r < HALF ? raw0 : raw1) + r % HALF * (QC * 16) + ch * 16);
     }
-    // the warp's largest |element| as bits
+    // the warp's largest finite |element| as bits (an infinite one must not scale the others to 0)
     static __device__ __forceinline__ uint32_t largest(const uint8_t* raw0, const uint8_t* raw1, int w, int lane,
                                                        int valid) {
         const int ch = lane % QC, sub = lane / QC;
@@ -391,7 +391,18 @@ struct AsConv {
             mx = as_max3(mx, fabsf(v.x), fabsf(v.y));
             mx = as_max3(mx, fabsf(v.z), fabsf(v.w));
         }
-        return __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+        uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+        if (top == 0x7f800000u) {
+            mx = 0.f;
+#pragma unroll 1
+            for (int q = 0; q < NI; ++q) {
+                const float4 v = chunk(raw0, raw1, (w + NW * q) * QR + sub, ch, valid);
+                for (const float x : {v.x, v.y, v.z, v.w})
+                    if (fabsf(x) < INFINITY) mx = fmaxf(mx, fabsf(x));
+            }
+            top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+        }
+        return top;
     }
     static __device__ __forceinline__ void store(const uint8_t* raw0, const uint8_t* raw1, uint8_t* tile, int w, int lane,
                                                  int valid, int e) {

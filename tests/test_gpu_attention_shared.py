@@ -517,3 +517,28 @@ def test_a_sequence_whose_scores_all_overflow():
         assert not got[3].any()
         keep = [0, 1, 2, 4]
         assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinite_values_keep_to_their_dimension(types, bad):
+    """An attended value that is infinite or NaN leaves no finite output in its own dimension
+    and the others as they are."""
+    import torch
+
+    q, kp, vp, k, v, slots, lens = make(7, 8, 2, 128, 150, 90, types, seed=15, lens=[90, 80, 0, 64, 65, 1, 90])
+    args = (q, kp, vp, k, v, slots, lens)
+    vp[20, 0, 3] = bad
+    v[int(slots[3]), 40, 1, 70] = bad
+    hit = torch.zeros(7, 8, 128, dtype=torch.bool, device="cuda")
+    hit[:, :4, 3] = True
+    hit[3, 4:, 70] = True
+    got = talos_b200.attention_shared_dev(*args)
+    assert not torch.isfinite(got[hit]).any()
+    vp[20, 0, 3] = 0
+    v[int(slots[3]), 40, 1, 70] = 0
+    ref, top, vmax, keys = oracle(*args)
+    bound = 2 * 2.0**-23 * ((128 / 16 + 5) * top + 64 + keys / 64) * vmax
+    if q.dtype != torch.float32:
+        bound = bound + torch.finfo(q.dtype).eps / 2 * (vmax + ref.abs())
+    assert bool(((got.double() - ref).abs() <= bound)[~hit].all())
