@@ -531,6 +531,7 @@ __global__ void __launch_bounds__((AsCfg<MODE, DP>::THREADS), 1)
                 before += __shfl_sync(0xffffffffu, x, 31);
             }
         }
+        as_fence_async();  // (cnt's bytes are written by TMA copies next)
         __syncthreads();
         rt = m->rt, b0 = m->b0, nb = m->nb;
     }
