@@ -519,10 +519,11 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * read. Types (q and out, cache): F32 with F32 (the reference's cache) or F16,
  * F16 with F16, BF16 with BF16; f32 queries get f32 accuracy on the tensor
  * cores. head_dim up to 128, a multiple of 8 (4 where all is F32); n_head at
- * most 128 times n_head_kv; n up to 1024. The last dimension is contiguous;
- * strides are in elements; pointers and strides are multiples of 16 bytes. K
- * and V share their strides. lens are clamped to 0 .. slot_len; a sequence
- * whose slot is out of range has no suffix. Keys that are attended to hold
+ * most 128 times n_head_kv; n up to 1024. UNSUPPORTED beyond 2^30 tiles of 64 keys (of
+ * one row tile over the kv heads, or of one kv head over the row tiles). The last
+ * dimension is contiguous; strides are in elements; pointers and strides are multiples
+ * of 16 bytes. K and V share their strides. lens are clamped to 0 .. slot_len; a
+ * sequence whose slot is out of range has no suffix. Keys that are attended to hold
  * finite values; an infinite or NaN value makes its own dimension of the outputs that
  * attend to it infinite or NaN. What a sequence's own rows hold does not reach another's
  * output.

@@ -153,8 +153,15 @@ extern "C" talos_status talos_attention_shared_dev(const talos_attention_shared_
         return set_err(TALOS_ERR_INVALID_ARG, "%u slots", a->n_slots);
     const uint64_t spt = 128 / (a->n_head / a->n_head_kv);
     const uint64_t tiles = a->prefix_len / 64 + 1 + std::min<uint64_t>(a->n, spt) * (a->slot_len / 64 + 1ull);
-    if (tiles * a->n_head_kv > 0x3fffffffull || a->prefix_len > 0x3fffffffu || a->slot_len > 0x3fffffffu)
-        return set_err(TALOS_ERR_UNSUPPORTED, "prefix of %u and slots of %u positions", a->prefix_len, a->slot_len);
+    // the kernels count the tiles of a row tile over the kv heads, of a kv head over the row
+    // tiles, a row tile's output elements and the second kernel's warps in 32 bits
+    const uint64_t row_tiles = (a->n + spt - 1) / spt;
+    if (tiles * std::max<uint64_t>(a->n_head_kv, row_tiles) > 0x3fffffffull || a->prefix_len > 0x3fffffffu ||
+        a->slot_len > 0x3fffffffu)
+        return set_err(TALOS_ERR_UNSUPPORTED, "prefix of %u and slots of %u positions for %u sequences", a->prefix_len,
+                       a->slot_len, a->n);
+    if (128ull * a->n_head_kv * a->head_dim > 0x3fffffffull || row_tiles * a->n_head_kv * 128 > 0x3fffffffull)
+        return set_err(TALOS_ERR_UNSUPPORTED, "%u sequences of %u heads", a->n, a->n_head);
     AttnSharedArgs k{};
     // a dimension of one element (or none) has no stride to speak of
     auto st = [](size_t stride, uint32_t count) { return count > 1 ? stride : 0; };

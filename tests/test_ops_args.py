@@ -119,3 +119,13 @@ def test_packed_arguments_have_the_structs_layout():
         fields = [name for name, _ in struct_._fields_]
         got = struct_.from_buffer_copy(packed.pack(*range(1, len(fields) + 1)))
         assert [int(getattr(got, name)) for name in fields] == list(range(1, len(fields) + 1))
+
+
+def test_attention_sizes_beyond_the_kernels_counts(lib):
+    """Row tiles times key tiles, and heads, that 32-bit counts do not hold."""
+    wide = dict(n=1024, n_head=128, n_head_kv=1, out_stride_n=128 * 64)
+    assert attention(lib, prefix_len=1 << 27, **wide) == _lib.UNSUPPORTED
+    assert attention(lib, slot_len=1 << 27, **wide) == _lib.UNSUPPORTED
+    for n, heads in ((128, 1 << 17), (1, 1 << 24)):
+        kw = dict(n=n, n_head=heads, n_head_kv=heads, prefix_len=0, out_stride_n=heads * 64)
+        assert attention(lib, **kw) == _lib.UNSUPPORTED
