@@ -292,9 +292,13 @@ talos_status talos_generate_batch_sample(talos_ctx* ctx, const uint32_t* tokens,
  * batched generation then attend to them once for all sequences (the tensor-core
  * attention of talos_attention_shared_dev) and to the slots' own rows from position n
  * on, and refuse positions below n. The slots keep rows by their absolute positions.
- * A call with a prefix in place extends it from the slot's rows behind it, or cuts it;
- * n = 0 ends the sharing (the slots' rows below the old prefix are then what they were
- * before it, so only slots that were filled themselves can go on). Takes the memory of
+ * A call with a prefix in place extends it from the slot's rows behind it, or cuts it.
+ * The slot is then the one that the prefix came from, or one whose sequence went on
+ * behind it (to extend it, up to the last of its positions); a slot that holds another
+ * prompt, or whose rows are older than the sharing, is refused (INVALID_ARG): end the
+ * sharing first. n = 0 ends it, whatever the slot (the slots' rows below the old prefix
+ * are then what they were before it, so only slots that were filled themselves can go
+ * on). Takes the memory of
  * one more slot, from the first call to the release of the slots. The attention's
  * scores and weights are exact to about 22 bits, like the f32 path's own roundings;
  * results with and without sharing differ in their last bits. Under tensor parallelism

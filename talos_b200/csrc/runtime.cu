@@ -369,6 +369,14 @@ struct LayerW {
 
 enum GraphMode { GM_LOGITS = 0, GM_HIDDEN = 1, GM_GREEDY = 2, GM_COUNT = 3 };
 
+// Which rows of a cache slot belong to the sequence that a batch step continues, beside a
+// shared prefix of P rows: talos_batch_share does not take another prompt's rows for it.
+struct SlotRows {
+    bool held = false;       // it may hold a prompt of its own
+    size_t same = 0;         // the sequence's first `same` positions are the prefix's
+    size_t low = 0, to = 0;  // same == P: the slot's rows low .. to - 1 are the sequence's
+};
+
 struct talos_ctx {
     talos_cfg cfg{};
     int device = 0;
@@ -461,6 +469,7 @@ struct talos_ctx {
     // shared prefix (talos_batch_share): its length, rows ([n_layer][kv_ctx][kv_dim] of K,
     // then of V) and the attention's workspace; one allocation, made at the first use
     size_t bprefix = 0;
+    SlotRows brows[TALOS_MAX_BATCH];
     void* bpmem = nullptr;
     float *bpk = nullptr, *bpv = nullptr;
     void* bpwork = nullptr;
@@ -1696,6 +1705,7 @@ static talos_status batch_free(talos_ctx* c) {
     if (c->bpmem) cudaFree(c->bpmem);
     c->bpmem = nullptr;
     c->bprefix = c->bpbytes = 0;
+    for (SlotRows& r : c->brows) r = SlotRows{};
     c->bmem = nullptr;
     c->bbytes = 0;
     c->bmax = 0;
@@ -2137,6 +2147,46 @@ static talos_status check_slot_pos(talos_ctx* c, uint32_t token, size_t pos) {
     return TALOS_OK;
 }
 
+// Positions from .. end - 1 of slot are about to be written by steps.
+static void slot_written(talos_ctx* c, int slot, size_t from, size_t end) {
+    SlotRows& r = c->brows[slot];
+    if (!c->bprefix) {
+        r.held = true;
+        return;
+    }
+    if (r.same != c->bprefix) r.same = r.low = r.to = c->bprefix;
+    if (from <= r.to) r.to = std::max(r.to, end);
+}
+
+// Rows were copied between slots.
+static void slots_moved(talos_ctx* c, const talos_kv_copy* moves, size_t n) {
+    SlotRows old[TALOS_MAX_BATCH];
+    std::copy(c->brows, c->brows + TALOS_MAX_BATCH, old);
+    const size_t P = c->bprefix;
+    for (size_t i = 0; i < n; ++i) {
+        const talos_kv_copy& m = moves[i];
+        if (m.src == m.dst || !m.len) continue;
+        const SlotRows& s = old[m.src];
+        SlotRows& d = c->brows[m.dst];
+        const size_t from = m.start, end = from + m.len, at = std::max(from, P);
+        if (!P) {
+            d.held |= s.held;
+        } else if (from == 0 && end >= P) {
+            d = s;
+            d.to = std::min(s.to, end);
+        } else {
+            if (from < P) {
+                d.held |= s.held;
+                if (d.low < P) d.same = 0;
+            }
+            if (end <= P) continue;
+            const bool follows = s.same == P && at >= s.low;
+            if (d.same != P && at == P && follows) d.same = d.low = d.to = P;
+            if (d.same == P && at <= d.to) d.to = follows ? std::max(at, std::min(end, s.to)) : at;
+        }
+    }
+}
+
 extern "C" talos_status talos_forward_batch(talos_ctx* c, const uint32_t* tokens, const size_t* pos, int n,
                                             float* logits_out) {
     if (!c || !tokens || !pos || !logits_out) return set_err(TALOS_ERR_INVALID_ARG, "NULL argument");
@@ -2146,6 +2196,7 @@ extern "C" talos_status talos_forward_batch(talos_ctx* c, const uint32_t* tokens
     for (int i = 0; i < n; ++i) TRY(check_slot_pos(c, tokens[i], pos[i]));
     TRY(bind_if_dirty(c));
     TRY(batch_check(c));
+    for (int i = 0; i < n; ++i) slot_written(c, i, pos[i], pos[i] + 1);
     TRY(batch_step(c, BM_DECODE, tokens, pos, nullptr, n, true));
     return batch_finish(c, n, logits_out);
 }
@@ -2160,6 +2211,7 @@ extern "C" talos_status talos_prefill_slot(talos_ctx* c, int slot, const uint32_
     for (size_t i = 0; i < n; ++i) TRY(check_slot_pos(c, tokens[i], pos0 + i));
     TRY(bind_if_dirty(c));
     TRY(batch_check(c));
+    slot_written(c, slot, pos0, pos0 + n);
     std::vector<size_t> pos(MB_SEQ);
     const std::vector<int> slots(MB_SEQ, slot);
     int last_n = 1;
@@ -2219,6 +2271,7 @@ static talos_status batch_generate(talos_ctx* c, int mode, const uint32_t* token
     }
     const int ntc = ntc_for(n);
     TRY(batch_graph(c, mode, ntc));
+    for (int i = 0; i < n; ++i) slot_written(c, i, pos[i], pos[i] + steps);
     TRY(set_batch_params(c, tokens, pos, nullptr, n, true));
     for (size_t k = 0; k < steps; ++k) CK(cudaGraphLaunch(c->bgraph[mode][ntc][with_prefix(c, mode)], c->stream));
     if (c->tp > 1) c->btpstep += (uint32_t)steps;
@@ -2255,6 +2308,15 @@ extern "C" talos_status talos_batch_share(talos_ctx* c, int slot, size_t n) {
         return set_err(TALOS_ERR_INVALID_ARG, "slot %d (the context holds %d; talos_ctx_set_batch)", slot, c->bmax);
     if (n > c->kv_ctx)
         return set_err(TALOS_ERR_INVALID_ARG, "a prefix of %zu rows (the context has %zu)", n, c->kv_ctx);
+    const size_t P = c->bprefix;
+    SlotRows& own = c->brows[slot];
+    if (P && n > P && (own.same != P || own.to < n))
+        return set_err(TALOS_ERR_INVALID_ARG,
+                       "rows %zu .. %zu of slot %d do not all follow the shared prefix (end its sharing first: n = 0)", P,
+                       n - 1, slot);
+    if (P && n && n <= P && own.held && own.same < n)
+        return set_err(TALOS_ERR_INVALID_ARG,
+                       "slot %d holds rows that are not the shared prefix's (end its sharing first: n = 0)", slot);
     CK(cudaSetDevice(c->device));
     if (n && !c->bpmem) {
         const int group = c->nkv_l ? c->nh_l / c->nkv_l : 0;
@@ -2275,16 +2337,29 @@ extern "C" talos_status talos_batch_share(talos_ctx* c, int slot, size_t n) {
         c->bpk = (float*)mem, c->bpv = (float*)((uint8_t*)mem + rows);
         c->bpwork = (uint8_t*)mem + 2 * rows;
     }
-    if (n > c->bprefix) {  // the rows behind the present prefix (a plane per layer)
-        const size_t from = c->bprefix * c->kv_l, pitch = c->kv_ctx * (size_t)c->kv_l * 4;
-        const size_t src = (size_t)slot * c->bseq_stride + from, width = (n - c->bprefix) * c->kv_l * 4;
+    if (n > P) {  // the rows behind the present prefix (a plane per layer)
+        const size_t from = P * c->kv_l, pitch = c->kv_ctx * (size_t)c->kv_l * 4;
+        const size_t src = (size_t)slot * c->bseq_stride + from, width = (n - P) * c->kv_l * 4;
         CK(cudaMemcpy2DAsync(c->bpk + from, pitch, c->bkc + src, pitch, width, c->cfg.n_layer,
                              cudaMemcpyDeviceToDevice, c->stream));
         CK(cudaMemcpy2DAsync(c->bpv + from, pitch, c->bvc + src, pitch, width, c->cfg.n_layer,
                              cudaMemcpyDeviceToDevice, c->stream));
     }
-    c->bprefix = n;
     CK(cudaStreamSynchronize(c->stream));
+    c->bprefix = n;
+    for (SlotRows& r : c->brows) {
+        if (n == 0) {
+            r.held |= r.same > 0;
+            r.same = 0;
+        } else if (n < P) {
+            r.same = std::min(r.same, n);
+            if (r.low > n) r.low = r.to = n;
+        }
+    }
+    if (n > P) {
+        own.same = n;
+        if (!P) own.low = 0, own.to = c->kv_ctx;  // what it was filled with
+    }
     return TALOS_OK;
 }
 
@@ -2305,6 +2380,7 @@ extern "C" talos_status talos_batch_move(talos_ctx* c, const talos_kv_copy* move
     g.outer_stride = c->kv_ctx * g.row_stride;
     TRY(talos_kv_move_dev(&g, moves, n, c->stream));
     CK(cudaStreamSynchronize(c->stream));
+    slots_moved(c, moves, n);
     return TALOS_OK;
 }
 

@@ -243,7 +243,8 @@ class Context:
 
     def batch_share(self, slot: int, n: int):
         """talos_batch_share: positions 0 .. n-1 of ``slot`` become the prefix of every
-        sequence of the batch (kept and read once); 0 ends the sharing."""
+        sequence of the batch (kept and read once); 0 ends the sharing. While a prefix is
+        shared, only slots that hold it or went on behind it can be named."""
         if n < 0:
             raise ValueError("a prefix of less than no rows")
         _lib.check(_lib.load().talos_batch_share(self.h, int(slot), int(n)))

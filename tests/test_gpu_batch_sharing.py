@@ -258,3 +258,67 @@ def test_a_row_without_a_choice_ends_the_call():
     with pytest.raises(TalosError, match="device check"):
         m.generate_batch_sample([1, 2], [0, 0], np.full((3, 2), 0.5))
     m.close()
+
+
+def test_sharing_another_prompt_is_refused_while_one_is_shared():
+    """A slot filled with a prompt of its own before the sharing is not taken for a
+    continuation of the shared one: naming it is refused, at equal, smaller and larger
+    lengths, and the prefix stays; after the sharing ended it can be shared."""
+    data = tiny_model(gguf.Q8_0)
+    a, b = list(prompt(20, 4096, 21)), list(prompt(30, 4096, 22))
+    m = load(data, 3)
+    m.prefill_slot(0, a)
+    m.prefill_slot(1, b)
+    m.batch_share(0, 20)
+    want = oracle_logits(data, a + [77])[-1]
+    for n in (20, 30, 7):
+        with pytest.raises(TalosError, match="INVALID_ARG"):
+            m.batch_share(1, n)
+        assert np.max(np.abs(m.forward_batch([77] * 3, [20] * 3) - want)) <= 1e-3
+        m.batch_share(0, 0)  # slot 1's row 20 is the step's now: fill it again
+        m.prefill_slot(1, b)
+        m.batch_share(0, 20)
+    m.batch_share(0, 0)
+    m.batch_share(1, 30)
+    want = oracle_logits(data, b + [78])[-1]
+    assert np.max(np.abs(m.forward_batch([78] * 3, [30] * 3) - want)) <= 1e-3
+    m.close()
+
+
+def test_slots_that_may_be_named_while_a_prefix_is_shared():
+    """The slot that it came from (to extend it, and back after another extended it), a reused
+    slot that went on behind it, a fork of either; not a slot whose rows behind it are older."""
+    data = tiny_model(gguf.Q4_0)
+    a, b, tail = list(prompt(40, 4096, 23)), list(prompt(60, 4096, 24)), list(prompt(12, 4096, 25))
+
+    def after(toks):
+        return oracle_logits(data, toks + [99])[-1]
+
+    def shares(want, n):
+        assert np.max(np.abs(m.forward_batch([99] * 4, [n] * 4) - want)) <= 1e-3
+
+    m = load(data, 6)
+    m.prefill_slot(0, a)
+    for s in (1, 2, 5):
+        m.prefill_slot(s, b)
+    m.batch_share(0, 25)
+    m.prefill_slot(4, tail, 25)
+    m.batch_share(0, 40)  # extended by its own rows
+    shares(after(a), 40)
+    m.batch_share(0, 25)  # cut
+    m.prefill_slot(1, tail, 25)  # a reused slot goes on: rows 25 .. 36
+    with pytest.raises(TalosError, match="INVALID_ARG"):
+        m.batch_share(1, 38)  # its row 37 is an older prompt's
+    m.batch_move([(1, 3, 25, 12), (1, 2, 0, 60)])
+    with pytest.raises(TalosError, match="INVALID_ARG"):
+        m.batch_share(2, 38)  # as the slot it was copied from
+    m.batch_share(3, 37)  # a fork behind the prefix extends it
+    shares(after(a[:25] + tail), 37)
+    m.batch_share(1, 30)  # a slot that went on behind it cuts it
+    shares(after(a[:25] + tail[:5]), 30)
+    m.batch_share(0, 25)
+    shares(after(a[:25]), 25)
+    m.batch_move([(5, 0, 0, 60)])  # the first slot holds another prompt now
+    with pytest.raises(TalosError, match="INVALID_ARG"):
+        m.batch_share(0, 10)
+    m.close()
