@@ -572,7 +572,8 @@ talos_status talos_attention_shared_dev(const talos_attention_shared_args* args,
  * (compaction, permutations, one slot to many). Rows outside the ranges keep
  * their values. A slot may be the destination of one move only (INVALID_ARG
  * otherwise); src == dst or len == 0 does nothing. At most 512 moves. The
- * geometry must not make rows overlap (INVALID_ARG). No reference counterpart
+ * geometry must not make rows overlap, within an array or between two (INVALID_ARG;
+ * interleaved arrays are fine). No reference counterpart
  * (the reference keeps one sequence, src/kv_cache.rs:7-52).
  */
 typedef struct talos_kv_slots {

@@ -272,19 +272,32 @@ void plan_moves(std::vector<talos_kv_copy> m, std::vector<MoveIns>& ins,
 
 // Rows are disjoint when, from the smallest stride to the largest, each steps
 // over all that lies below it.
-bool disjoint(const talos_kv_slots& g) {
-    struct Dim {
-        size_t stride, count;
-    } d[3] = {{g.row_stride, g.n_rows}, {g.outer_stride, g.n_outer}, {g.slot_stride, g.n_slots}};
-    std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+struct MoveDim {
+    size_t stride, count;
+};
+bool disjoint(const talos_kv_slots& g, MoveDim (&d)[3]) {
+    d[0] = {g.row_stride, g.n_rows}, d[1] = {g.outer_stride, g.n_outer}, d[2] = {g.slot_stride, g.n_slots};
+    std::sort(d, d + 3, [](const MoveDim& x, const MoveDim& y) { return x.stride < y.stride; });
     size_t span = g.row_bytes;
-    for (const Dim& x : d) {
+    for (const MoveDim& x : d) {
         if (x.count <= 1) continue;
         if (x.stride < span) return false;
         if (x.stride > ((size_t)1 << 62) / x.count) return false;
         span = x.stride * (x.count - 1) + span;
     }
     return true;
+}
+// Whether a row of one array lies over one of another whose base is `off` bytes away: some
+// difference of indexes brings them together. The stride of a (disjoint) geometry's largest
+// dimension exceeds all that the others reach, so its difference is one of three.
+bool rows_meet(int64_t off, const MoveDim* d, int n, int64_t row_bytes) {
+    if (n == 0) return off < row_bytes && -off < row_bytes;
+    const MoveDim& x = d[n - 1];
+    if (x.count <= 1) return rows_meet(off, d, n - 1, row_bytes);
+    const int64_t s = (int64_t)x.stride, most = (int64_t)x.count - 1, k0 = -(off / s);
+    for (int64_t k = std::max(k0 - 1, -most); k <= std::min(k0 + 1, most); ++k)
+        if (rows_meet(off + k * s, d, n - 1, row_bytes)) return true;
+    return false;
 }
 
 }  // namespace
@@ -302,7 +315,12 @@ extern "C" talos_status talos_kv_move_dev(const talos_kv_slots* g, const talos_k
     if (n > (size_t)MOVE_MAX) return set_err(TALOS_ERR_INVALID_ARG, "%zu moves (at most %d)", n, MOVE_MAX);
     if (!g->row_bytes || !g->n_outer || g->row_bytes > 0xffffffffu)
         return set_err(TALOS_ERR_INVALID_ARG, "rows of %zu bytes in %u planes", g->row_bytes, g->n_outer);
-    if (!disjoint(*g)) return set_err(TALOS_ERR_INVALID_ARG, "the strides make rows overlap");
+    MoveDim dims[3];
+    if (!disjoint(*g, dims)) return set_err(TALOS_ERR_INVALID_ARG, "the strides make rows overlap");
+    for (int i = 0; i < g->n_base; ++i)
+        for (int j = 0; j < i; ++j)
+            if (rows_meet((int64_t)((uintptr_t)g->base[i] - (uintptr_t)g->base[j]), dims, 3, (int64_t)g->row_bytes))
+                return set_err(TALOS_ERR_INVALID_ARG, "rows of arrays %d and %d overlap", j, i);
     try {
         std::vector<talos_kv_copy> live;
         std::vector<uint32_t> dsts;

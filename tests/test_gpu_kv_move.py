@@ -162,3 +162,21 @@ def test_long_runs_of_several_chains():
     run(cs, [1, 2, 3, 6, 7], [0, 1, 2, 5, 6], [1024, 1003, 700, 1021, 977])
     run(cs, [3, 4, 8, 7], [2, 3, 6, 5], [1000, 1024, 1, 513], [24, 0, 1023, 11])
     run(cs, [0, 1, 4, 4], [1, 0, 7, 8], [1024, 1024, 301, 1024])
+
+
+def test_arrays_within_one_tensor():
+    """Keys and values side by side in one tensor's rows, planes or slots are moved; views that
+    share rows are refused and stay as they are."""
+    import torch
+
+    for dim in range(4):
+        shape = [4, 3, 10, 8]
+        shape.insert(dim, 2)
+        x = torch.randn(shape, device="cuda")
+        run(list(x.unbind(dim)), [0, 1, 3], [1, 0, 2], [10, 10, 7], [0, 0, 3])
+    x = torch.randn(4, 3, 10, 8, device="cuda")
+    keep = x.clone()
+    for a, b in ((x[:, :, :9], x[:, :, 1:]), (x[:, :2], x[:, 1:]), (x[:3], x[1:]), (x[..., :5], x[..., 3:])):
+        with pytest.raises(TalosError, match="INVALID_ARG"):
+            talos_b200.kv_move_dev([a, b], [0, 1], [1, 0], [5, 5])
+    assert torch.equal(x, keep)

@@ -129,3 +129,41 @@ def test_attention_sizes_beyond_the_kernels_counts(lib):
     for n, heads in ((128, 1 << 17), (1, 1 << 24)):
         kw = dict(n=n, n_head=heads, n_head_kv=heads, prefix_len=0, out_stride_n=heads * 64)
         assert attention(lib, **kw) == _lib.UNSUPPORTED
+
+
+def test_move_arrays_that_overlap(lib):
+    """Two arrays whose rows coincide in part are refused, interleaved ones are not: compared
+    with the rows' bytes one by one."""
+    def geometry(dims, row_bytes, off):
+        (n_rows, row_stride), (n_outer, outer_stride), (n_slots, slot_stride) = dims
+        base = (C.c_void_p * 2)(1 << 20, (1 << 20) + off)
+        g = _lib.KvSlots(0, 2, C.addressof(base), n_slots, n_outer, n_rows, slot_stride, outer_stride, row_stride,
+                         row_bytes)
+        return lib.talos_kv_move_dev(C.byref(g), None, 0, None)
+
+    dims = ((8, 64), (2, 512), (4, 1024))
+    for off in (64, -64, 32, 512, 1024, 1024 + 64, -3 * 1024 - 512, 4096 - 64):
+        assert geometry(dims, 64, off) == _lib.INVALID_ARG, off
+    assert geometry(dims, 64, 4096) == geometry(dims, 64, -4096) == _lib.OK
+    wide = ((8, 128), (2, 1024), (4, 2048))  # K and V rows in turn
+    assert geometry(wide, 64, 64) == geometry(wide, 64, -64) == _lib.OK
+    assert geometry(wide, 64, 63) == geometry(wide, 64, 65) == _lib.INVALID_ARG
+
+    rng = np.random.default_rng(0)
+    seen = set()
+    for _ in range(2000):
+        row_bytes = int(rng.integers(1, 5))
+        span, dims = row_bytes, []
+        for _ in range(3):
+            count = int(rng.integers(1, 4))
+            stride = span + int(rng.integers(0, 12))
+            dims.append((count, stride))
+            span += stride * (count - 1)
+        dims = [dims[i] for i in rng.permutation(3)]
+        at = {a * dims[0][1] + b * dims[1][1] + c * dims[2][1] + x for a in range(dims[0][0]) for b in range(dims[1][0])
+              for c in range(dims[2][0]) for x in range(row_bytes)}
+        off = int(rng.integers(1, span + 5)) * (1 if rng.random() < 0.5 else -1)
+        want = _lib.INVALID_ARG if any(x + off in at for x in at) else _lib.OK
+        assert geometry(dims, row_bytes, off) == want, (dims, row_bytes, off)
+        seen.add(want)
+    assert len(seen) == 2
