@@ -62,6 +62,22 @@ def _stream(T: _Torch, dev: int, stream) -> int:
     return T.stream(dev) if stream is None else int(stream)
 
 
+def _empty(T: _Torch, dev: int, stream, like, shape, dtype):
+    """A new tensor on like's device for work on ``stream``. With another stream than the
+    current one it comes from torch's memory for that stream, so that what is released while
+    the work is in flight goes to later work behind it, and its release waits for what the
+    current stream has done with it."""
+    if stream is None or int(stream) == T.stream(dev):
+        return like.new_empty(shape, dtype=dtype)
+    cuda = T.torch.cuda
+    current = cuda.current_stream(dev)
+    handle = int(stream)
+    with cuda.stream(cuda.ExternalStream(0 if handle == 1 else handle, device=dev)):  # (1: cudaStreamLegacy)
+        new = like.new_empty(shape, dtype=dtype)
+    new.record_stream(current)
+    return new
+
+
 def _pack(s: struct.Struct, *values) -> bytes:
     try:
         return s.pack(*values)
@@ -89,8 +105,12 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
     ``lens`` int32 on the device. f32 queries go with f32 or f16 caches, f16 and
     bf16 with their own; the last dimension is contiguous. ``scale`` None is
     1 / sqrt(head_dim). Returns ``out`` ([n, n_head, head_dim], q's type): zeros for
-    a sequence without keys. The workspace comes from torch's allocator on the
-    current stream; with another ``stream`` the caller orders the two."""
+    a sequence without keys. An infinite or NaN value in an attended row makes its
+    dimension of the output infinite or NaN; keys are finite; an element of an f32
+    cache keeps 22 bits, or 2^-39 of the largest among the 64 rows of its tile. With
+    another ``stream`` than the current one, the workspace and a new ``out`` belong
+    to that stream, and the caller orders the inputs before it and what reads
+    ``out`` behind it."""
     T = _torch()
     dev = _device(q, "q")
     if q.dim() != 3 or k.dim() != 4 or k_prefix.dim() != 3:
@@ -114,7 +134,7 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
     if q.dtype not in T.tag or kt not in T.tag:
         raise ValueError(f"queries of {q.dtype} with a cache of {kt}")
     if out is None:
-        out = q.new_empty((n, n_head, hd))
+        out = _empty(T, dev, stream, q, (n, n_head, hd), q.dtype)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (hd > 1 and out.stride(2) != 1):
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device} with a contiguous last dimension")
     if n == 0:
@@ -125,7 +145,7 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
         need = C.c_size_t()
         _lib.check(T.lib.talos_attention_shared_work(dev, n, n_head, n_kv, C.byref(need)))
         size = _work_bytes[key] = need.value
-    work = q.new_empty(size, dtype=T.u8)
+    work = _empty(T, dev, stream, q, size, T.u8)
     os_ = out.stride()
     a = _pack(
         _ATTENTION, dev, T.tag[q.dtype], T.tag[kt], n, n_head, n_kv, hd, prefix, n_slots, rows, q.data_ptr(), qs[0], qs[1],
@@ -143,7 +163,9 @@ def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
     value per row; ``temperature`` 0 is the greedy choice (the lowest index of
     equal logits), ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 keep everything.
     Returns (tokens int32, probs f32), written into ``tokens`` / ``probs`` if given;
-    a row with nothing above -inf gives -1."""
+    a row with nothing above -inf gives -1. With another ``stream`` than the current
+    one, new ones belong to that stream, and the caller orders the inputs before it
+    and what reads them behind it."""
     T = _torch()
     dev = _device(logits, "logits")
     tag = T.tag.get(logits.dtype)
@@ -156,9 +178,9 @@ def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
                          f"{tuple(logits.shape)} with strides {logits.stride()}")
     n, vocab = logits.shape
     if tokens is None:
-        tokens = logits.new_empty(n, dtype=T.i32)
+        tokens = _empty(T, dev, stream, logits, n, T.i32)
     if probs is None:
-        probs = logits.new_empty(n, dtype=T.f32)
+        probs = _empty(T, dev, stream, logits, n, T.f32)
     td = kd = pd = md = 0
     if not isinstance(temperature, (int, float)):
         td, temperature = _vector(T, temperature, "temperature", n, T.f32, dev), 0.0

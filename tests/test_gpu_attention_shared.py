@@ -542,3 +542,57 @@ def test_infinite_values_keep_to_their_dimension(types, bad):
     if q.dtype != torch.float32:
         bound = bound + torch.finfo(q.dtype).eps / 2 * (vmax + ref.abs())
     assert bool(((got.double() - ref).abs() <= bound)[~hit].all())
+
+
+def test_stream_argument_has_memory_of_its_own(monkeypatch):
+    """Calls for two streams, made one after the other on a third, do not share a workspace or
+    an output that was released in between (the launches are left out here)."""
+    import torch
+
+    from talos_b200 import ops
+
+    args = make(8, 8, 2, 64, 500, 50, TYPES[1])
+    talos_b200.attention_shared_dev(*args)
+    torch.cuda.synchronize()
+    works = []
+
+    def launch(a, work, size, stream):
+        works.append((work, stream))
+        return 0
+
+    monkeypatch.setattr(ops._torch().lib, "talos_attention_shared_dev", launch)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    seen = set()
+    for s in (*sides, None):
+        out = talos_b200.attention_shared_dev(*args, stream=None if s is None else s.cuda_stream)
+        assert out.data_ptr() not in seen
+        seen.add(out.data_ptr())
+        del out
+    assert [s for _, s in works] == [*(s.cuda_stream for s in sides), torch.cuda.current_stream().cuda_stream]
+    assert len({w for w, _ in works}) == 3 and not seen & {w for w, _ in works}
+
+
+def test_stream_argument():
+    """The work of different calls on several given streams at once, while the current stream
+    goes on allocating and writing."""
+    import torch
+
+    sets = [make(n, 32, 8, 128, prefix, 200, t, seed=n) for n, prefix, t in
+            ((40, 3000, TYPES[0]), (33, 9000, TYPES[3]), (64, 700, TYPES[1]))]
+    want = [check(a) for a in sets]
+    sides = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for a, s in zip(sets, sides):
+            got.append(talos_b200.attention_shared_dev(*a, stream=s.cuda_stream))
+            junk = [torch.full((1 << k,), float("nan"), device="cuda") for k in range(8, 23)]
+            del junk
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % len(sets)])
+    default = talos_b200.attention_shared_dev(*sets[0], stream=0)
+    with torch.cuda.stream(sides[0]):
+        other = talos_b200.attention_shared_dev(*sets[0], stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(default, want[0]) and torch.equal(other, want[0])

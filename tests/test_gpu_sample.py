@@ -315,3 +315,22 @@ def test_slices_that_are_read_again(settings, dtype, vocab, pad):
 
     lg, rng = rows(44, vocab, 7, getattr(torch, dtype), pad)
     check(lg, rng.random(44).astype(np.float32), *settings)
+
+
+def test_stream_argument():
+    """Results for a given stream are not handed out again while its work may be in flight."""
+    import torch
+
+    lg, rng = rows(40, 50000, 61, torch.float32)
+    u = torch.from_numpy(rng.random(40).astype(np.float32)).cuda()
+    want = talos_b200.sample_dev(lg, u, top_p=0.9)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    first = talos_b200.sample_dev(lg, u, top_p=0.9, stream=side.cuda_stream)
+    at = {x.data_ptr() for x in first}
+    del first
+    fresh = [torch.full((40,), -5, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not at & {x.data_ptr() for x in fresh}
+    got = talos_b200.sample_dev(lg, u, top_p=0.9, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all((x == -5).all() for x in fresh)
