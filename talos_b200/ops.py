@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 from array import array
+from numbers import Integral, Real
 
 import numpy as np
 
@@ -91,6 +92,16 @@ def _vector(T: _Torch, t, name: str, n: int, dtype, dev: int) -> int:
         raise ValueError(f"{name} must be a contiguous [{n}] {dtype} tensor on cuda:{dev}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
+
+
+def _setting(T: _Torch, x, name: str, n: int, dtype, dev: int, kind):
+    """(pointer, number) of a setting that is no plain Python number: a tensor with a value per
+    row, or a number of another kind (numpy's, say)."""
+    if isinstance(x, T.torch.Tensor):
+        return _vector(T, x, name, n, dtype, dev), 0
+    if isinstance(x, kind):
+        return 0, x
+    raise ValueError(f"{name} must be a number or a [{n}] {dtype} tensor, got {x!r}")
 
 
 _work_bytes: dict[tuple[int, int, int, int], int] = {}  # of talos_attention_shared_work
@@ -183,13 +194,13 @@ def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
         probs = _empty(T, dev, stream, logits, n, T.f32)
     td = kd = pd = md = 0
     if not isinstance(temperature, (int, float)):
-        td, temperature = _vector(T, temperature, "temperature", n, T.f32, dev), 0.0
+        td, temperature = _setting(T, temperature, "temperature", n, T.f32, dev, Real)
     if not isinstance(top_k, int):
-        kd, top_k = _vector(T, top_k, "top_k", n, T.i32, dev), 0
+        kd, top_k = _setting(T, top_k, "top_k", n, T.i32, dev, Integral)
     if not isinstance(top_p, (int, float)):
-        pd, top_p = _vector(T, top_p, "top_p", n, T.f32, dev), 0.0
+        pd, top_p = _setting(T, top_p, "top_p", n, T.f32, dev, Real)
     if not isinstance(min_p, (int, float)):
-        md, min_p = _vector(T, min_p, "min_p", n, T.f32, dev), 0.0
+        md, min_p = _setting(T, min_p, "min_p", n, T.f32, dev, Real)
     a = _pack(_SAMPLE, dev, tag, n, vocab, logits.data_ptr(), logits.stride(0), _vector(T, u, "u", n, T.f32, dev), td,
               kd, pd, md, temperature, top_k, top_p, min_p, _vector(T, tokens, "tokens", n, T.i32, dev),
               _vector(T, probs, "probs", n, T.f32, dev))

@@ -334,3 +334,19 @@ def test_stream_argument():
     got = talos_b200.sample_dev(lg, u, top_p=0.9, stream=side.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and all((x == -5).all() for x in fresh)
+
+
+def test_numpy_numbers_as_settings():
+    import torch
+
+    lg, rng = rows(4, 900, 12, torch.float32)
+    u = torch.from_numpy(rng.random(4).astype(np.float32)).cuda()
+    for kind, whole in ((np.float32, np.int64), (np.float64, np.int32), (np.float16, np.uint8)):
+        got = talos_b200.sample_dev(lg, u, temperature=kind(0.5), top_k=whole(50), top_p=kind(0.75), min_p=kind(0.25))
+        want = talos_b200.sample_dev(lg, u, temperature=0.5, top_k=50, top_p=0.75, min_p=0.25)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(TalosError, match="INVALID_ARG"):
+        talos_b200.sample_dev(lg, u, top_k=np.int64(-1))
+    for bad in (dict(top_k=1.5), dict(top_k=np.float32(2)), dict(temperature="1"), dict(min_p=None)):
+        with pytest.raises(ValueError):
+            talos_b200.sample_dev(lg, u, **bad)
