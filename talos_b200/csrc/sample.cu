@@ -131,12 +131,17 @@ __device__ __forceinline__ double sp_weight(float v, const SpScale& q, const dou
 __device__ __forceinline__ u64 sp_fixed(float v, const SpScale& q, const double* pow) {
     return (u64)__double_as_longlong(sp_weight(v, q, pow, 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52
 }
+// The bins: bin of v = half (vmax - v) scale. half is 1/2 where vmax - v can pass the largest
+// f32 (the product with it is exact in the fma), else 1.
+struct SpBins {
+    float vmax, top, half, scale;  // top: half vmax
+};
 // Bin of value v, SP_NB for weight 0. Non-decreasing as v falls: every rounding here is monotone.
-__device__ __forceinline__ float sp_z(float v, float vmax, float scale) {
-    return v == vmax ? 0.f : __fmul_rn(__fsub_rn(vmax, v), scale);
+__device__ __forceinline__ float sp_z(float v, const SpBins& g) {
+    return v == g.vmax ? 0.f : __fmul_rn(__fmaf_rn(-g.half, v, g.top), g.scale);
 }
-__device__ __forceinline__ int sp_bin(float v, float vmax, float scale) {
-    const float z = sp_z(v, vmax, scale);
+__device__ __forceinline__ int sp_bin(float v, const SpBins& g) {
+    const float z = sp_z(v, g);
     return z < (float)SP_NB ? (int)z : SP_NB;  // NaN (-inf at a scale of 0) gives SP_NB
 }
 
@@ -281,7 +286,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     // SP_CAP and took 193,000 clocks instead of 85,000 (64 rows with top-p: 105 -> 63 us).
     // (1e30: logits closer than 1e-27 to each other all lie in bin 0, where an infinite
     // scale would leave the maximum alone.)
-    const float scale = fmaxf((float)inv_t * SP_PER_NAT, fminf((float)(SP_NB - 1) / (vmax - vmin), 1e30f));
+    const float half = vmax < INFINITY && !(vmax - vmin < INFINITY) ? 0.5f : 1.f;
+    const float per_nat = SP_PER_NAT / half;
+    const SpBins bins{vmax, half * vmax, half,
+                      fmaxf((float)inv_t * per_nat,
+                            fminf((float)(SP_NB - 1) / fmaf(-half, vmin, half * vmax), 1e30f))};
     const double min_w = (double)minp * SP_ONE;
 
     auto zero_hist = [&]() {
@@ -335,7 +344,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             case SP_WEIGH:
                 zero_hist();
                 each([&](float v, uint32_t) {
-                    const int b = sp_bin(v, vmax, scale);
+                    const int b = sp_bin(v, bins);
                     if (b < SP_NB) {
                         atomicAdd(&s.cnt[b], 1u);
                         if (c.op == SP_WEIGH) add_hist(b, sp_fixed(v, q, s.pow));
@@ -346,7 +355,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             case SP_GATHER_BINS: {
                 const float z0 = (float)c.b0, z1 = (float)(c.b1 + 1);  // b0 <= bin <= b1
                 each([&](float v, uint32_t i) {
-                    const float z = sp_z(v, vmax, scale);
+                    const float z = sp_z(v, bins);
                     if (z >= z0 && z < z1) gather(sp_key(v, i));
                 });
                 hand_over();
@@ -355,14 +364,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             case SP_GATHER_KEYS:
                 each([&](float v, uint32_t i) {
                     const u64 k = sp_key(v, i);
-                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, scale) < SP_NB) gather(k);
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, bins) < SP_NB) gather(k);
                 });
                 hand_over();
                 break;
             case SP_RANGE: {
                 u64 lo = ~0ull, hi = 0ull;
                 each([&](float v, uint32_t i) {
-                    if (sp_bin(v, vmax, scale) == c.b0) {
+                    if (sp_bin(v, bins) == c.b0) {
                         const u64 k = sp_key(v, i);
                         lo = k < lo ? k : lo;
                         hi = k > hi ? k : hi;
@@ -391,7 +400,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
                 zero_hist();
                 each([&](float v, uint32_t i) {
                     const u64 k = sp_key(v, i);
-                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, vmax, scale) < SP_NB) {
+                    if (k >= c.k0 && k <= c.k1 && sp_bin(v, bins) < SP_NB) {
                         const int b = (int)((k - c.k0) >> c.shift);
                         atomicAdd(&s.cnt[b], 1u);
                         add_hist(b, sp_fixed(v, q, s.pow));
@@ -402,7 +411,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
             case SP_SUM_MIN: {
                 u64 sum = 0;
                 each([&](float v, uint32_t) {
-                    if (sp_bin(v, vmax, scale) < SP_NB) {
+                    if (sp_bin(v, bins) < SP_NB) {
                         if (sp_weight(v, q, s.pow, 0.0) >= min_w) sum += sp_fixed(v, q, s.pow);
                     }
                 });
@@ -571,7 +580,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(const __grid_constant_
     const bool sum_known = !k_active && !count_only;
     if (minp > 0.f && (sum_known || !(topp < 1.f))) {
         // w < m beyond -ln m nats; one bin more covers the roundings of both
-        const float zb = -logf(minp) * (scale / (float)inv_t) + 2.0f;
+        const float zb = -logf(minp) * (half * bins.scale / (float)inv_t) + 2.0f;
         const int b = zb < (float)(SP_NB - 1) ? (int)zb : SP_NB - 1;
         if (b < bcut) {
             __syncthreads();

@@ -350,3 +350,17 @@ def test_numpy_numbers_as_settings():
     for bad in (dict(top_k=1.5), dict(top_k=np.float32(2)), dict(temperature="1"), dict(min_p=None)):
         with pytest.raises(ValueError):
             talos_b200.sample_dev(lg, u, **bad)
+
+
+@pytest.mark.parametrize("t", [1e37, 1e38, 3e38, float("inf")])
+def test_ranges_beyond_the_largest_float(t):
+    """Logits further apart than the largest f32, at temperatures that leave them weights."""
+    import torch
+
+    rng = np.random.default_rng(6)
+    x = np.stack([np.linspace(-3.4e38, 3.4e38, 3000), rng.uniform(-3e38, 3e38, 3000), rng.uniform(-3e38, 1e31, 3000),
+                  np.where(np.arange(3000) % 3, 3.0e38, -3.4028234663852886e38)]).astype(np.float32)
+    x[1, ::7] = -np.inf
+    u = np.array([0.93, 0.41, 0.77, 0.999], np.float32)
+    for kw in (dict(), dict(k=700, p=0.7), dict(p=0.999), dict(m=0.2), dict(k=3), dict(k=900, m=0.3)):
+        check(torch.from_numpy(x).cuda(), u, t=t, **kw)
