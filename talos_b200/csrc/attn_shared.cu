@@ -186,11 +186,6 @@ __device__ __forceinline__ void as_ld32(uint32_t t, float* v) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(t));
 }
-__device__ __forceinline__ void as_ld8(uint32_t t, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(t));
-}
 __device__ __forceinline__ void as_st8(uint32_t t, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -266,10 +261,6 @@ __device__ __forceinline__ void as_split(float a, float b, uint32_t& hi, uint32_
     const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = as_pack<false>(a - f.x, b - f.y);
-}
-__device__ __forceinline__ void as_split_bf(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = as_pack<true>(a, b);
-    lo = as_pack<true>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 // The same split of a pair whose hi keeps 10 mantissa bits by truncation (exact in
 // f16 for |x| in its normal range; below it both parts round): fewer conversions.
@@ -1339,6 +1330,9 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
 }
 
 cudaError_t launch_attn_shared(AttnSharedArgs a, int q_type, int kv_type, void* work, int sms, cudaStream_t s) {
+    // the 16-bit caches' copies know neither rows that start behind the slot's first nor a
+    // prefix that ends before its map does
+    if ((a.slot_row0 || a.prefix_dev) && as_mode(q_type, kv_type) != 0) return cudaErrorInvalidValue;
     const size_t cta = as_grid(a.n, a.group, sms);
     a.part_ml = (float2*)work;
     a.part_o = (float4*)((uint8_t*)work + cta * 2 * AS_ROWS * 8);

@@ -72,7 +72,7 @@ struct AttnSharedArgs {
     const int32_t* lens;   // suffix rows of each sequence
     const int32_t* slots;  // its slot (null: sequence i in slot i)
     float scale;
-    // batched steps: the sequence count and the prefix length in device memory (n and
+    // batched steps (f32 queries and cache): the sequence count and the prefix length in device memory (n and
     // prefix are then their largest values), positions instead of lengths (the
     // suffix has pos + 1 - prefix rows), suffix rows stored from row `prefix` of
     // the slot (slot_row0 = 1), error bits for a wait that ran out
