@@ -301,7 +301,8 @@ talos_status talos_generate_batch_sample(talos_ctx* ctx, const uint32_t* tokens,
  * on). Takes the memory of
  * one more slot, from the first call to the release of the slots. The attention's
  * scores and weights are exact to about 22 bits, like the f32 path's own roundings;
- * results with and without sharing differ in their last bits. Under tensor parallelism
+ * results with and without sharing differ in their last bits. It pays from some hundred
+ * shared rows on: behind a prefix of 64 rows a step was up to 11 % slower with it. Under tensor parallelism
  * every rank makes the call. No reference counterpart.
  */
 talos_status talos_batch_share(talos_ctx* ctx, int slot, size_t n);
@@ -519,8 +520,8 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * and zeros where there is no key at all, or none whose score in f32 is above -inf
  * (such a key has no weight beside others). The prefix is read once for all
  * sequences of a row tile (128 / (n_head / n_head_kv) of them) instead of once
- * per sequence. Rows behind lens[i], and slots that no sequence names, are not
- * read. Types (q and out, cache): F32 with F32 (the reference's cache) or F16,
+ * per sequence. What lies behind lens[i] changes nothing (the rest of a tile of a
+ * named slot may be read along); slots that no sequence names are not read. Types (q and out, cache): F32 with F32 (the reference's cache) or F16,
  * F16 with F16, BF16 with BF16; f32 queries get f32 accuracy on the tensor
  * cores. head_dim up to 128, a multiple of 8 (4 where all is F32); n_head at
  * most 128 times n_head_kv; n up to 1024. UNSUPPORTED beyond 2^30 tiles of 64 keys (of
@@ -539,7 +540,9 @@ talos_status talos_sample(const float* logits, size_t n, float u, float temperat
  * wait ran out are NaN. f32 accuracy: q keeps 22 bits per element (of its row's largest
  * element), the weights 22 bits, an element of an f32 cache 22 bits or 2^-39 of the
  * largest element among the 64 rows of its tile. 16-bit types: the weights are rounded
- * to the type (half a step of 2^-11 or 2^-8 each) and summed as rounded, the rest is f32.
+ * to the type (half a step of 2^-11 or 2^-8 each) and summed as rounded, the rest is f32
+ * (the tensor core's sums of 16 tiles at a time lose about 1.5e-5 of themselves). An output
+ * has therefore 1.3 to 1.4 times the error of one from unrounded weights.
  * No reference counterpart (the reference decodes one sequence at a time).
  */
 typedef struct talos_attention_shared_args {

@@ -54,13 +54,12 @@
 //    the products of its neighbours. Tiles that end early take fewer of both. The
 //    copies bring along the rows behind a suffix's last key, which may hold anything:
 //    the PV warp clears those V rows that its product reads.
-// Bound: HBM (the keys once) up to one row tile; above, the exponentials and the
-// tensor cores. Measured: 64 sequences, 64 / 8 heads of 128, bf16, 32768 shared and up to
-// 1024 own positions 148-153 us, 0.47 PFLOP/s (2,300 clocks a dense tile,
-// where its products take 1,024); 32 sequences, f32 queries and f16 cache, 8192 and up
-// to 512, 46 us, 1.5 TB/s of keys once (suffix tiles: the latencies from S to O);
-// 32 sequences, 32 / 8 heads, f32, 1024 and up to 256, 34 us (the f32 tiles'
-// conversion).
+// Bound: the latencies between the roles of the one CTA an SM. Measured: 64 sequences,
+// 64 / 8 heads of 128, bf16, 32768 shared and up to 1024 own positions 155-162 us, 0.44
+// PFLOP/s (2,300 clocks a dense tile; its exponentials and its products would take 1,024
+// each, side by side); 32 sequences, f32 queries and f16 cache, 8192 and up to 512, 43-48
+// us, 1.5 TB/s of keys once (suffix tiles: from S to O); 32 sequences, 32 / 8 heads, f32,
+// 1024 and up to 256, 33-35 us (the f32 tiles' conversion).
 //
 // Every wait is bounded; on expiry a CTA flag makes all roles run on without
 // waiting or multiplying, and the rows come out as NaN.
@@ -1305,8 +1304,11 @@ static cudaError_t as_launch(AttnSharedArgs a, int sms, cudaStream_t s) {
         if (e == cudaSuccess) e = as_map(&maps.v, type, es, !C::KF32, a.v, 4, d, st, box);
     }
     if (e != cudaSuccess) return e;
-    // Few tiles per (row tile, kv head): one CTA each, and no partials to add. A
-    // tile takes a CTA about 1 us with its latencies, the second kernel about 3.
+    // Few tiles per (row tile, kv head): one CTA each, and no partials to add. Measured with
+    // 4 sequences, 32 / 8 heads of 128 and 1, 2, 3, 4 tiles of a prefix, one CTA each against
+    // all CTAs and the second kernel: bf16 9.3 / 10.3 / 12.3 / 14.4 us against 10.3 / 12.3 /
+    // 12.3 / 12.3; f32 11.1 / 14.2 / 16.4 / 18.5 against 12.3 / 14.4 / 14.4 / 14.4. So it gains
+    // up to two tiles and costs 2 to 4 us at the four it goes to.
     const long long most = (a.prefix + C::KT - 1) / C::KT +
                            (long long)(a.n < spt ? a.n : spt) * ((a.slot_len + C::KT - 1) / C::KT);
     a.whole = !a.prefix_dev && most <= 4 && (long long)R * a.n_kv <= 0x7fffffff;

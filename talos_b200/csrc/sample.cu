@@ -19,9 +19,11 @@
 // the third power (|r| <= 1/2: the fourth is below 9e-15), nine f64 operations where
 // exp() took about a hundred instructions (64 rows of 128256: 117 -> 99 us).
 //
-// Bound: the weighing pass (about 50 instructions a logit for the exact weight), then
-// the chain of phases; over the kernel the issue slots are 42 % busy. 64 rows of 128256 f32: plain temperature 48 us (0.69 TB/s), top-p 61, top-k
-// 35; 32 rows of 32000 with top-p 27 us; one row of 32000 14 us.
+// Bound: the weighing pass (about 50 instructions and two or three shared-memory atomics a
+// logit for the exact weight), then the chain of phases, most of it in the leading CTA alone;
+// over the kernel the issue slots are 42 % busy. 64 rows of 128256 f32: plain temperature
+// 48 us (0.69 TB/s), top-p 62, top-k 35, mixed settings 58; 32 rows of 32000 with top-p 28
+// us; one row of 32000 14-15 us.
 //
 // Structure: a cluster of 1 .. 8 CTAs takes a row; each CTA keeps its slice in
 // shared memory, so the row is read from HBM once. No sort of the row: a

@@ -169,7 +169,7 @@ def attention_shared_dev(q, k_prefix, v_prefix, k, v, slots, lens, out=None, sca
 
 def sample_dev(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, probs=None, stream=None):
     """talos_sample_dev: the token of each row of ``logits`` ([n, vocab] or [vocab],
-    f32 / f16 / bf16, any row stride) for the random numbers ``u`` ([n] f32 in
+    f32 / f16 / bf16, rows any stride of at least vocab apart) for the random numbers ``u`` ([n] f32 in
     [0, 1)). The settings are numbers, or [n] tensors (f32; top_k int32) with one
     value per row; ``temperature`` 0 is the greedy choice (the lowest index of
     equal logits), ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 keep everything.
