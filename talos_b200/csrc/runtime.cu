@@ -2147,7 +2147,8 @@ static talos_status check_slot_pos(talos_ctx* c, uint32_t token, size_t pos) {
     return TALOS_OK;
 }
 
-// Positions from .. end - 1 of slot are about to be written by steps.
+// Positions from .. end - 1 of slot are about to be written by steps: what lies behind them
+// is older then.
 static void slot_written(talos_ctx* c, int slot, size_t from, size_t end) {
     SlotRows& r = c->brows[slot];
     if (!c->bprefix) {
@@ -2155,7 +2156,7 @@ static void slot_written(talos_ctx* c, int slot, size_t from, size_t end) {
         return;
     }
     if (r.same != c->bprefix) r.same = r.low = r.to = c->bprefix;
-    if (from <= r.to) r.to = std::max(r.to, end);
+    if (from <= r.to) r.to = end;
 }
 
 // Rows were copied between slots.

@@ -322,3 +322,28 @@ def test_slots_that_may_be_named_while_a_prefix_is_shared():
     with pytest.raises(TalosError, match="INVALID_ARG"):
         m.batch_share(0, 10)
     m.close()
+
+
+def test_rows_behind_a_newly_written_position_are_older():
+    """The slot that the prefix came from goes on with other tokens in the middle of its rows:
+    the older rows behind them do not extend the prefix, the new ones do."""
+    data = tiny_model(gguf.Q8_0)
+    a = list(prompt(40, 4096, 26))
+    m = load(data, 2)
+    m.prefill_slot(0, a)
+    m.batch_share(0, 25)
+    m.generate_batch_greedy([7, 8], [25, 25], 1)
+    with pytest.raises(TalosError, match="INVALID_ARG"):
+        m.batch_share(0, 40)
+    m.batch_share(0, 26)
+    want = oracle_logits(data, a[:25] + [7, 9])[-1]
+    assert np.max(np.abs(m.forward_batch([9, 9], [26, 26]) - want)) <= 1e-3
+    # fed once more as it was, a position leaves nothing behind it in doubt
+    m.batch_share(0, 0)
+    m.prefill_slot(0, a)
+    m.batch_share(0, 25)
+    m.prefill_slot(0, a[39:], 39)
+    m.batch_share(0, 40)
+    want = oracle_logits(data, a + [9])[-1]
+    assert np.max(np.abs(m.forward_batch([9, 9], [40, 40]) - want)) <= 1e-3
+    m.close()
